@@ -181,7 +181,8 @@ def prepare(case, seed):
               case["cols"], case["bits"], case["group"])
     if own:
         if op in ("linear", "cached"):
-            s["layer"] = _engine().Linear8.from_tensors(s["w"], s["b"], gate=case["gate"])
+            s["layer"] = _engine().Linear8.from_tensors(s["w"], s["b"], gate=case["gate"],
+                                                        segments=case["frames"] if op == "cached" else 1)
     return s
 
 
