@@ -124,6 +124,20 @@ SIGNATURES = {
     "dn_conv2d_output_size": (_I, [_P, _I, _I, _IP, _IP]),
     "dn_conv2d_forward": (_I, [_P, _P, _I, _I, _I, _I, _P, _P]),
     "dn_conv2d_sync": (_I, [_P, _P]),
+    # include/denoiser_b200_quant.h
+    "dn_launch_cache_write": (_I, [_P, _I, _I64, _I64, _I, _P, _I64, _P, _I64, _P, _I64, _I, _I, _P, _P]),
+    "dn_launch_cache_read_rows": (_I, [_P, _I64, _P, _I64, _I, _I, _I, _P, _I64, _I64, _P, _I, _I64, _P, _P]),
+    "dn_launch_cache_read_pages": (_I, [_P, _I64, _P, _I64, _I, _I, _I, _I64, _P, _I64, _I64, _P, _I, _I64, _P, _I,
+                                        _I64, _I64, _P, _P]),
+    "dn_linear8_create": (_I, [_P, _c.c_char_p, _c.c_char_p, _I, _I, _I, _PP]),
+    "dn_linear8_create_device": (_I, [_P, _I, _I64, _P, _I, _I, _I, _I, _I, _P, _PP]),
+    "dn_linear8_destroy": (_I, [_P]),
+    "dn_linear8_info": (_I, [_P, _IP, _IP, _IP, _IP]),
+    "dn_linear8_workspace": (_I, [_P, _I64, _I, _I64P]),
+    "dn_linear8_forward": (_I, [_P, _P, _I, _I64, _I64, _P, _I, _I64, _P, _I64, _P]),
+    "dn_linear8_forward_nchw": (_I, [_P, _P, _I, _I, _I, _P, _P, _I64, _P]),
+    "dn_linear8_forward_cached": (_I, [_P, _P, _I64, _P, _I64, _I64, _I64P, _I, _I64, _P, _I, _I64, _P]),
+    "dn_linear8_sync": (_I, [_P, _P]),
     # include/denoiser_b200_io.h
     "dn_image_probe": (_I, [_c.c_char_p, _IP, _IP, _IP]),
     "dn_image_read": (_I, [_c.c_char_p, _P, _I, _I, _I]),

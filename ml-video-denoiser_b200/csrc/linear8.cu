@@ -1,0 +1,458 @@
+// Linear8: y[m, n] = s_x[m] s_w[n] sum_k q_x[m, k] q_w[n, k] + bias[n] in 8-bit
+// integers (include/denoiser_b200_quant.h has the definition).
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <memory>
+#include <new>
+#include <string>
+#include <vector>
+
+#include "capi_internal.h"
+#include "denoiser_b200_quant.h"
+#include "launch.cuh"
+#include "quant.cuh"
+#include "row_cache.h"
+#include "status.h"
+
+namespace dnb {
+namespace {
+
+constexpr int kMaxSegments = 16;
+constexpr int kMaxK = 131072;  // 127 * 127 * 131072 < 2^31
+
+struct ProductArgs {
+    const int8_t* a;   // codes of the tokens
+    int64_t lda;
+    const float* as;   // a scale per code row
+    int64_t arow[kMaxSegments];  // first code row of each segment
+    int segs, seg_c, seg_p;      // segments, their channels, their bytes in a weight row
+    const int8_t* w;   // [cout][ldw]
+    int64_t ldw;
+    const float* ws;
+    const float* bias; // null: none
+    int cout, n_out, gate;
+    int64_t rows;
+    void* out;
+    int64_t ldo;       // row stride of out; planes: pixels of a plane
+    int planes;        // out[(m / ldo) * n_out + c][m % ldo] instead of out[m][c]
+};
+
+__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+
+template <typename T>
+__global__ void __launch_bounds__(256) product_kernel(const __grid_constant__ ProductArgs a) {
+    pdl_trigger();
+    pdl_wait();
+    __shared__ int sa[64][17], sb[2][64][17];
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const int64_t m0 = static_cast<int64_t>(blockIdx.x) * 64;
+    const int c0 = blockIdx.y * 64;
+    const int halves = a.gate ? 2 : 1;
+    float y[2][4][4] = {};
+    for (int t = 0; t < a.segs; ++t) {
+        int acc[2][4][4] = {};
+        for (int k0 = 0; k0 < a.seg_p; k0 += 64) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < 64 * 16; i += 256) {
+                const int r = i >> 4, k = k0 + (i & 15) * 4;
+                const int64_t m = m0 + r;
+                sa[r][i & 15] = (m < a.rows && k < a.seg_c)
+                                    ? *reinterpret_cast<const int*>(a.a + (a.arow[t] + m) * a.lda + k)
+                                    : 0;
+                for (int h = 0; h < halves; ++h) {
+                    const int c = c0 + r;
+                    sb[h][r][i & 15] = (c < a.n_out && k < a.seg_p)
+                                           ? *reinterpret_cast<const int*>(a.w + static_cast<int64_t>(c + h * a.n_out) * a.ldw +
+                                                                           t * a.seg_p + k)
+                                           : 0;
+                }
+            }
+            __syncthreads();
+            for (int k = 0; k < 16; ++k)
+                for (int h = 0; h < halves; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            acc[h][i][j] = __dp4a(sa[ty * 4 + i][k], sb[h][tx * 4 + j][k], acc[h][i][j]);
+        }
+        for (int i = 0; i < 4; ++i) {
+            const int64_t m = m0 + ty * 4 + i;
+            const float s = m < a.rows ? a.as[a.arow[t] + m] : 0.f;
+            for (int h = 0; h < halves; ++h)
+                for (int j = 0; j < 4; ++j) y[h][i][j] = fmaf(static_cast<float>(acc[h][i][j]), s, y[h][i][j]);
+        }
+    }
+    T* out = static_cast<T*>(a.out);
+    for (int i = 0; i < 4; ++i) {
+        const int64_t m = m0 + ty * 4 + i;
+        if (m >= a.rows) continue;
+        for (int j = 0; j < 4; ++j) {
+            const int c = c0 + tx * 4 + j;
+            if (c >= a.n_out) continue;
+            float v = fmaf(y[0][i][j], a.ws[c], a.bias ? a.bias[c] : 0.f);
+            if (a.gate) v *= fmaf(y[1][i][j], a.ws[c + a.n_out], a.bias ? a.bias[c + a.n_out] : 0.f);
+            const int64_t img = a.planes ? m / a.ldo : 0;
+            put(out + (a.planes ? (img * a.n_out + c) * a.ldo + (m - img * a.ldo) : m * a.ldo + c), v);
+        }
+    }
+}
+
+// Codes and scales of the pixels of NCHW planes: a thread per pixel.
+__global__ void __launch_bounds__(256) quantise_planes_kernel(const __half* __restrict__ x, int64_t rows, int K, int64_t hw,
+                                                              uint8_t* __restrict__ codes, int64_t ldc,
+                                                              float* __restrict__ scales) {
+    using Q = QuantOf<__half>;
+    pdl_trigger();
+    pdl_wait();
+    const int64_t m = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const bool live = m < rows;
+    const int64_t img = live ? m / hw : 0;
+    const __half* src = x + (img * K * hw + (live ? m - img * hw : 0));
+    uint32_t mag = 0;
+    for (int k = 0; k < K; ++k) mag = max(mag, static_cast<uint32_t>(__half_as_ushort(src[k * hw])) & 0x7fffu);
+    const GroupScale g = group_scale<__half>(mag, 127.f);
+    const bool fix = __any_sync(0xffffffffu, g.fix != 0.f);
+    if (!live) return;
+    for (int k = 0; k < K; k += 8) {
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (k + i < K) w[i >> 1] |= static_cast<uint32_t>(__half_as_ushort(src[(k + i) * hw])) << ((i & 1) * 16);
+        *reinterpret_cast<uint2*>(codes + m * ldc + k) = codes8<__half>(Q::Vec{make_uint4(w[0], w[1], w[2], w[3])}, g, fix);
+    }
+    scales[m] = g.s;
+}
+
+__global__ void bias_kernel(const void* b, int dtype, float* out, int n) {
+    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    if (i < n) out[i] = dtype == 1 ? __half2float(static_cast<const __half*>(b)[i]) : static_cast<const float*>(b)[i];
+}
+
+struct DeviceScope {
+    int prev = -1;
+    explicit DeviceScope(int d) {
+        cudaGetDevice(&prev);
+        if (prev != d) cudaSetDevice(d);
+    }
+    ~DeviceScope() {
+        int cur = -1;
+        cudaGetDevice(&cur);
+        if (prev >= 0 && cur != prev) cudaSetDevice(prev);
+    }
+};
+
+int64_t round16(int64_t v) { return (v + 15) / 16 * 16; }
+
+}  // namespace
+}  // namespace dnb
+
+using namespace dnb;
+
+struct dn_linear8 {
+    int device = 0;
+    int cout = 0, cin = 0, gate = 0, segs = 1, seg_c = 0, seg_p = 0;
+    int64_t ldw = 0;
+    uint8_t* arena = nullptr;  // weight codes, scales, bias, error word
+    int8_t* w = nullptr;
+    float* ws = nullptr;
+    float* bias = nullptr;  // null: none
+    uint32_t* err = nullptr;
+    int n_out() const { return gate ? cout / 2 : cout; }
+};
+
+namespace {
+
+int check_shape(int64_t cout, int64_t cin, int gate, int segments) {
+    if (cout <= 0 || cin <= 0) return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_create: empty weight");
+    if (cin > kMaxK) return dn_fail(DN_ERR_UNSUPPORTED, "dn_linear8_create: more than 131072 input channels");
+    if (cout > (1 << 20)) return dn_fail(DN_ERR_UNSUPPORTED, "dn_linear8_create: more than 2^20 output channels");
+    if (gate && cout % 2) return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_create: the gate needs an even number of channels");
+    if (segments < 1 || cin % segments)
+        return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_create: segments does not divide the input channels");
+    if (segments > kMaxSegments) return dn_fail(DN_ERR_UNSUPPORTED, "dn_linear8_create: more than 16 segments");
+    return DN_OK;
+}
+
+// The layer's own copy of the weight, quantised; the current device is the layer's.
+cudaError_t lay_out(dn_linear8* L, const void* weight, int dtype, int64_t ldw, const void* bias, cudaStream_t s, int& rc) {
+    const int64_t codes = L->cout * L->ldw;
+    const size_t total = static_cast<size_t>(round16(codes)) + static_cast<size_t>(L->cout) * 8 + 16;
+    cudaError_t e = cudaMalloc(&L->arena, total);
+    if (e != cudaSuccess) return e;
+    L->w = reinterpret_cast<int8_t*>(L->arena);
+    L->ws = reinterpret_cast<float*>(L->arena + round16(codes));
+    float* b = L->ws + L->cout;
+    L->err = reinterpret_cast<uint32_t*>(b + L->cout);
+    if ((e = cudaMemsetAsync(L->arena, 0, total, s)) != cudaSuccess) return e;
+    uint8_t* dense = L->arena;
+    const bool apart = L->segs > 1 && L->seg_p != L->seg_c;  // segments that are padded one by one
+    if (apart && (e = cudaMalloc(&dense, static_cast<size_t>(L->cout) * L->cin)) != cudaSuccess) return e;
+    rc = launch_cache_write(CacheWrite{weight, dtype, ldw, L->cout, L->cin, nullptr, 0, dense, apart ? L->cin : L->ldw,
+                                       L->ws, L->cout, 8, L->cin, nullptr},
+                            s);
+    for (int t = 0; apart && rc == DN_OK && e == cudaSuccess && t < L->segs; ++t)
+        e = cudaMemcpy2DAsync(L->w + t * L->seg_p, L->ldw, dense + t * L->seg_c, L->cin, L->seg_c, L->cout,
+                              cudaMemcpyDeviceToDevice, s);
+    if (bias && rc == DN_OK && e == cudaSuccess) {
+        bias_kernel<<<(L->cout + 255) / 256, 256, 0, s>>>(bias, dtype, b, L->cout);
+        L->bias = b;
+        e = cudaGetLastError();
+    }
+    const cudaError_t e2 = cudaStreamSynchronize(s);
+    if (apart) cudaFree(dense);
+    return e != cudaSuccess ? e : e2;
+}
+
+int create(const void* weight, int dtype, int64_t ldw, const void* bias, int cout, int cin, int gate, int segments,
+           int device, cudaStream_t s, dn_linear8** out) {
+    std::unique_ptr<dn_linear8> L(new (std::nothrow) dn_linear8);
+    if (!L) return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_create: out of host memory");
+    L->device = device;
+    L->cout = cout;
+    L->cin = cin;
+    L->gate = gate ? 1 : 0;
+    L->segs = segments;
+    L->seg_c = cin / segments;
+    L->seg_p = static_cast<int>(round16(L->seg_c));
+    L->ldw = static_cast<int64_t>(L->seg_p) * segments;
+    int rc = DN_OK;
+    const cudaError_t e = lay_out(L.get(), weight, dtype, ldw, bias, s, rc);
+    if (e != cudaSuccess || rc != DN_OK) {
+        cudaFree(L->arena);
+        return rc != DN_OK ? rc : dn_cuda_fail(e, "dn_linear8_create: upload");
+    }
+    *out = L.release();
+    return DN_OK;
+}
+
+ProductArgs product_args(const dn_linear8* L) {
+    ProductArgs a{};
+    a.segs = L->segs;
+    a.seg_c = L->seg_c;
+    a.seg_p = L->seg_p;
+    a.w = L->w;
+    a.ldw = L->ldw;
+    a.ws = L->ws;
+    a.bias = L->bias;
+    a.cout = L->cout;
+    a.n_out = L->n_out();
+    a.gate = L->gate;
+    return a;
+}
+
+int run_product(const ProductArgs& a, int out_dtype, cudaStream_t s) {
+    const dim3 grid(static_cast<unsigned>((a.rows + 63) / 64), static_cast<unsigned>((a.n_out + 63) / 64));
+    const cudaError_t e = out_dtype == 1 ? launch_pdl(product_kernel<__half>, grid, dim3(256), 0, s, a)
+                                         : launch_pdl(product_kernel<float>, grid, dim3(256), 0, s, a);
+    return e == cudaSuccess ? DN_OK : dn_cuda_fail(e, "dn_linear8: launch");
+}
+
+bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+int check_matrix(const void* p, int dtype, int64_t rows, int64_t ld, int64_t cols, const std::string& what) {
+    if (dtype != 0 && dtype != 1) return dn_fail_str(DN_ERR_DTYPE, what + ": dtype must be 0 (FP32) or 1 (FP16)");
+    if (rows < 0 || rows >= (1LL << 31)) return dn_fail_str(DN_ERR_INVALID_ARG, what + ": rows outside [0, 2^31)");
+    if (rows == 0) return DN_OK;
+    if (!p) return dn_fail_str(DN_ERR_INVALID_ARG, what + ": null pointer");
+    if (!aligned_to(p, dtype == 1 ? 2 : 4)) return dn_fail_str(DN_ERR_INVALID_ARG, what + ": misaligned pointer");
+    if (ld < cols && rows > 1) return dn_fail_str(DN_ERR_INVALID_ARG, what + ": row stride is less than a row");
+    return DN_OK;
+}
+
+int64_t workspace_bytes_of(const dn_linear8* L, int64_t rows) { return rows * (round16(L->cin) + 4); }
+
+int check_workspace(const dn_linear8* L, int64_t rows, const void* ws, int64_t bytes, const char* what) {
+    const int64_t need = workspace_bytes_of(L, rows);
+    if (need == 0) return DN_OK;
+    if (!ws || bytes < need)
+        return dn_fail_str(DN_ERR_INVALID_ARG, std::string(what) + ": the workspace holds " + std::to_string(ws ? bytes : 0) +
+                                                   " bytes, " + std::to_string(need) + " are needed");
+    if (!aligned_to(ws, 16)) return dn_fail_str(DN_ERR_INVALID_ARG, std::string(what) + ": misaligned workspace");
+    return DN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dn_linear8_create(const dn_weights* store, const char* weight_name, const char* bias_name, int gate, int segments,
+                      int device, dn_linear8** out) {
+    if (!store || !weight_name || !out) return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_create: null argument");
+    *out = nullptr;
+    try {
+        const HostWeights& hw = *store->hw;
+        if (!hw.contains(weight_name)) return dn_fail_str(DN_ERR_NOT_FOUND, std::string("weight not found: ") + weight_name);
+        if (bias_name && !hw.contains(bias_name))
+            return dn_fail_str(DN_ERR_NOT_FOUND, std::string("weight not found: ") + bias_name);
+        const auto& sh = hw.entry(weight_name).shape;
+        if (!(sh.size() == 2 || (sh.size() == 4 && sh[2] == 1 && sh[3] == 1)))
+            return dn_fail(DN_ERR_FORMAT, "dn_linear8_create: weight must be (Cout, Cin) or (Cout, Cin, 1, 1)");
+        DN_TRY(check_shape(sh[0], sh[1], gate, segments));
+        const int cout = static_cast<int>(sh[0]), cin = static_cast<int>(sh[1]);
+        const std::vector<float> w = hw.to_f32(weight_name);
+        std::vector<float> b;
+        if (bias_name) {
+            b = hw.to_f32(bias_name);
+            if (static_cast<int64_t>(b.size()) != cout) return dn_fail(DN_ERR_FORMAT, "dn_linear8_create: bias size");
+        }
+        DeviceScope scope(device);
+        float* dev = nullptr;
+        const size_t nw = w.size() * 4, nb = b.size() * 4;
+        cudaError_t e = cudaMalloc(&dev, nw + nb);
+        if (e == cudaSuccess) e = cudaMemcpy(dev, w.data(), nw, cudaMemcpyHostToDevice);
+        if (e == cudaSuccess && nb) e = cudaMemcpy(dev + w.size(), b.data(), nb, cudaMemcpyHostToDevice);
+        int rc = e == cudaSuccess ? create(dev, 0, cin, nb ? dev + w.size() : nullptr, cout, cin, gate, segments, device,
+                                           nullptr, out)
+                                  : dn_cuda_fail(e, "dn_linear8_create: upload");
+        cudaFree(dev);
+        return rc;
+    } catch (const std::exception& ex) {
+        return dn_fail_str(DN_ERR_FORMAT, ex.what());
+    }
+}
+
+int dn_linear8_create_device(const void* weight, int dtype, int64_t ldw, const void* bias, int cout, int cin, int gate,
+                             int segments, int device, void* stream, dn_linear8** out) {
+    if (!out) return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_create_device: null argument");
+    *out = nullptr;
+    DN_TRY(check_shape(cout, cin, gate, segments));
+    DN_TRY(check_matrix(weight, dtype, cout, ldw, cin, "dn_linear8_create_device"));
+    if (!aligned_to(bias, dtype == 1 ? 2 : 4))
+        return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_create_device: misaligned bias");
+    DeviceScope scope(device);
+    return create(weight, dtype, ldw, bias, cout, cin, gate, segments, device, static_cast<cudaStream_t>(stream), out);
+}
+
+int dn_linear8_destroy(dn_linear8* L) {
+    if (!L) return DN_OK;
+    DeviceScope scope(L->device);
+    cudaFree(L->arena);
+    delete L;
+    return DN_OK;
+}
+
+int dn_linear8_info(const dn_linear8* L, int* out_channels, int* in_channels, int* gate, int* segments) {
+    if (!L) return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_info: null layer");
+    if (out_channels) *out_channels = L->n_out();
+    if (in_channels) *in_channels = L->cin;
+    if (gate) *gate = L->gate;
+    if (segments) *segments = L->segs;
+    return DN_OK;
+}
+
+int dn_linear8_workspace(const dn_linear8* L, int64_t rows, int dtype, int64_t* bytes) {
+    if (!L || !bytes) return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_workspace: null argument");
+    if (rows < 0 || rows >= (1LL << 31)) return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_workspace: rows outside [0, 2^31)");
+    if (dtype != 0 && dtype != 1) return dn_fail(DN_ERR_DTYPE, "dn_linear8_workspace: dtype must be 0 (FP32) or 1 (FP16)");
+    *bytes = workspace_bytes_of(L, rows);
+    return DN_OK;
+}
+
+int dn_linear8_forward(dn_linear8* L, const void* x, int dtype, int64_t ldx, int64_t rows, void* out, int out_dtype,
+                       int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream) {
+    const char* name = "dn_linear8_forward";
+    if (!L) return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_forward: null layer");
+    if (L->segs != 1) return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_forward: a layer with segments reads cached rows");
+    DN_TRY(check_matrix(x, dtype, rows, ldx, L->cin, name));
+    DN_TRY(check_matrix(out, out_dtype, rows, ldo, L->n_out(), name));
+    if (rows == 0) return DN_OK;
+    DN_TRY(check_workspace(L, rows, workspace, workspace_bytes, name));
+    DeviceScope scope(L->device);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    ProductArgs a = product_args(L);
+    a.lda = round16(L->cin);
+    auto* codes = static_cast<uint8_t*>(workspace);
+    auto* scales = reinterpret_cast<float*>(codes + rows * a.lda);
+    DN_TRY(launch_cache_write(CacheWrite{x, dtype, ldx, rows, L->cin, nullptr, 0, codes, a.lda, scales, rows, 8, L->cin,
+                                         nullptr},
+                              s));
+    a.a = reinterpret_cast<const int8_t*>(codes);
+    a.as = scales;
+    a.rows = rows;
+    a.out = out;
+    a.ldo = ldo;
+    return run_product(a, out_dtype, s);
+}
+
+int dn_linear8_forward_nchw(dn_linear8* L, const void* input, int N, int H, int W, void* output, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
+    const char* name = "dn_linear8_forward_nchw";
+    if (!L) return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_forward_nchw: null layer");
+    if (L->segs != 1) return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_forward_nchw: a layer with segments reads cached rows");
+    if (N < 0 || H < 0 || W < 0) return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_forward_nchw: negative size");
+    const int64_t hw = static_cast<int64_t>(H) * W;
+    if (hw >= (1LL << 31)) return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_forward_nchw: rows outside [0, 2^31)");
+    const int64_t rows = hw * N;
+    DN_TRY(check_matrix(input, 1, rows, L->cin, L->cin, name));
+    DN_TRY(check_matrix(output, 1, rows, L->n_out(), L->n_out(), name));
+    if (rows == 0) return DN_OK;
+    DN_TRY(check_workspace(L, rows, workspace, workspace_bytes, name));
+    DeviceScope scope(L->device);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    ProductArgs a = product_args(L);
+    a.lda = round16(L->cin);
+    auto* codes = static_cast<uint8_t*>(workspace);
+    auto* scales = reinterpret_cast<float*>(codes + rows * a.lda);
+    const cudaError_t e = launch_pdl(quantise_planes_kernel, dim3(static_cast<unsigned>((rows + 255) / 256)), dim3(256), 0, s,
+                                     static_cast<const __half*>(input), rows, L->cin, hw, codes, a.lda, scales);
+    if (e != cudaSuccess) return dn_cuda_fail(e, "dn_linear8_forward_nchw: quantise launch");
+    a.a = reinterpret_cast<const int8_t*>(codes);
+    a.as = scales;
+    a.rows = rows;
+    a.out = output;
+    a.ldo = hw;
+    a.planes = 1;
+    return run_product(a, 1, s);
+}
+
+int dn_linear8_forward_cached(dn_linear8* L, const void* codes, int64_t ld_codes, const float* scales, int64_t capacity,
+                              int64_t page_rows, const int64_t* pages, int n_pages, int64_t rows, void* out,
+                              int out_dtype, int64_t ldo, void* stream) {
+    const char* name = "dn_linear8_forward_cached";
+    if (!L || !pages) return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_forward_cached: null argument");
+    if (n_pages != L->segs)
+        return dn_fail_str(DN_ERR_INVALID_ARG, std::string(name) + ": " + std::to_string(n_pages) +
+                                                   " pages for a layer of " + std::to_string(L->segs) + " segments");
+    if (capacity < 0 || capacity >= (1LL << 31) || page_rows <= 0 || page_rows >= (1LL << 31) || rows > page_rows)
+        return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_forward_cached: bad cache or page size");
+    if (ld_codes < L->seg_c || ld_codes % 16 || !aligned_to(codes, 16) || !aligned_to(scales, 4))
+        return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_forward_cached: codes rows must be 16-byte aligned and hold a segment");
+    DN_TRY(check_matrix(out, out_dtype, rows, ldo, L->n_out(), name));
+    ProductArgs a = product_args(L);
+    for (int t = 0; t < n_pages; ++t) {
+        if (pages[t] < 0 || pages[t] > (capacity - page_rows) / page_rows || capacity < page_rows)
+            return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_forward_cached: page outside the cache");
+        a.arow[t] = pages[t] * page_rows;
+    }
+    if (rows == 0) return DN_OK;
+    if (!codes || !scales) return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_forward_cached: null cache");
+    DeviceScope scope(L->device);
+    a.a = static_cast<const int8_t*>(codes);
+    a.lda = ld_codes;
+    a.as = scales;
+    a.rows = rows;
+    a.out = out;
+    a.ldo = ldo;
+    return run_product(a, out_dtype, static_cast<cudaStream_t>(stream));
+}
+
+int dn_linear8_sync(dn_linear8* L, void* stream) {
+    if (!L) return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_sync: null layer");
+    DeviceScope scope(L->device);
+    cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return dn_cuda_fail(e, "dn_linear8_sync");
+    uint32_t word = 0;
+    e = cudaMemcpy(&word, L->err, 4, cudaMemcpyDeviceToHost);
+    if (e != cudaSuccess) return dn_cuda_fail(e, "dn_linear8_sync: error word");
+    if (word) {
+        cudaMemset(L->err, 0, 4);
+        return dn_fail_str(DN_ERR_DEVICE, "linear8 kernel reported device error word " + std::to_string(word));
+    }
+    return DN_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,189 @@
+// Quantisation of a group of values to 8 or 4 bits, and its inverse.
+//
+//   s = max(fl32(a * fl32(1 / qmax)), 2^-126), a = max |x_k|;   q_k = nearest(x_k / s), halves to even.
+//
+// The codes are exact: x_k and s are taken as they are, and the quotient is
+// never rounded to the wrong side of a border between two codes.
+//
+//   FP32 rows. q0 = rint(x * fl32(1/s)) is off by at most one, and
+//   r = fma(-q0, s, x) is exact (x - q0 s is a multiple of ulp(s)/2 below
+//   0.51 s), so comparing 2|r| with s settles it.
+//
+//   FP16 rows. x / s = (qmax x / a)(1 + d) with |d| < 2^-22, and qmax x / a
+//   is a quotient of whole numbers (11-bit significands): it is a half, or at
+//   least 2^-19 (relative) away from one. So x * fl32(1/s) is on the right
+//   side but where qmax x / a is a half exactly. Then the sign of
+//   s - a / qmax decides, which fma(s, qmax, -a) gives exactly: scaling 1/s
+//   by 1 -+ 2^-21 moves those products to the side they belong to and no
+//   other one across a border. Where s = a / qmax exactly, the quotient can
+//   be a half, and one correction step, t + fma(-t, s, x) / s, returns it
+//   correctly rounded. This was checked for all pairs of significands; it
+//   costs a multiply and an add per value instead of a division.
+#pragma once
+
+#include <cstdint>
+#include <cuda_fp16.h>
+
+#include "sm100.cuh"
+
+namespace dnb {
+
+constexpr float kTinyScale = 1.17549435e-38f;  // 2^-126
+constexpr float kRint = 12582912.f;            // 1.5 * 2^23: adding it rounds to a whole number, held in the low bits
+
+// One group's scale and what the codes are made with.
+struct GroupScale {
+    float s;
+    float inv;      // 0 for a group that holds a NaN or an infinity
+    float fix;      // fl32(1/s) where the correction step is needed, else 0
+    uint32_t mask;  // all ones, or 0 for such a group: its codes are 0
+};
+
+// Magnitude bits of 8 packed fp16 values / of fp32 values: the unsigned
+// maximum orders finite < infinity < NaN.
+__device__ __forceinline__ uint32_t umax16x2(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+
+template <typename T>
+struct QuantOf;
+
+template <>
+struct QuantOf<__half> {
+    static constexpr bool kF32 = false;
+    struct Vec {  // 8 values
+        uint4 v;
+    };
+    __device__ static __forceinline__ Vec zero() { return Vec{make_uint4(0, 0, 0, 0)}; }
+    __device__ static __forceinline__ Vec load(const __half* p) { return Vec{__ldg(reinterpret_cast<const uint4*>(p))}; }
+    __device__ static __forceinline__ Vec load_some(const __half* p, int n) {  // the first n of 8, any alignment
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) w[i >> 1] |= static_cast<uint32_t>(__half_as_ushort(p[i])) << ((i & 1) * 16);
+        return Vec{make_uint4(w[0], w[1], w[2], w[3])};
+    }
+    __device__ static __forceinline__ uint32_t mag(const Vec& x) {
+        const uint32_t m = 0x7fff7fffu;
+        const uint32_t a = umax16x2(umax16x2(x.v.x & m, x.v.y & m), umax16x2(x.v.z & m, x.v.w & m));
+        return max(a >> 16, a & 0xffffu);
+    }
+    __device__ static __forceinline__ float mag_value(uint32_t bits) {
+        return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+    }
+    __device__ static __forceinline__ void unpack(const Vec& x, float (&f)[8]) { h8_to_f(x.v, f); }
+};
+
+template <>
+struct QuantOf<float> {
+    static constexpr bool kF32 = true;
+    struct Vec {
+        float4 a, b;
+    };
+    __device__ static __forceinline__ Vec zero() {
+        return Vec{make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+    }
+    __device__ static __forceinline__ Vec load(const float* p) {
+        return Vec{__ldg(reinterpret_cast<const float4*>(p)), __ldg(reinterpret_cast<const float4*>(p) + 1)};
+    }
+    __device__ static __forceinline__ Vec load_some(const float* p, int n) {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = i < n ? p[i] : 0.f;
+        return Vec{make_float4(f[0], f[1], f[2], f[3]), make_float4(f[4], f[5], f[6], f[7])};
+    }
+    __device__ static __forceinline__ void unpack(const Vec& x, float (&f)[8]) {
+        f[0] = x.a.x, f[1] = x.a.y, f[2] = x.a.z, f[3] = x.a.w;
+        f[4] = x.b.x, f[5] = x.b.y, f[6] = x.b.z, f[7] = x.b.w;
+    }
+    __device__ static __forceinline__ uint32_t mag(const Vec& x) {
+        float f[8];
+        unpack(x, f);
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
+        return m;
+    }
+    __device__ static __forceinline__ float mag_value(uint32_t bits) { return __uint_as_float(bits); }
+};
+
+template <typename T>
+__device__ __forceinline__ GroupScale group_scale(uint32_t mag, float qmax) {
+    const float a = QuantOf<T>::mag_value(mag);
+    GroupScale g;
+    g.mask = a <= 3.402823466e38f ? 0xffffffffu : 0u;
+    g.s = g.mask ? fmaxf(__fmul_rn(a, qmax == 127.f ? 1.f / 127.f : 1.f / 7.f), kTinyScale) : __uint_as_float(0x7fc00000u);
+    g.inv = g.mask ? __frcp_rn(g.s) : 0.f;
+    g.fix = 0.f;
+    if (!QuantOf<T>::kF32) {
+        const float d = fmaf(g.s, qmax, -a);  // exact sign of s - a / qmax
+        if (d == 0.f)
+            g.fix = g.inv;
+        else
+            g.inv *= d > 0.f ? 1.f - 4.76837158e-7f : 1.f + 4.76837158e-7f;
+    }
+    return g;
+}
+
+// Codes of 8 values, one a byte. `fix`: whether any lane of the warp has
+// g.fix != 0 (FP16 only; warp-uniform).
+template <typename T>
+__device__ __forceinline__ uint2 codes8(const typename QuantOf<T>::Vec& x, const GroupScale& g, bool fix) {
+    float f[8];
+    QuantOf<T>::unpack(x, f);
+    uint32_t u[8];
+    if (QuantOf<T>::kF32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float v = g.mask ? f[i] : 0.f;  // a group that is not finite: codes 0
+            const float q0 = __fsub_rn(__fmaf_rn(v, g.inv, kRint), kRint);
+            const float r = __fmaf_rn(-q0, g.s, v);
+            const float r2 = 2.f * fabsf(r);  // exact; infinite for no finite group (r < 0.51 s)
+            const int q = static_cast<int>(q0);
+            const bool over = r2 > g.s || (r2 == g.s && (q & 1));
+            u[i] = static_cast<uint32_t>(over ? q + (r > 0.f ? 1 : -1) : q);
+        }
+    } else {
+        const float2 inv2 = make_float2(g.inv, g.inv), zero2 = make_float2(0.f, 0.f);
+        const float2 magic2 = make_float2(kRint, kRint), one2 = make_float2(1.f, 1.f);
+        const float2 ns2 = make_float2(-g.s, -g.s), fix2 = make_float2(g.fix, g.fix);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 v = make_float2(f[2 * i], f[2 * i + 1]);
+            float2 t = ffma2(v, inv2, zero2);
+            if (fix) t = ffma2(ffma2(t, ns2, v), fix2, t);
+            t = ffma2(t, one2, magic2);
+            u[2 * i] = __float_as_uint(t.x);
+            u[2 * i + 1] = __float_as_uint(t.y);
+        }
+    }
+    uint2 w;
+    w.x = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410) & g.mask;
+    w.y = __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410) & g.mask;
+    return w;
+}
+
+// 8 byte codes -> 8 nibbles (the even one in the low half of each byte).
+__device__ __forceinline__ uint32_t pack_nibbles(uint2 w) {
+    const uint32_t a = w.x & 0x0f0f0f0fu, b = w.y & 0x0f0f0f0fu;
+    return __byte_perm(a | (a >> 4), b | (b >> 4), 0x6420);
+}
+
+// Four signed byte codes as floats: the byte, biased to unsigned, becomes the
+// low mantissa byte of 2^23 + (q + 128).
+__device__ __forceinline__ void bytes_to_f(uint32_t w, float (&f)[4]) {
+    const uint32_t b = w ^ 0x80808080u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        f[i] = __uint_as_float(__byte_perm(b, 0x4b000000u, 0x7440 | i)) - 8388736.f;
+}
+
+// Eight nibble codes as floats, in order.
+__device__ __forceinline__ void nibbles_to_f(uint32_t w, float (&f)[8]) {
+    const uint32_t lo = (w & 0x0f0f0f0fu) ^ 0x08080808u, hi = ((w >> 4) & 0x0f0f0f0fu) ^ 0x08080808u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[2 * i] = __uint_as_float(__byte_perm(lo, 0x4b000000u, 0x7440 | i)) - 8388616.f;
+        f[2 * i + 1] = __uint_as_float(__byte_perm(hi, 0x4b000000u, 0x7440 | i)) - 8388616.f;
+    }
+}
+
+}  // namespace dnb

@@ -1,0 +1,531 @@
+// The 8/4-bit row cache: rows are quantised as they are written to scattered
+// or consecutive cache rows, and read back through row numbers or page tables
+// (include/denoiser_b200_quant.h has the definition, quant.cuh the arithmetic).
+//
+// Both directions move each byte once and are bound by HBM. A sub-warp of SG
+// lanes takes one group of a row, a lane 8 columns (a 16-byte load of FP16),
+// so the group's maximum is log2(SG) shuffles and nothing passes through
+// shared memory; every lane has the loads of several groups in flight before
+// it uses the first. Groups that do not fit this (a column count or an address
+// that is no multiple of the vectors) take a warp per group with scalar
+// accesses.
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <string>
+
+#include "denoiser_b200_quant.h"
+#include "launch.cuh"
+#include "quant.cuh"
+#include "row_cache.h"
+#include "status.h"
+
+namespace dnb {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr uint32_t kSiteWrite = 0x60, kSiteRead = 0x61;
+
+// Rows of one scattered write may name the same slot; the last one counts.
+//   up to kScanRows rows: every group looks through the later slots;
+//   more: the slot's scale words, which are about to be overwritten, first
+//   hold the largest row index that names the slot (two small kernels). An
+//   index below 2^23 is never the bit pattern of a scale (scales are >= 2^-126,
+//   0x00800000, or NaN), so a group that finds another value has lost.
+constexpr int64_t kScanRows = 256;
+constexpr int64_t kMarkRows = 1 << 23;
+enum : int { kOrderNone = 0, kOrderScan = 1, kOrderMark = 2 };
+
+struct WriteArgs {
+    CacheWrite p;
+    int ngroups;
+    int order;
+};
+
+__device__ __forceinline__ int64_t slot_of(const WriteArgs& a, int64_t row) {
+    return a.p.slots ? a.p.slots[row] : a.p.row0 + row;
+}
+
+// Whether group g of `row` is written; reports a slot behind the cache.
+// Warp-wide call; the SG lanes of a sub-warp pass the same row.
+template <int SG>
+__device__ __forceinline__ bool wins(const WriteArgs& a, int64_t row, int g, int64_t slot, bool live) {
+    if (live && slot >= a.p.capacity) report_error(a.p.err, kSiteWrite, kErrBadShape);
+    live = live && slot >= 0 && slot < a.p.capacity;
+    if (a.order == kOrderScan) {
+        const int lane = threadIdx.x & 31;
+        bool later = false;
+        for (int64_t j = lane % SG; j < a.p.rows; j += SG) later = later || (j > row && a.p.slots[j] == slot);
+        const uint32_t hit = __ballot_sync(0xffffffffu, later);
+        const uint32_t mine = SG == 32 ? 0xffffffffu : ((1u << (SG & 31)) - 1u) << (lane / SG * SG);
+        live = live && !(hit & mine);
+    } else if (a.order == kOrderMark && live) {
+        live = __ldcg(reinterpret_cast<const int*>(a.p.scales + slot * a.ngroups + g)) == static_cast<int>(row);
+    }
+    __syncwarp();  // every lane has read the mark before one of them writes the scale over it
+    return live;
+}
+
+__global__ void __launch_bounds__(kThreads) mark_kernel(const WriteArgs a, int phase) {
+    pdl_trigger();
+    pdl_wait();
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+    const int64_t row = i / a.ngroups;
+    if (row >= a.p.rows) return;
+    const int64_t slot = a.p.slots[row];
+    if (slot < 0 || slot >= a.p.capacity) return;
+    int* m = reinterpret_cast<int*>(a.p.scales + slot * a.ngroups + (i - row * a.ngroups));
+    if (phase == 0)
+        *m = -1;
+    else
+        atomicMax(m, static_cast<int>(row));
+}
+
+template <typename T, int SG, int V, int U>
+__global__ void __launch_bounds__(kThreads) write_vec_kernel(const WriteArgs a) {
+    using Q = QuantOf<T>;
+    pdl_trigger();
+    pdl_wait();
+    constexpr int kPer = 32 / SG;  // groups of a warp at a time
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int sub = lane / SG, l = lane % SG;
+    const int nv = a.p.group / 8;
+    const int64_t units = a.p.rows * a.ngroups;
+    const int64_t u0 = (static_cast<int64_t>(blockIdx.x) * kWarps + warp) * (kPer * U);
+    if (u0 >= units) return;
+    const float qmax = a.p.bits == 8 ? 127.f : 7.f;
+    const T* x = static_cast<const T*>(a.p.x);
+    typename Q::Vec v[U][V];
+    int64_t row[U];
+    int grp[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int64_t u = u0 + i * kPer + sub;
+        row[i] = a.ngroups == 1 ? u : u / a.ngroups;
+        grp[i] = a.ngroups == 1 ? 0 : static_cast<int>(u - row[i] * a.ngroups);
+        const T* src = x + row[i] * a.p.ldx + static_cast<int64_t>(grp[i]) * a.p.group;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int c = l + k * SG;
+            v[i][k] = (u < units && c < nv) ? Q::load(src + c * 8) : Q::zero();
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const bool there = u0 + i * kPer + sub < units;
+        uint32_t mag = Q::mag(v[i][0]);
+#pragma unroll
+        for (int k = 1; k < V; ++k) mag = max(mag, Q::mag(v[i][k]));
+#pragma unroll
+        for (int d = SG / 2; d > 0; d >>= 1) mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, d));
+        const GroupScale g = group_scale<T>(mag, qmax);
+        const bool fix = !Q::kF32 && __any_sync(0xffffffffu, g.fix != 0.f);
+        const int64_t slot = there ? slot_of(a, row[i]) : -1;
+        if (!wins<SG>(a, row[i], grp[i], slot, there)) continue;
+        uint8_t* dst = a.p.codes + slot * a.p.ldc + static_cast<int64_t>(grp[i]) * a.p.group * a.p.bits / 8;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const int c = l + k * SG;
+            if (c < nv) {
+                const uint2 w = codes8<T>(v[i][k], g, fix);
+                if (a.p.bits == 8)
+                    *reinterpret_cast<uint2*>(dst + c * 8) = w;
+                else
+                    *reinterpret_cast<uint32_t*>(dst + c * 4) = pack_nibbles(w);
+            }
+        }
+        if (l == 0) a.p.scales[slot * a.ngroups + grp[i]] = g.s;
+    }
+}
+
+// Any size and alignment: a warp per group, two passes over it.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) write_any_kernel(const WriteArgs a) {
+    using Q = QuantOf<T>;
+    pdl_trigger();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+    if (u >= a.p.rows * a.ngroups) return;
+    const int64_t row = u / a.ngroups;
+    const int grp = static_cast<int>(u - row * a.ngroups);
+    const int n = a.p.group;
+    const T* src = static_cast<const T*>(a.p.x) + row * a.p.ldx + static_cast<int64_t>(grp) * n;
+    const float qmax = a.p.bits == 8 ? 127.f : 7.f;
+    uint32_t mag = 0;
+    for (int c = lane * 8; c < n; c += 256) mag = max(mag, Q::mag(Q::load_some(src + c, min(8, n - c))));
+    mag = __reduce_max_sync(0xffffffffu, mag);
+    const GroupScale g = group_scale<T>(mag, qmax);
+    const bool fix = !Q::kF32 && g.fix != 0.f;  // the same on every lane
+    const int64_t slot = slot_of(a, row);
+    if (!wins<32>(a, row, grp, slot, true)) return;
+    uint8_t* dst = a.p.codes + slot * a.p.ldc + static_cast<int64_t>(grp) * n * a.p.bits / 8;
+    for (int c = lane * 8; c < n; c += 256) {
+        const int m = min(8, n - c);
+        const uint2 w = codes8<T>(Q::load_some(src + c, m), g, fix);
+        if (a.p.bits == 8) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < m) dst[c + i] = static_cast<uint8_t>((i < 4 ? w.x : w.y) >> ((i & 3) * 8));
+        } else {
+            const uint32_t b = pack_nibbles(w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (2 * i < m) dst[c / 2 + i] = static_cast<uint8_t>(b >> (i * 8));
+        }
+    }
+    if (lane == 0) a.p.scales[slot * a.ngroups + grp] = g.s;
+}
+
+// ---------------------------------------------------------------------------
+// Reading
+// ---------------------------------------------------------------------------
+
+struct ReadArgs {
+    const uint8_t* codes;
+    int64_t ldc;
+    const float* scales;
+    int64_t capacity;
+    int cols, bits, group, ngroups;
+    const int64_t* slots;  // read_rows: slots or row0
+    int64_t row0;
+    const int32_t* table;  // read_pages (else null)
+    int64_t table_ld;
+    uint32_t page_rows;
+    const int32_t* lengths;
+    int64_t rows;          // rows of out a sequence may fill
+    void* out;
+    int64_t out_batch, ldo;
+    uint32_t* err;
+};
+
+// Cache row of out row i of sequence b, or -1. i < 2^31.
+__device__ __forceinline__ int64_t source_row(const ReadArgs& a, int b, int64_t i, int64_t n) {
+    if (i >= n) return -1;
+    int64_t r;
+    if (a.table) {
+        const uint32_t q = static_cast<uint32_t>(i) / a.page_rows;
+        const int32_t page = a.table[b * a.table_ld + q];
+        if (page < 0) return -1;
+        r = static_cast<int64_t>(page) * a.page_rows + (static_cast<uint32_t>(i) - q * a.page_rows);
+    } else {
+        r = a.slots ? a.slots[i] : a.row0 + i;
+        if (r < 0) return -1;
+    }
+    if (r >= a.capacity) {
+        report_error(a.err, kSiteRead, kErrBadShape);
+        return -1;
+    }
+    return r;
+}
+
+__device__ __forceinline__ int64_t sequence_rows(const ReadArgs& a, int b) {
+    if (!a.lengths) return a.rows;
+    const int64_t n = a.lengths[b];
+    return n < 0 ? 0 : (n < a.rows ? n : a.rows);
+}
+
+__device__ __forceinline__ void store8(__half* p, const float (&f)[8]) { *reinterpret_cast<uint4*>(p) = f_to_h8(f); }
+__device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+}
+__device__ __forceinline__ void store1(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
+
+// SG lanes per row (a lane 8 columns at a time), U rows of each sub-warp in
+// flight.
+template <typename T, int BITS, int SG, int U>
+__global__ void __launch_bounds__(kThreads) read_vec_kernel(const ReadArgs a) {
+    pdl_trigger();
+    pdl_wait();
+    constexpr int kPer = 32 / SG;
+    const int lane = threadIdx.x & 31;
+    const int sub = lane / SG, l = lane % SG;
+    const int b = blockIdx.y;
+    const int64_t n = sequence_rows(a, b);
+    const int64_t i0 = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * (kPer * U) + sub;
+    if (i0 - sub >= n) return;
+    const int nv = a.cols / 8;
+    int64_t src[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) src[k] = source_row(a, b, i0 + k * kPer, n);
+    T* out = static_cast<T*>(a.out) + b * a.out_batch;
+    for (int c = l; c < nv; c += SG) {
+        uint2 w[U];
+        float s[U];
+        const int g = a.ngroups == 1 ? 0 : c * 8 / a.group;
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            if (src[k] < 0) continue;
+            const uint8_t* p = a.codes + src[k] * a.ldc;
+            if (BITS == 8)
+                w[k] = *reinterpret_cast<const uint2*>(p + c * 8);
+            else
+                w[k].x = *reinterpret_cast<const uint32_t*>(p + c * 4);
+            s[k] = a.scales[src[k] * a.ngroups + g];
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            if (src[k] < 0) continue;
+            float f[8];
+            if (BITS == 8) {
+                float lo[4], hi[4];
+                bytes_to_f(w[k].x, lo);
+                bytes_to_f(w[k].y, hi);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[i] = lo[i], f[i + 4] = hi[i];
+            } else {
+                nibbles_to_f(w[k].x, f);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] *= s[k];
+            store8(out + (i0 + k * kPer) * a.ldo + c * 8, f);
+        }
+    }
+}
+
+// Any size and alignment: a warp per row.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) read_any_kernel(const ReadArgs a) {
+    pdl_trigger();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int b = blockIdx.y;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+    const int64_t src = source_row(a, b, i, sequence_rows(a, b));
+    if (src < 0) return;
+    const uint8_t* p = a.codes + src * a.ldc;
+    const float* sc = a.scales + src * a.ngroups;
+    T* out = static_cast<T*>(a.out) + b * a.out_batch + i * a.ldo;
+    for (int c = lane; c < a.cols; c += 32) {
+        int q;
+        if (a.bits == 8)
+            q = static_cast<int8_t>(p[c]);
+        else
+            q = static_cast<int>((p[c >> 1] >> ((c & 1) * 4)) & 15u) - ((p[c >> 1] >> ((c & 1) * 4)) & 8u ? 16 : 0);
+        store1(out + c, static_cast<float>(q) * sc[a.ngroups == 1 ? 0 : c / a.group]);
+    }
+}
+
+bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+int pow2_lanes(int nv) {
+    int s = 1;
+    while (s < nv && s < 32) s <<= 1;
+    return s;
+}
+
+template <typename T, int SG, int V, int U>
+cudaError_t write_run(const WriteArgs& a, cudaStream_t s) {
+    const int64_t per = static_cast<int64_t>(kWarps) * (32 / SG) * U;
+    const int64_t units = a.p.rows * a.ngroups;
+    return launch_pdl(write_vec_kernel<T, SG, V, U>, dim3(static_cast<unsigned>((units + per - 1) / per)), dim3(kThreads),
+                      0, s, a);
+}
+
+template <typename T>
+cudaError_t write_type(const WriteArgs& a, cudaStream_t s) {
+    const CacheWrite& p = a.p;
+    const int nv = p.group / 8;
+    // A vector of 8 codes has `bits` bytes.
+    const bool vec = p.group % 8 == 0 && nv <= 256 && aligned(p.x, 16) && p.ldx * sizeof(T) % 16 == 0 &&
+                     aligned(p.codes, p.bits) && p.ldc % p.bits == 0;
+    if (!vec) {
+        const int64_t units = p.rows * a.ngroups;
+        return launch_pdl(write_any_kernel<T>, dim3(static_cast<unsigned>((units + kWarps - 1) / kWarps)),
+                          dim3(kThreads), 0, s, a);
+    }
+    switch (pow2_lanes(nv)) {
+        case 1: return write_run<T, 1, 1, 4>(a, s);
+        case 2: return write_run<T, 2, 1, 4>(a, s);
+        case 4: return write_run<T, 4, 1, 4>(a, s);
+        case 8: return write_run<T, 8, 1, 4>(a, s);
+        case 16: return write_run<T, 16, 1, 4>(a, s);
+        default: break;
+    }
+    if (nv <= 32) return write_run<T, 32, 1, 4>(a, s);
+    if (nv <= 64) return write_run<T, 32, 2, 2>(a, s);
+    if (nv <= 128) return write_run<T, 32, 4, 1>(a, s);
+    return write_run<T, 32, 8, 1>(a, s);
+}
+
+template <typename T, int BITS, int SG, int U>
+cudaError_t read_run(const ReadArgs& a, int batch, cudaStream_t s) {
+    const int64_t per = static_cast<int64_t>(kWarps) * (32 / SG) * U;
+    return launch_pdl(read_vec_kernel<T, BITS, SG, U>, dim3(static_cast<unsigned>((a.rows + per - 1) / per), batch),
+                      dim3(kThreads), 0, s, a);
+}
+
+template <typename T, int BITS>
+cudaError_t read_bits(const ReadArgs& a, int batch, cudaStream_t s) {
+    switch (pow2_lanes(a.cols / 8)) {
+        case 1: return read_run<T, BITS, 1, 4>(a, batch, s);
+        case 2: return read_run<T, BITS, 2, 4>(a, batch, s);
+        case 4: return read_run<T, BITS, 4, 4>(a, batch, s);
+        case 8: return read_run<T, BITS, 8, 4>(a, batch, s);
+        case 16: return read_run<T, BITS, 16, 4>(a, batch, s);
+        default: return read_run<T, BITS, 32, 4>(a, batch, s);
+    }
+}
+
+template <typename T>
+cudaError_t read_type(const ReadArgs& a, int batch, cudaStream_t s) {
+    const bool vec = a.cols % 8 == 0 && a.group % 8 == 0 && aligned(a.codes, a.bits) && a.ldc % a.bits == 0 &&
+                     aligned(a.out, 16) && a.ldo * sizeof(T) % 16 == 0 && a.out_batch * sizeof(T) % 16 == 0;
+    if (!vec)
+        return launch_pdl(read_any_kernel<T>, dim3(static_cast<unsigned>((a.rows + kWarps - 1) / kWarps), batch),
+                          dim3(kThreads), 0, s, a);
+    return a.bits == 8 ? read_bits<T, 8>(a, batch, s) : read_bits<T, 4>(a, batch, s);
+}
+
+int run_read(const ReadArgs& a, int batch, int dtype, cudaStream_t s, const char* name) {
+    const cudaError_t e = dtype == 1 ? read_type<__half>(a, batch, s) : read_type<float>(a, batch, s);
+    return e == cudaSuccess ? DN_OK : dn_cuda_fail(e, name);
+}
+
+// The shape of a cache: DN_OK, or the status of what is wrong with it.
+int check_cache(const void* codes, int64_t ldc, const float* scales, int64_t capacity, int cols, int bits, int& group,
+                int dtype, const std::string& name) {
+    if (dtype != 0 && dtype != 1) return dn_fail_str(DN_ERR_DTYPE, name + ": dtype must be 0 (FP32) or 1 (FP16)");
+    if (bits != 8 && bits != 4) return dn_fail_str(DN_ERR_INVALID_ARG, name + ": bits must be 8 or 4");
+    if (cols <= 0 || cols > (1 << 24)) return dn_fail_str(DN_ERR_INVALID_ARG, name + ": cols outside [1, 2^24]");
+    if (group == 0) group = cols;
+    if (group < 0 || cols % group != 0) return dn_fail_str(DN_ERR_INVALID_ARG, name + ": group does not divide cols");
+    if (group != cols && group % 8 != 0)
+        return dn_fail_str(DN_ERR_INVALID_ARG, name + ": a group smaller than a row must be a multiple of 8");
+    if (capacity < 0 || capacity >= (1LL << 31))
+        return dn_fail_str(DN_ERR_INVALID_ARG, name + ": capacity outside [0, 2^31)");
+    if (ldc < (static_cast<int64_t>(cols) * bits + 7) / 8)
+        return dn_fail_str(DN_ERR_INVALID_ARG, name + ": ld_codes is less than a row");
+    if (capacity > 0 && (!codes || !scales)) return dn_fail_str(DN_ERR_INVALID_ARG, name + ": null cache");
+    if (!aligned(scales, 4)) return dn_fail_str(DN_ERR_INVALID_ARG, name + ": scales must be 4-byte aligned");
+    return DN_OK;
+}
+
+// Rows of a caller's matrix: aligned to their type, strides that hold a row.
+int check_rows(const void* x, int dtype, int64_t rows, int64_t ld, int cols, const std::string& name) {
+    if (rows < 0 || rows >= (1LL << 31)) return dn_fail_str(DN_ERR_INVALID_ARG, name + ": rows outside [0, 2^31)");
+    if (rows == 0) return DN_OK;
+    if (!x) return dn_fail_str(DN_ERR_INVALID_ARG, name + ": null pointer");
+    if (!aligned(x, dtype == 1 ? 2 : 4)) return dn_fail_str(DN_ERR_INVALID_ARG, name + ": misaligned pointer");
+    if (ld < cols && rows > 1) return dn_fail_str(DN_ERR_INVALID_ARG, name + ": row stride is less than a row");
+    return DN_OK;
+}
+
+}  // namespace
+
+int launch_cache_write(const CacheWrite& p0, cudaStream_t s) {
+    const int ngroups = p0.cols / p0.group;
+    // A launch takes up to 2^23 rows (marks) and 2^30 groups.
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(p0.slots ? kMarkRows : (1LL << 30), (1LL << 30) / ngroups));
+    for (int64_t r = 0; r < p0.rows; r += most) {
+        WriteArgs a{p0, ngroups, kOrderNone};
+        a.p.rows = std::min(most, p0.rows - r);
+        a.p.x = static_cast<const char*>(p0.x) + r * p0.ldx * (p0.dtype == 1 ? 2 : 4);
+        a.p.row0 = p0.row0 + r;
+        if (p0.slots) {
+            a.p.slots = p0.slots + r;
+            a.order = a.p.rows == 1 ? kOrderNone : a.p.rows <= kScanRows ? kOrderScan : kOrderMark;
+        }
+        if (a.order == kOrderMark) {
+            const unsigned blocks = static_cast<unsigned>((a.p.rows * ngroups + kThreads - 1) / kThreads);
+            for (int phase = 0; phase < 2; ++phase) {
+                const cudaError_t e = launch_pdl(mark_kernel, dim3(blocks), dim3(kThreads), 0, s, a, phase);
+                if (e != cudaSuccess) return dn_cuda_fail(e, "cache write: mark launch");
+            }
+        }
+        const cudaError_t e = p0.dtype == 1 ? write_type<__half>(a, s) : write_type<float>(a, s);
+        if (e != cudaSuccess) return dn_cuda_fail(e, "cache write: launch");
+    }
+    return DN_OK;
+}
+
+}  // namespace dnb
+
+using namespace dnb;
+
+extern "C" {
+
+int dn_launch_cache_write(const void* x, int dtype, int64_t ldx, int64_t rows, int cols, const int64_t* slots,
+                          int64_t row0, void* codes, int64_t ld_codes, float* scales, int64_t capacity, int bits,
+                          int group, uint32_t* err_dev, void* stream) {
+    const char* name = "dn_launch_cache_write";
+    DN_TRY(check_cache(codes, ld_codes, scales, capacity, cols, bits, group, dtype, name));
+    DN_TRY(check_rows(x, dtype, rows, ldx, cols, name));
+    if (!slots && (row0 < 0 || row0 > capacity - rows))
+        return dn_fail(DN_ERR_INVALID_ARG, "dn_launch_cache_write: rows outside the cache");
+    if (rows == 0) return DN_OK;
+    return launch_cache_write(CacheWrite{x, dtype, ldx, rows, cols, slots, row0, static_cast<uint8_t*>(codes), ld_codes,
+                                         scales, capacity, bits, group, err_dev},
+                              static_cast<cudaStream_t>(stream));
+}
+
+int dn_launch_cache_read_rows(const void* codes, int64_t ld_codes, const float* scales, int64_t capacity, int cols,
+                              int bits, int group, const int64_t* slots, int64_t row0, int64_t rows, void* out,
+                              int dtype, int64_t ldo, uint32_t* err_dev, void* stream) {
+    const char* name = "dn_launch_cache_read_rows";
+    DN_TRY(check_cache(codes, ld_codes, scales, capacity, cols, bits, group, dtype, name));
+    DN_TRY(check_rows(out, dtype, rows, ldo, cols, name));
+    if (!slots && (row0 < 0 || row0 > capacity - rows))
+        return dn_fail(DN_ERR_INVALID_ARG, "dn_launch_cache_read_rows: rows outside the cache");
+    if (rows == 0) return DN_OK;
+    ReadArgs a{};
+    a.codes = static_cast<const uint8_t*>(codes);
+    a.ldc = ld_codes;
+    a.scales = scales;
+    a.capacity = capacity;
+    a.cols = cols;
+    a.bits = bits;
+    a.group = group;
+    a.ngroups = cols / group;
+    a.slots = slots;
+    a.row0 = row0;
+    a.rows = rows;
+    a.out = out;
+    a.ldo = ldo;
+    a.err = err_dev;
+    return run_read(a, 1, dtype, static_cast<cudaStream_t>(stream), name);
+}
+
+int dn_launch_cache_read_pages(const void* codes, int64_t ld_codes, const float* scales, int64_t capacity, int cols,
+                               int bits, int group, int64_t page_rows, const int32_t* table, int64_t table_ld,
+                               int64_t table_cols, const int32_t* lengths, int batch, int64_t max_rows, void* out,
+                               int dtype, int64_t out_batch, int64_t ldo, uint32_t* err_dev, void* stream) {
+    const char* name = "dn_launch_cache_read_pages";
+    DN_TRY(check_cache(codes, ld_codes, scales, capacity, cols, bits, group, dtype, name));
+    if (page_rows <= 0 || page_rows >= (1LL << 31))
+        return dn_fail(DN_ERR_INVALID_ARG, "dn_launch_cache_read_pages: page_rows outside [1, 2^31)");
+    if (batch < 0 || batch > 65535) return dn_fail(DN_ERR_INVALID_ARG, "dn_launch_cache_read_pages: batch outside [0, 65535]");
+    if (table_cols < 0 || table_cols >= (1LL << 31) || (batch > 1 && table_ld < table_cols))
+        return dn_fail(DN_ERR_INVALID_ARG, "dn_launch_cache_read_pages: bad page table");
+    DN_TRY(check_rows(out, dtype, max_rows, ldo, cols, name));
+    const int64_t rows = std::min(max_rows, table_cols * page_rows);
+    if (rows == 0 || batch == 0) return DN_OK;
+    if (!table) return dn_fail(DN_ERR_INVALID_ARG, "dn_launch_cache_read_pages: null page table");
+    if (batch > 1 && out_batch < (max_rows - 1) * ldo + cols)
+        return dn_fail(DN_ERR_INVALID_ARG, "dn_launch_cache_read_pages: out_batch is less than a sequence");
+    ReadArgs a{};
+    a.codes = static_cast<const uint8_t*>(codes);
+    a.ldc = ld_codes;
+    a.scales = scales;
+    a.capacity = capacity;
+    a.cols = cols;
+    a.bits = bits;
+    a.group = group;
+    a.ngroups = cols / group;
+    a.table = table;
+    a.table_ld = table_ld;
+    a.page_rows = static_cast<uint32_t>(page_rows);
+    a.lengths = lengths;
+    a.rows = rows;
+    a.out = out;
+    a.out_batch = batch > 1 ? out_batch : 0;
+    a.ldo = ldo;
+    a.err = err_dev;
+    return run_read(a, batch, dtype, static_cast<cudaStream_t>(stream), name);
+}
+
+}  // extern "C"
