@@ -12,6 +12,7 @@
 #include "capi_internal.h"
 #include "denoiser_b200_quant.h"
 #include "launch.cuh"
+#include "linear8.h"
 #include "quant.cuh"
 #include "row_cache.h"
 #include "status.h"
@@ -19,87 +20,7 @@
 namespace dnb {
 namespace {
 
-constexpr int kMaxSegments = 16;
 constexpr int kMaxK = 131072;  // 127 * 127 * 131072 < 2^31
-
-struct ProductArgs {
-    const int8_t* a;   // codes of the tokens
-    int64_t lda;
-    const float* as;   // a scale per code row
-    int64_t arow[kMaxSegments];  // first code row of each segment
-    int segs, seg_c, seg_p;      // segments, their channels, their bytes in a weight row
-    const int8_t* w;   // [cout][ldw]
-    int64_t ldw;
-    const float* ws;
-    const float* bias; // null: none
-    int cout, n_out, gate;
-    int64_t rows;
-    void* out;
-    int64_t ldo;       // row stride of out; planes: pixels of a plane
-    int planes;        // out[(m / ldo) * n_out + c][m % ldo] instead of out[m][c]
-};
-
-__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void put(float* p, float v) { *p = v; }
-
-template <typename T>
-__global__ void __launch_bounds__(256) product_kernel(const __grid_constant__ ProductArgs a) {
-    pdl_trigger();
-    pdl_wait();
-    __shared__ int sa[64][17], sb[2][64][17];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int64_t m0 = static_cast<int64_t>(blockIdx.x) * 64;
-    const int c0 = blockIdx.y * 64;
-    const int halves = a.gate ? 2 : 1;
-    float y[2][4][4] = {};
-    for (int t = 0; t < a.segs; ++t) {
-        int acc[2][4][4] = {};
-        for (int k0 = 0; k0 < a.seg_p; k0 += 64) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-                const int r = i >> 4, k = k0 + (i & 15) * 4;
-                const int64_t m = m0 + r;
-                sa[r][i & 15] = (m < a.rows && k < a.seg_c)
-                                    ? *reinterpret_cast<const int*>(a.a + (a.arow[t] + m) * a.lda + k)
-                                    : 0;
-                for (int h = 0; h < halves; ++h) {
-                    const int c = c0 + r;
-                    sb[h][r][i & 15] = (c < a.n_out && k < a.seg_p)
-                                           ? *reinterpret_cast<const int*>(a.w + static_cast<int64_t>(c + h * a.n_out) * a.ldw +
-                                                                           t * a.seg_p + k)
-                                           : 0;
-                }
-            }
-            __syncthreads();
-            for (int k = 0; k < 16; ++k)
-                for (int h = 0; h < halves; ++h)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            acc[h][i][j] = __dp4a(sa[ty * 4 + i][k], sb[h][tx * 4 + j][k], acc[h][i][j]);
-        }
-        for (int i = 0; i < 4; ++i) {
-            const int64_t m = m0 + ty * 4 + i;
-            const float s = m < a.rows ? a.as[a.arow[t] + m] : 0.f;
-            for (int h = 0; h < halves; ++h)
-                for (int j = 0; j < 4; ++j) y[h][i][j] = fmaf(static_cast<float>(acc[h][i][j]), s, y[h][i][j]);
-        }
-    }
-    T* out = static_cast<T*>(a.out);
-    for (int i = 0; i < 4; ++i) {
-        const int64_t m = m0 + ty * 4 + i;
-        if (m >= a.rows) continue;
-        for (int j = 0; j < 4; ++j) {
-            const int c = c0 + tx * 4 + j;
-            if (c >= a.n_out) continue;
-            float v = fmaf(y[0][i][j], a.ws[c], a.bias ? a.bias[c] : 0.f);
-            if (a.gate) v *= fmaf(y[1][i][j], a.ws[c + a.n_out], a.bias ? a.bias[c + a.n_out] : 0.f);
-            const int64_t img = a.planes ? m / a.ldo : 0;
-            put(out + (a.planes ? (img * a.n_out + c) * a.ldo + (m - img * a.ldo) : m * a.ldo + c), v);
-        }
-    }
-}
 
 // Codes and scales of the pixels of NCHW planes: a thread per pixel.
 __global__ void __launch_bounds__(256) quantise_planes_kernel(const __half* __restrict__ x, int64_t rows, int K, int64_t hw,
@@ -156,6 +77,7 @@ struct dn_linear8 {
     int device = 0;
     int cout = 0, cin = 0, gate = 0, segs = 1, seg_c = 0, seg_p = 0;
     int64_t ldw = 0;
+    int sms = 148;
     uint8_t* arena = nullptr;  // weight codes, scales, bias, error word
     int8_t* w = nullptr;
     float* ws = nullptr;
@@ -173,7 +95,7 @@ int check_shape(int64_t cout, int64_t cin, int gate, int segments) {
     if (gate && cout % 2) return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_create: the gate needs an even number of channels");
     if (segments < 1 || cin % segments)
         return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_create: segments does not divide the input channels");
-    if (segments > kMaxSegments) return dn_fail(DN_ERR_UNSUPPORTED, "dn_linear8_create: more than 16 segments");
+    if (segments > kMaxSegments) return dn_fail(DN_ERR_UNSUPPORTED, "dn_linear8_create: more than 8 segments");
     return DN_OK;
 }
 
@@ -220,6 +142,7 @@ int create(const void* weight, int dtype, int64_t ldw, const void* bias, int cou
     L->seg_p = static_cast<int>(round16(L->seg_c));
     L->ldw = static_cast<int64_t>(L->seg_p) * segments;
     int rc = DN_OK;
+    cudaDeviceGetAttribute(&L->sms, cudaDevAttrMultiProcessorCount, device);
     const cudaError_t e = lay_out(L.get(), weight, dtype, ldw, bias, s, rc);
     if (e != cudaSuccess || rc != DN_OK) {
         cudaFree(L->arena);
@@ -241,14 +164,8 @@ ProductArgs product_args(const dn_linear8* L) {
     a.cout = L->cout;
     a.n_out = L->n_out();
     a.gate = L->gate;
+    a.err = L->err;
     return a;
-}
-
-int run_product(const ProductArgs& a, int out_dtype, cudaStream_t s) {
-    const dim3 grid(static_cast<unsigned>((a.rows + 63) / 64), static_cast<unsigned>((a.n_out + 63) / 64));
-    const cudaError_t e = out_dtype == 1 ? launch_pdl(product_kernel<__half>, grid, dim3(256), 0, s, a)
-                                         : launch_pdl(product_kernel<float>, grid, dim3(256), 0, s, a);
-    return e == cudaSuccess ? DN_OK : dn_cuda_fail(e, "dn_linear8: launch");
 }
 
 bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -372,10 +289,11 @@ int dn_linear8_forward(dn_linear8* L, const void* x, int dtype, int64_t ldx, int
                               s));
     a.a = reinterpret_cast<const int8_t*>(codes);
     a.as = scales;
+    a.a_rows = rows;
     a.rows = rows;
     a.out = out;
     a.ldo = ldo;
-    return run_product(a, out_dtype, s);
+    return launch_product_tc(a, out_dtype, L->sms, s);
 }
 
 int dn_linear8_forward_nchw(dn_linear8* L, const void* input, int N, int H, int W, void* output, void* workspace,
@@ -402,11 +320,12 @@ int dn_linear8_forward_nchw(dn_linear8* L, const void* input, int N, int H, int 
     if (e != cudaSuccess) return dn_cuda_fail(e, "dn_linear8_forward_nchw: quantise launch");
     a.a = reinterpret_cast<const int8_t*>(codes);
     a.as = scales;
+    a.a_rows = rows;
     a.rows = rows;
     a.out = output;
     a.ldo = hw;
     a.planes = 1;
-    return run_product(a, 1, s);
+    return launch_product_tc(a, 1, L->sms, s);
 }
 
 int dn_linear8_forward_cached(dn_linear8* L, const void* codes, int64_t ld_codes, const float* scales, int64_t capacity,
@@ -434,10 +353,11 @@ int dn_linear8_forward_cached(dn_linear8* L, const void* codes, int64_t ld_codes
     a.a = static_cast<const int8_t*>(codes);
     a.lda = ld_codes;
     a.as = scales;
+    a.a_rows = capacity;
     a.rows = rows;
     a.out = out;
     a.ldo = ldo;
-    return run_product(a, out_dtype, static_cast<cudaStream_t>(stream));
+    return launch_product_tc(a, out_dtype, L->sms, static_cast<cudaStream_t>(stream));
 }
 
 int dn_linear8_sync(dn_linear8* L, void* stream) {

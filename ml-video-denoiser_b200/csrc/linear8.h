@@ -1,0 +1,35 @@
+// Internal interface of the 8-bit product: what a launch needs, shared by the
+// layer (linear8.cu) and its kernels (linear8_tc.cu).
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace dnb {
+
+constexpr int kMaxSegments = 8;
+
+struct ProductArgs {
+    const int8_t* a;             // codes of the tokens, rows of lda bytes (a multiple of 16)
+    int64_t lda, a_rows;         // a_rows: rows that `a` has
+    const float* as;             // a scale per code row
+    int64_t arow[kMaxSegments];  // first code row of each segment
+    int segs, seg_c, seg_p;      // segments, their channels, their bytes in a weight row (a multiple of 16)
+    const int8_t* w;             // [cout][ldw]
+    int64_t ldw;
+    const float* ws;             // [cout]
+    const float* bias;           // [cout], or null
+    int cout, n_out, gate;
+    int64_t rows;
+    void* out;
+    int64_t ldo;                 // row stride of out; planes: pixels of a plane
+    int planes;                  // out[(m / ldo) * n_out + c][m % ldo] instead of out[m][c]
+    uint32_t* err;
+};
+
+// The product on the tensor cores; out_dtype 0 FP32, 1 FP16; `sms` of the
+// current device.
+int launch_product_tc(const ProductArgs& a, int out_dtype, int sms, cudaStream_t s);
+
+}  // namespace dnb

@@ -1,0 +1,404 @@
+// The 8-bit product on the tensor cores (tcgen05 kind::i8, int32 in TMEM):
+//
+//   y[m, n] = s_w[n] sum_t s_x[t, m] (sum_c q_x[t, m, c] q_w[n, t, c]) + bias[n]
+//
+// A persistent, warp-specialised kernel (352 threads, one CTA per SM) over
+// tiles of 128 tokens x NT channels:
+//   warp 8      TMA loads of the token codes: boxes of 128 rows x KC bytes,
+//               swizzled by KC = 128 / 64 / 32 (the least that holds a
+//               segment); bytes behind a segment read as zeros;
+//   warp 9      TMA loads of the weight rows (gated layers: the two halves'
+//               rows, so that a tile has both factors of its outputs);
+//   warp 10     one thread issues the MMAs (M = 128, N = NT, K = 32): a TMEM
+//               accumulator of NT columns per segment, two sets of them where
+//               they fit, so that a tile's epilogue overlaps the next one's
+//               products;
+//   warps 0-7   epilogue: a lane is a token; scales, bias, SimpleGate in FP32,
+//               then through a swizzled 4 KB tile per warp and a TMA store
+//               (rows whose address or stride does not allow it, and planes,
+//               are stored directly).
+// A segment's int32 sum is exact; it is scaled once, in FP32. Every wait is
+// bounded.
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <string>
+
+#include "denoiser_b200.h"
+#include "launch.cuh"
+#include "linear8.h"
+#include "sm100.cuh"
+#include "status.h"
+
+namespace dnb {
+
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();  // gemm_tc.cu
+
+namespace {
+
+constexpr int kRows = 128;
+constexpr int kThreads = 352;
+constexpr int kEpiWarps = 8;
+constexpr int kStageA = kRows * 128;
+constexpr int kStgWarp = 32 * 128;  // staging tile of an epilogue warp: 32 rows x 128 bytes
+
+template <int NT>
+struct Plan {
+    static constexpr int kStage = kStageA + NT * 128;
+    static constexpr int kStages = NT == 256 ? 4 : NT == 128 ? 5 : 6;
+    static constexpr int kBytes = 1024 + kStages * kStage + kEpiWarps * kStgWarp;
+};
+
+struct Maps {
+    CUtensorMap a, b, out;
+};
+
+struct TcArgs {
+    ProductArgs p;
+    int kc, chunks;      // bytes of a K chunk, chunks of a segment
+    int m_tiles, n_tiles;
+    int bufs;            // accumulator sets in TMEM
+    int tma_out;         // 1: staged TMA stores
+    int vec_out;         // direct stores: 16-byte vectors of a row are aligned
+};
+
+__host__ __device__ constexpr uint32_t idesc_s8(int M, int N) {
+    return (2u << 4)                                 // D: s32
+           | (1u << 7) | (1u << 10)                  // A, B: s8
+           | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_s8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                       uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, int (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+        "%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+
+// sum_t s_t acc_t of 32 columns, then the channels' scale and bias (columns
+// past the layer's are not stored; their parameters are not read).
+__device__ __forceinline__ void scaled32(const TcArgs& g, uint32_t taddr, int nt, int64_t row, bool live, int c0,
+                                         float (&y)[32]) {
+    const ProductArgs& p = g.p;
+    int acc[32];
+    for (int t = 0; t < p.segs; ++t) {
+        const float s = live ? __ldg(p.as + p.arow[t] + row) : 0.f;
+        tmem_ld32(taddr + t * nt, acc);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) y[i] = t == 0 ? static_cast<float>(acc[i]) * s : fmaf(static_cast<float>(acc[i]), s, y[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        const int c = c0 + i;
+        const bool in = c < p.cout;
+        const float w = in ? __ldg(p.ws + c) : 0.f, b = in && p.bias ? __ldg(p.bias + c) : 0.f;
+        y[i] = fmaf(y[i], w, b);
+    }
+}
+
+__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+
+// 16 bytes of a row from 8 (FP16) or 4 (FP32) values.
+__device__ __forceinline__ uint4 pack16(const float* y, __half*) {
+    return make_uint4(pack_half2(y[0], y[1]), pack_half2(y[2], y[3]), pack_half2(y[4], y[5]), pack_half2(y[6], y[7]));
+}
+__device__ __forceinline__ uint4 pack16(const float* y, float*) {
+    return make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
+}
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_constant__ TcArgs g,
+                                                                 const __grid_constant__ Maps maps) {
+    using P = Plan<NT>;
+    constexpr int kSt = P::kStages;
+    constexpr int kVec = 16 / sizeof(T);      // values of 16 bytes
+    constexpr int kUnit = 128 / sizeof(T);    // columns of a staging tile
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    __shared__ uint64_t bar_full[kSt], bar_empty[kSt], bar_acc_full[2], bar_acc_empty[2];
+    __shared__ uint32_t tslot;
+    __shared__ volatile int s_abort;
+    const ProductArgs& p = g.p;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tiles = g.m_tiles * g.n_tiles;
+    const uint32_t set_cols = p.segs * NT;  // TMEM columns of one accumulator set
+    uint32_t cols = 32;
+    while (cols < set_cols * g.bufs) cols <<= 1;
+
+    if (warp == 10) {
+        tmem_alloc(&tslot, cols);
+        tmem_relinquish();
+    }
+    if (tid == 0) {
+        for (int s = 0; s < kSt; ++s) {
+            mbar_init(&bar_full[s], 2);
+            mbar_init(&bar_empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&bar_acc_full[b], 1);
+            mbar_init(&bar_acc_empty[b], kEpiWarps);
+        }
+        s_abort = 0;
+        fence_mbar_init();
+        prefetch_tmap(&maps.a);
+        prefetch_tmap(&maps.b);
+        if (g.tma_out) prefetch_tmap(&maps.out);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tslot;
+    pdl_trigger();
+    if (warp != 9) pdl_wait();  // the weights (warp 9) were there before; codes, scales and `out` belong to earlier kernels
+
+    const int half = NT / 2;
+    const int out_cols = p.gate ? half : NT;  // output columns of a tile
+
+    if (warp == 8 || warp == 9) {
+        if (lane == 0) {
+            const uint32_t bytes = static_cast<uint32_t>(warp == 8 ? kRows : NT) * g.kc;
+            int it = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+                const int m0 = (tile / g.n_tiles) * kRows, n0 = (tile % g.n_tiles) * out_cols;
+                for (int t = 0; ok && t < p.segs; ++t)
+                    for (int j = 0; j < g.chunks; ++j, ++it) {
+                        const int s = it % kSt;
+                        ok = wait_or_abort(&bar_empty[s], ((it / kSt) & 1) ^ 1, &s_abort, p.err, 0x70);
+                        if (!ok) break;
+                        uint8_t* sa = smem + s * P::kStage;
+                        mbar_arrive_expect_tx(&bar_full[s], bytes);
+                        if (warp == 8) {
+                            tma_load_2d(sa, &maps.a, j * g.kc, static_cast<int>(p.arow[t]) + m0, &bar_full[s]);
+                        } else {
+                            uint8_t* sb = sa + kStageA;
+                            const int k = t * p.seg_p + j * g.kc;
+                            tma_load_2d(sb, &maps.b, k, n0, &bar_full[s]);
+                            if (p.gate) tma_load_2d(sb + half * g.kc, &maps.b, k, p.n_out + n0, &bar_full[s]);
+                        }
+                    }
+            }
+            // After a wait that ran out: the copies in flight land before the CTA leaves.
+            if (!ok)
+                for (int k = max(0, it - kSt); k < it; ++k) mbar_wait(&bar_full[k % kSt], (k / kSt) & 1, 100000000ull);
+        }
+    } else if (warp == 10) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = idesc_s8(kRows, NT);
+            const uint32_t sm0 = smem_u32(smem);
+            const uint64_t ad0 = sdesc_kmajor_sw(sm0, g.kc), bd0 = sdesc_kmajor_sw(sm0 + kStageA, g.kc);
+            int it = 0, n = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++n) {
+                const int b = g.bufs == 2 ? n & 1 : 0, use = g.bufs == 2 ? n >> 1 : n;
+                ok = wait_or_abort(&bar_acc_empty[b], (use & 1) ^ 1, &s_abort, p.err, 0x71);
+                tc_fence_after();
+                for (int t = 0; ok && t < p.segs; ++t) {
+                    const uint32_t acc = tmem + b * set_cols + t * NT;
+                    for (int j = 0; j < g.chunks; ++j, ++it) {
+                        const int s = it % kSt;
+                        ok = wait_or_abort(&bar_full[s], (it / kSt) & 1, &s_abort, p.err, 0x72);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint64_t so = static_cast<uint64_t>(s) * (P::kStage >> 4);
+                        const int steps = min(g.kc, p.seg_c - j * g.kc + 31) / 32;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (k < steps) mma_s8(acc, ad0 + so + 2 * k, bd0 + so + 2 * k, idesc, (j > 0 || k > 0) ? 1u : 0u);
+                        mma_commit(&bar_empty[s]);
+                    }
+                }
+                if (ok) mma_commit(&bar_acc_full[b]);
+            }
+        }
+    } else {
+        const int quad = warp & 3, group = warp >> 2;
+        uint8_t* stg = smem + kSt * P::kStage + warp * kStgWarp;
+        const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+        T* out = static_cast<T*>(p.out);
+        int n = 0;
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
+            const int b = g.bufs == 2 ? n & 1 : 0, use = g.bufs == 2 ? n >> 1 : n;
+            const int64_t m0 = static_cast<int64_t>(tile / g.n_tiles) * kRows + quad * 32;
+            const int n0 = (tile % g.n_tiles) * out_cols;
+            bool ok = lane == 0 ? wait_or_abort(&bar_acc_full[b], use & 1, &s_abort, p.err, 0x73) : true;
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            if (!ok) break;
+            tc_fence_after();
+            const int64_t row = m0 + lane;
+            const bool live = row < p.rows;
+            const int64_t img = p.planes ? row / p.ldo : 0;
+            const uint32_t acc = lane_base + b * set_cols;
+            // The two groups of four warps take the tile's 32-column runs, or
+            // whole staging tiles, in turn.
+            const int span = g.tma_out ? kUnit : 32;
+            for (int c0 = 0, u = n & 1; c0 < out_cols; c0 += span, ++u) {
+                if ((u & 1) != group || n0 + c0 >= p.n_out) continue;
+                if (g.tma_out) {  // the staging tile is free again
+                    if (lane == 0) bulk_wait_read0();
+                    __syncwarp();
+                }
+                for (int c = c0; c < c0 + span; c += 32) {
+                    float y[32];
+                    scaled32(g, acc + c, NT, row, live, n0 + c, y);
+                    if (p.gate) {
+                        float z[32];
+                        scaled32(g, acc + half + c, NT, row, live, p.n_out + n0 + c, z);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) y[i] *= z[i];
+                    }
+                    if (g.tma_out) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += kVec) {
+                            const int j = (c - c0 + i) / kVec;
+                            *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                                pack16(y + i, static_cast<T*>(nullptr));
+                        }
+                    } else if (p.planes) {
+                        T* o = out + (img * p.n_out + n0 + c) * p.ldo + (row - img * p.ldo);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (live && n0 + c + i < p.n_out) put(o + i * p.ldo, y[i]);
+                    } else if (live) {
+                        T* o = out + row * p.ldo + n0 + c;
+#pragma unroll
+                        for (int i = 0; i < 32; i += kVec) {
+                            if (g.vec_out && n0 + c + i + kVec <= p.n_out) {
+                                *reinterpret_cast<uint4*>(o + i) = pack16(y + i, static_cast<T*>(nullptr));
+                            } else {
+#pragma unroll
+                                for (int k = 0; k < kVec; ++k)
+                                    if (n0 + c + i + k < p.n_out) put(o + i + k, y[i + k]);
+                            }
+                        }
+                    }
+                }
+                if (g.tma_out) {
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0 && m0 < p.rows) {
+                        tma_store_2d(&maps.out, n0 + c0, static_cast<int>(m0), stg);
+                        bulk_commit();
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar_acc_empty[b]);
+        }
+        if (g.tma_out && lane == 0) bulk_wait_read0();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 10) tmem_dealloc(tmem, cols);
+}
+
+int encode(CUtensorMap* m, CUtensorMapDataType type, int esz, const void* base, int64_t cols, int64_t rows, int64_t ld,
+           int box_cols, int box_rows) {
+    auto fn = tensor_map_encoder();
+    if (!fn) return dn_fail(DN_ERR_CUDA, "linear8: cuTensorMapEncodeTiled unavailable");
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * esz};
+    const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
+    const cuuint32_t estr[2] = {1, 1};
+    const int span = box_cols * esz;
+    const CUtensorMapSwizzle swz = span == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                   : span == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                : CU_TENSOR_MAP_SWIZZLE_32B;
+    const CUresult r = fn(m, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          swz, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return dn_fail_str(DN_ERR_CUDA, "linear8: cuTensorMapEncodeTiled failed (" + std::to_string(r) + ")");
+    return DN_OK;
+}
+
+template <typename T, int NT>
+int run(TcArgs& g, int sms, cudaStream_t s) {
+    const ProductArgs& p = g.p;
+    const int out_cols = p.gate ? NT / 2 : NT;
+    g.kc = p.seg_c > 64 ? 128 : p.seg_c > 32 ? 64 : 32;
+    g.chunks = (p.seg_c + g.kc - 1) / g.kc;
+    g.m_tiles = static_cast<int>((p.rows + kRows - 1) / kRows);
+    g.n_tiles = (p.n_out + out_cols - 1) / out_cols;
+    g.bufs = 2 * p.segs * NT <= 512 ? 2 : 1;
+    const bool al16 = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo * sizeof(T) % 16 == 0;
+    // A TMA store moves 128 bytes of a row; narrower tiles and planes go directly.
+    g.tma_out = !p.planes && al16 && out_cols * sizeof(T) >= 128;
+    g.vec_out = !p.planes && al16;
+    Maps maps{};
+    DN_TRY(encode(&maps.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.a, p.seg_c, p.a_rows, p.lda, g.kc, kRows));
+    DN_TRY(encode(&maps.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.ldw, p.cout, p.ldw, g.kc, p.gate ? NT / 2 : NT));
+    if (g.tma_out)
+        DN_TRY(encode(&maps.out, sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+                      sizeof(T), p.out, p.n_out, p.rows, p.ldo, 128 / sizeof(T), 32));
+    const int64_t tiles = static_cast<int64_t>(g.m_tiles) * g.n_tiles;
+    if (tiles >= (1LL << 30)) return dn_fail(DN_ERR_UNSUPPORTED, "linear8: the product has 2^30 tiles or more");
+    static bool configured[64] = {};  // per device
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess && (device >= 64 || !configured[device])) {
+        e = cudaFuncSetAttribute(product_tc_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Plan<NT>::kBytes);
+        if (e == cudaSuccess && device < 64) configured[device] = true;
+    }
+    if (e == cudaSuccess)
+        e = launch_pdl(product_tc_kernel<T, NT>, dim3(static_cast<unsigned>(std::min<int64_t>(tiles, sms))), dim3(kThreads),
+                       Plan<NT>::kBytes, s, g, maps);
+    return e == cudaSuccess ? DN_OK : dn_cuda_fail(e, "linear8: product launch");
+}
+
+// The widest tile whose accumulators fit and that still gives every SM a tile.
+int tile_width(const ProductArgs& p, int sms) {
+    const int64_t m_tiles = (p.rows + kRows - 1) / kRows;
+    const int least = p.gate ? 64 : 32;
+    int nt = 256;
+    while (nt > least && p.segs * nt > 512) nt >>= 1;
+    while (nt > least) {
+        const int oc = p.gate ? nt / 2 : nt;
+        if (oc / 2 >= p.n_out || m_tiles * ((p.n_out + oc - 1) / oc) < sms)
+            nt >>= 1;
+        else
+            break;
+    }
+    return nt;
+}
+
+template <typename T>
+int run_type(TcArgs& g, int nt, int sms, cudaStream_t s) {
+    switch (nt) {
+        case 32: return run<T, 32>(g, sms, s);
+        case 64: return run<T, 64>(g, sms, s);
+        case 128: return run<T, 128>(g, sms, s);
+        default: return run<T, 256>(g, sms, s);
+    }
+}
+
+}  // namespace
+
+int launch_product_tc(const ProductArgs& a, int out_dtype, int sms, cudaStream_t s) {
+    TcArgs g{};
+    g.p = a;
+    const int nt = tile_width(a, sms);
+    return out_dtype == 1 ? run_type<__half>(g, nt, sms, s) : run_type<float>(g, nt, sms, s);
+}
+
+}  // namespace dnb

@@ -431,7 +431,7 @@ def test_planes(Q, n_img, k, h, w, n, gate):
 
 @gpu
 @pytest.mark.parametrize("frames,rows,cols,n", [(1, 1, 16, 2), (1, 200, 64, 64), (2, 129, 20, 6), (3, 1003, 96, 100),
-                                                (5, 640, 64, 64), (5, 300, 32, 32), (7, 128, 33, 130), (16, 70, 48, 34),
+                                                (5, 640, 64, 64), (5, 300, 32, 32), (7, 128, 33, 130), (8, 70, 48, 34),
                                                 (4, 257, 200, 300), (2, 500, 512, 512), (8, 390, 128, 256),
                                                 (1, 333, 260, 260), (3, 64, 8, 16)])
 @pytest.mark.parametrize("gate", [False, True])
