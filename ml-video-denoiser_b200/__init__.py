@@ -133,7 +133,7 @@ SIGNATURES = {
     "dn_linear8_create_device": (_I, [_P, _I, _I64, _P, _I, _I, _I, _I, _I, _P, _PP]),
     "dn_linear8_destroy": (_I, [_P]),
     "dn_linear8_info": (_I, [_P, _IP, _IP, _IP, _IP]),
-    "dn_linear8_workspace": (_I, [_P, _I64, _I, _I64P]),
+    "dn_linear8_workspace": (_I, [_P, _I64, _I, _I, _I64P]),
     "dn_linear8_forward": (_I, [_P, _P, _I, _I64, _I64, _P, _I, _I64, _P, _I64, _P]),
     "dn_linear8_forward_nchw": (_I, [_P, _P, _I, _I, _I, _P, _P, _I64, _P]),
     "dn_linear8_forward_cached": (_I, [_P, _P, _I64, _P, _I64, _I64, _I64P, _I, _I64, _P, _I, _I64, _P]),

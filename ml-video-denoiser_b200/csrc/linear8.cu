@@ -180,10 +180,21 @@ int check_matrix(const void* p, int dtype, int64_t rows, int64_t ld, int64_t col
     return DN_OK;
 }
 
-int64_t workspace_bytes_of(const dn_linear8* L, int64_t rows) { return rows * (round16(L->cin) + 4); }
+// How the product of `rows` tokens runs. One pass where the tokens are few or
+// the layer is narrow; otherwise the tokens are quantised into the workspace
+// and the product reads their codes.
+enum class Path { kFew, kFused, kTwoPass };
 
-int check_workspace(const dn_linear8* L, int64_t rows, const void* ws, int64_t bytes, const char* what) {
-    const int64_t need = workspace_bytes_of(L, rows);
+Path path_of(const ProductArgs& a, int dtype) {
+    if (product_few_takes(a)) return Path::kFew;
+    return dtype == 1 && product_fused_takes(a) ? Path::kFused : Path::kTwoPass;
+}
+
+int64_t workspace_bytes_of(const ProductArgs& a, int dtype) {
+    return path_of(a, dtype) == Path::kTwoPass ? a.rows * (round16(a.seg_c) + 4) : 0;
+}
+
+int check_workspace(int64_t need, const void* ws, int64_t bytes, const char* what) {
     if (need == 0) return DN_OK;
     if (!ws || bytes < need)
         return dn_fail_str(DN_ERR_INVALID_ARG, std::string(what) + ": the workspace holds " + std::to_string(ws ? bytes : 0) +
@@ -261,11 +272,14 @@ int dn_linear8_info(const dn_linear8* L, int* out_channels, int* in_channels, in
     return DN_OK;
 }
 
-int dn_linear8_workspace(const dn_linear8* L, int64_t rows, int dtype, int64_t* bytes) {
+int dn_linear8_workspace(const dn_linear8* L, int64_t rows, int dtype, int nchw, int64_t* bytes) {
     if (!L || !bytes) return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_workspace: null argument");
     if (rows < 0 || rows >= (1LL << 31)) return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_workspace: rows outside [0, 2^31)");
     if (dtype != 0 && dtype != 1) return dn_fail(DN_ERR_DTYPE, "dn_linear8_workspace: dtype must be 0 (FP32) or 1 (FP16)");
-    *bytes = workspace_bytes_of(L, rows);
+    ProductArgs a = product_args(L);
+    a.rows = rows;
+    a.planes = nchw ? 1 : 0;
+    *bytes = workspace_bytes_of(a, dtype);
     return DN_OK;
 }
 
@@ -277,10 +291,16 @@ int dn_linear8_forward(dn_linear8* L, const void* x, int dtype, int64_t ldx, int
     DN_TRY(check_matrix(x, dtype, rows, ldx, L->cin, name));
     DN_TRY(check_matrix(out, out_dtype, rows, ldo, L->n_out(), name));
     if (rows == 0) return DN_OK;
-    DN_TRY(check_workspace(L, rows, workspace, workspace_bytes, name));
+    ProductArgs a = product_args(L);
+    a.rows = rows;
+    a.out = out;
+    a.ldo = ldo;
+    DN_TRY(check_workspace(workspace_bytes_of(a, dtype), workspace, workspace_bytes, name));
     DeviceScope scope(L->device);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    ProductArgs a = product_args(L);
+    const Path path = path_of(a, dtype);
+    if (path == Path::kFew) return launch_product_few(a, x, dtype, ldx, out_dtype, L->sms, s);
+    if (path == Path::kFused) return launch_product_fused(a, x, ldx, out_dtype, L->sms, s);
     a.lda = round16(L->cin);
     auto* codes = static_cast<uint8_t*>(workspace);
     auto* scales = reinterpret_cast<float*>(codes + rows * a.lda);
@@ -290,9 +310,6 @@ int dn_linear8_forward(dn_linear8* L, const void* x, int dtype, int64_t ldx, int
     a.a = reinterpret_cast<const int8_t*>(codes);
     a.as = scales;
     a.a_rows = rows;
-    a.rows = rows;
-    a.out = out;
-    a.ldo = ldo;
     return launch_product_tc(a, out_dtype, L->sms, s);
 }
 
@@ -308,10 +325,15 @@ int dn_linear8_forward_nchw(dn_linear8* L, const void* input, int N, int H, int 
     DN_TRY(check_matrix(input, 1, rows, L->cin, L->cin, name));
     DN_TRY(check_matrix(output, 1, rows, L->n_out(), L->n_out(), name));
     if (rows == 0) return DN_OK;
-    DN_TRY(check_workspace(L, rows, workspace, workspace_bytes, name));
+    ProductArgs a = product_args(L);
+    a.rows = rows;
+    a.out = output;
+    a.ldo = hw;
+    a.planes = 1;
+    DN_TRY(check_workspace(workspace_bytes_of(a, 1), workspace, workspace_bytes, name));
     DeviceScope scope(L->device);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    ProductArgs a = product_args(L);
+    if (path_of(a, 1) == Path::kFused) return launch_product_fused(a, input, 0, 1, L->sms, s);
     a.lda = round16(L->cin);
     auto* codes = static_cast<uint8_t*>(workspace);
     auto* scales = reinterpret_cast<float*>(codes + rows * a.lda);
@@ -321,10 +343,6 @@ int dn_linear8_forward_nchw(dn_linear8* L, const void* input, int N, int H, int 
     a.a = reinterpret_cast<const int8_t*>(codes);
     a.as = scales;
     a.a_rows = rows;
-    a.rows = rows;
-    a.out = output;
-    a.ldo = hw;
-    a.planes = 1;
     return launch_product_tc(a, 1, L->sms, s);
 }
 

@@ -1,0 +1,84 @@
+// Device pieces shared by the tensor-core kernels of the 8-bit product
+// (linear8_tc.cu, linear8_fused.cu), and the tensor maps they use.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cudaTypedefs.h>
+
+#include <cstdint>
+
+#include "sm100.cuh"
+
+namespace dnb {
+
+// A tensor map over a [rows][cols] matrix of `esz`-byte elements, row stride
+// ld elements, boxes of box_rows x box_cols swizzled by their width (32, 64 or
+// 128 bytes). Base and row stride are multiples of 16 bytes.
+int linear8_map(CUtensorMap* m, CUtensorMapDataType type, int esz, const void* base, int64_t cols, int64_t rows,
+                int64_t ld, int box_cols, int box_rows);
+
+__host__ __device__ constexpr uint32_t idesc_s8(int M, int N) {
+    return (2u << 4)                                 // D: s32
+           | (1u << 7) | (1u << 10)                  // A, B: s8
+           | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_s8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                       uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, int (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+        "%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+
+__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+
+// 16 bytes of a row from 8 (FP16) or 4 (FP32) values.
+__device__ __forceinline__ uint4 pack16(const float* y, __half*) {
+    return make_uint4(pack_half2(y[0], y[1]), pack_half2(y[2], y[3]), pack_half2(y[4], y[5]), pack_half2(y[6], y[7]));
+}
+__device__ __forceinline__ uint4 pack16(const float* y, float*) {
+    return make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
+}
+
+// 32 values of a row, columns c .. c + 31 of n_out, stored directly.
+template <typename T>
+__device__ __forceinline__ void store_row32(T* o, const float (&y)[32], int c, int n_out, bool vec) {
+    constexpr int kVec = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 32; i += kVec) {
+        if (vec && c + i + kVec <= n_out) {
+            *reinterpret_cast<uint4*>(o + i) = pack16(y + i, static_cast<T*>(nullptr));
+        } else {
+#pragma unroll
+            for (int k = 0; k < kVec; ++k)
+                if (c + i + k < n_out) put(o + i + k, y[i + k]);
+        }
+    }
+}
+
+// 32 channels of a pixel into planes of `plane` pixels; o: channel c's value.
+template <typename T>
+__device__ __forceinline__ void store_planes32(T* o, int64_t plane, const float (&y)[32], int c, int n_out) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+        if (c + i < n_out) put(o + i * plane, y[i]);
+}
+
+}  // namespace dnb

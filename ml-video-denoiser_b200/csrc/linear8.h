@@ -32,4 +32,14 @@ struct ProductArgs {
 // current device.
 int launch_product_tc(const ProductArgs& a, int out_dtype, int sms, cudaStream_t s);
 
+// One pass over FP16 tokens (rows with stride ldx, or planes) of a narrow
+// layer; a.a, a.lda and a.as are not used. `takes` goes by sizes alone.
+bool product_fused_takes(const ProductArgs& a);
+int launch_product_fused(const ProductArgs& a, const void* x, int64_t ldx, int out_dtype, int sms, cudaStream_t s);
+
+// One pass over a few token rows.
+bool product_few_takes(const ProductArgs& a);
+int launch_product_few(const ProductArgs& a, const void* x, int dtype, int64_t ldx, int out_dtype, int sms,
+                       cudaStream_t s);
+
 }  // namespace dnb

@@ -1,0 +1,189 @@
+// The 8-bit product of a few tokens (serving one token at a time): one launch
+// that quantises the tokens and streams the weight once. Bound by the weight's
+// bytes (Cout * Cin) where it is large, by latency where it is small.
+//
+// Every CTA quantises all tokens into shared memory itself (a few KB out of
+// L2), behind the loads of its first weight bytes; a warp then takes CPW
+// weight rows at a time, a lane 16 bytes of each, and R tokens with dp4a:
+// each weight byte is used R times from registers, and the int32 sums meet in
+// one warp-wide reduction per (token, channel).
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "denoiser_b200.h"
+#include "launch.cuh"
+#include "linear8.cuh"
+#include "linear8.h"
+#include "quant.cuh"
+#include "status.h"
+
+namespace dnb {
+namespace {
+
+constexpr int kThreads = 128;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxTokens = 8;
+constexpr int kMaxBytes = 64 * 1024;  // codes of all tokens in shared memory
+
+struct FewArgs {
+    ProductArgs p;
+    const void* x;
+    int64_t ldx;
+    int vec_in;   // 16-byte loads of x are aligned
+    int out_f32;
+};
+
+template <typename T, int R, int CPW>
+__global__ void __launch_bounds__(kThreads) product_few_kernel(const __grid_constant__ FewArgs g) {
+    using Q = QuantOf<T>;
+    const ProductArgs& p = g.p;
+    extern __shared__ __align__(16) uint8_t s_codes[];  // [R][ldw]
+    __shared__ uint32_t s_mag[R];
+    __shared__ float s_scale[R];
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int K = p.seg_c, vecs = static_cast<int>(p.ldw / 16);
+    // The warp's weight rows: slots 0 .. CPW-1 are channels c0 ..; of a gated
+    // layer slot 2 i and 2 i + 1 are the two factors of output c0 + i.
+    const int outs = p.gate ? CPW / 2 : CPW;
+    const int c0 = (blockIdx.x * kWarps + (tid >> 5)) * outs;
+    const int8_t* w[CPW];
+#pragma unroll
+    for (int j = 0; j < CPW; ++j) {
+        const int c = p.gate ? c0 + j / 2 : c0 + j;
+        // Slots behind the last channel repeat it; their sums are not stored.
+        w[j] = p.w + static_cast<int64_t>(min(c, p.n_out - 1) + (p.gate && (j & 1) ? p.n_out : 0)) * p.ldw;
+    }
+    uint4 wv[CPW];
+#pragma unroll
+    for (int j = 0; j < CPW; ++j)
+        wv[j] = lane < vecs ? __ldg(reinterpret_cast<const uint4*>(w[j]) + lane) : make_uint4(0, 0, 0, 0);
+    if (tid < R) s_mag[tid] = 0;
+    __syncthreads();
+    pdl_trigger();
+    pdl_wait();
+
+    const T* x = static_cast<const T*>(g.x);
+    const int rows = static_cast<int>(p.rows);
+    const int groups = (K + 7) / 8;
+    auto load = [&](int r, int k) {
+        const T* src = x + r * g.ldx + k * 8;
+        return g.vec_in ? Q::load(src) : Q::load_some(src, min(8, K - k * 8));
+    };
+    for (int r = 0; r < rows; ++r) {
+        uint32_t mag = 0;
+        for (int k = tid; k < groups; k += kThreads) mag = max(mag, Q::mag(load(r, k)));
+        mag = __reduce_max_sync(0xffffffffu, mag);
+        if (lane == 0) atomicMax(&s_mag[r], mag);
+    }
+    __syncthreads();
+    for (int r = 0; r < R; ++r) {
+        const GroupScale q = group_scale<T>(r < rows ? s_mag[r] : 0u, 127.f);
+        if (tid == 0) s_scale[r] = q.s;
+        const bool fix = !Q::kF32 && q.fix != 0.f;  // the same on every thread
+        for (int k = tid; k < vecs * 2; k += kThreads)
+            *reinterpret_cast<uint2*>(s_codes + r * p.ldw + k * 8) =
+                codes8<T>(r < rows && k < groups ? load(r, k) : Q::zero(), q, fix);
+    }
+    __syncthreads();
+
+    int acc[R][CPW];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < CPW; ++j) acc[r][j] = 0;
+    for (int v = lane; v < vecs; v += 32) {
+        uint4 cur[CPW];
+#pragma unroll
+        for (int j = 0; j < CPW; ++j) {
+            cur[j] = wv[j];
+            if (v + 32 < vecs) wv[j] = __ldg(reinterpret_cast<const uint4*>(w[j]) + v + 32);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const uint4 a = *reinterpret_cast<const uint4*>(s_codes + r * p.ldw + v * 16);
+#pragma unroll
+            for (int j = 0; j < CPW; ++j) {
+                int s = __dp4a(static_cast<int>(a.x), static_cast<int>(cur[j].x), acc[r][j]);
+                s = __dp4a(static_cast<int>(a.y), static_cast<int>(cur[j].y), s);
+                s = __dp4a(static_cast<int>(a.z), static_cast<int>(cur[j].z), s);
+                acc[r][j] = __dp4a(static_cast<int>(a.w), static_cast<int>(cur[j].w), s);
+            }
+        }
+    }
+    // Sums over the warp; lane r * CPW + j keeps that of token r, slot j.
+    int mine = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < CPW; ++j) {
+            const int s = __reduce_add_sync(0xffffffffu, acc[r][j]);
+            if (lane == r * CPW + j) mine = s;
+        }
+    const int r = lane / CPW, j = lane % CPW;
+    const int o = p.gate ? c0 + j / 2 : c0 + j;
+    const bool in = r < R && o < p.n_out;
+    const int c = o + (p.gate && (j & 1) ? p.n_out : 0);
+    float y = 0.f;
+    if (in) y = fmaf(static_cast<float>(mine) * s_scale[r], p.ws[c], p.bias ? p.bias[c] : 0.f);
+    if (p.gate) y *= __shfl_down_sync(0xffffffffu, y, 1);
+    if (in && r < rows && !(p.gate && (j & 1))) {
+        if (g.out_f32)
+            static_cast<float*>(p.out)[r * p.ldo + o] = y;
+        else
+            static_cast<__half*>(p.out)[r * p.ldo + o] = __float2half_rn(y);
+    }
+}
+
+template <typename T, int R, int CPW>
+cudaError_t run(const FewArgs& g, cudaStream_t s) {
+    const int per = kWarps * (g.p.gate ? CPW / 2 : CPW);
+    const size_t smem = static_cast<size_t>(R) * g.p.ldw;
+    if (smem > 32 * 1024) {
+        static bool configured[64] = {};
+        int device = 0;
+        cudaError_t e = cudaGetDevice(&device);
+        if (e == cudaSuccess && (device >= 64 || !configured[device])) {
+            e = cudaFuncSetAttribute(product_few_kernel<T, R, CPW>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxBytes);
+            if (e == cudaSuccess && device < 64) configured[device] = true;
+        }
+        if (e != cudaSuccess) return e;
+    }
+    return launch_pdl(product_few_kernel<T, R, CPW>, dim3((g.p.n_out + per - 1) / per), dim3(kThreads), smem, s, g);
+}
+
+template <typename T, int R>
+cudaError_t run_cpw(const FewArgs& g, int sms, cudaStream_t s) {
+    // Four weight rows a warp where that still gives every SM two CTAs.
+    return g.p.cout >= 2 * sms * kWarps * 4 ? run<T, R, 4>(g, s) : run<T, R, 2>(g, s);
+}
+
+template <typename T>
+cudaError_t run_rows(const FewArgs& g, int sms, cudaStream_t s) {
+    if (g.p.rows == 1) return run_cpw<T, 1>(g, sms, s);
+    if (g.p.rows == 2) return run_cpw<T, 2>(g, sms, s);
+    if (g.p.rows <= 4) return run_cpw<T, 4>(g, sms, s);
+    return run_cpw<T, 8>(g, sms, s);
+}
+
+}  // namespace
+
+bool product_few_takes(const ProductArgs& a) {
+    const int64_t r = a.rows <= 2 ? a.rows : a.rows <= 4 ? 4 : 8;
+    return a.rows <= kMaxTokens && !a.planes && a.segs == 1 && r * a.ldw <= kMaxBytes;
+}
+
+int launch_product_few(const ProductArgs& a, const void* x, int dtype, int64_t ldx, int out_dtype, int sms,
+                       cudaStream_t s) {
+    FewArgs g{};
+    g.p = a;
+    g.x = x;
+    g.ldx = ldx;
+    g.out_f32 = out_dtype == 0;
+    g.vec_in = a.seg_c % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * (dtype == 1 ? 2 : 4) % 16 == 0;
+    const cudaError_t e = dtype == 1 ? run_rows<__half>(g, sms, s) : run_rows<float>(g, sms, s);
+    return e == cudaSuccess ? DN_OK : dn_cuda_fail(e, "linear8: launch over a few tokens");
+}
+
+}  // namespace dnb

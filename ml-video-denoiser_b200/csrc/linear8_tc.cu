@@ -19,16 +19,15 @@
 //               are stored directly).
 // A segment's int32 sum is exact; it is scaled once, in FP32. Every wait is
 // bounded.
-#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
-#include <cudaTypedefs.h>
 
 #include <algorithm>
 #include <string>
 
 #include "denoiser_b200.h"
 #include "launch.cuh"
+#include "linear8.cuh"
 #include "linear8.h"
 #include "sm100.cuh"
 #include "status.h"
@@ -65,34 +64,6 @@ struct TcArgs {
     int vec_out;         // direct stores: 16-byte vectors of a row are aligned
 };
 
-__host__ __device__ constexpr uint32_t idesc_s8(int M, int N) {
-    return (2u << 4)                                 // D: s32
-           | (1u << 7) | (1u << 10)                  // A, B: s8
-           | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
-}
-
-__device__ __forceinline__ void mma_s8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                       uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, int (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
-        "%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
-}
-
 // sum_t s_t acc_t of 32 columns, then the channels' scale and bias (columns
 // past the layer's are not stored; their parameters are not read).
 __device__ __forceinline__ void scaled32(const TcArgs& g, uint32_t taddr, int nt, int64_t row, bool live, int c0,
@@ -113,17 +84,6 @@ __device__ __forceinline__ void scaled32(const TcArgs& g, uint32_t taddr, int nt
         const float w = in ? __ldg(p.ws + c) : 0.f, b = in && p.bias ? __ldg(p.bias + c) : 0.f;
         y[i] = fmaf(y[i], w, b);
     }
-}
-
-__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void put(float* p, float v) { *p = v; }
-
-// 16 bytes of a row from 8 (FP16) or 4 (FP32) values.
-__device__ __forceinline__ uint4 pack16(const float* y, __half*) {
-    return make_uint4(pack_half2(y[0], y[1]), pack_half2(y[2], y[3]), pack_half2(y[4], y[5]), pack_half2(y[6], y[7]));
-}
-__device__ __forceinline__ uint4 pack16(const float* y, float*) {
-    return make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
 }
 
 template <typename T, int NT>
@@ -274,23 +234,10 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
                             *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) =
                                 pack16(y + i, static_cast<T*>(nullptr));
                         }
-                    } else if (p.planes) {
-                        T* o = out + (img * p.n_out + n0 + c) * p.ldo + (row - img * p.ldo);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (live && n0 + c + i < p.n_out) put(o + i * p.ldo, y[i]);
+                    } else if (live && p.planes) {
+                        store_planes32(out + (img * p.n_out + n0 + c) * p.ldo + (row - img * p.ldo), p.ldo, y, n0 + c, p.n_out);
                     } else if (live) {
-                        T* o = out + row * p.ldo + n0 + c;
-#pragma unroll
-                        for (int i = 0; i < 32; i += kVec) {
-                            if (g.vec_out && n0 + c + i + kVec <= p.n_out) {
-                                *reinterpret_cast<uint4*>(o + i) = pack16(y + i, static_cast<T*>(nullptr));
-                            } else {
-#pragma unroll
-                                for (int k = 0; k < kVec; ++k)
-                                    if (n0 + c + i + k < p.n_out) put(o + i + k, y[i + k]);
-                            }
-                        }
+                        store_row32(out + row * p.ldo + n0 + c, y, n0 + c, p.n_out, g.vec_out);
                     }
                 }
                 if (g.tma_out) {
@@ -313,25 +260,6 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
     if (warp == 10) tmem_dealloc(tmem, cols);
 }
 
-int encode(CUtensorMap* m, CUtensorMapDataType type, int esz, const void* base, int64_t cols, int64_t rows, int64_t ld,
-           int box_cols, int box_rows) {
-    auto fn = tensor_map_encoder();
-    if (!fn) return dn_fail(DN_ERR_CUDA, "linear8: cuTensorMapEncodeTiled unavailable");
-    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * esz};
-    const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
-    const cuuint32_t estr[2] = {1, 1};
-    const int span = box_cols * esz;
-    const CUtensorMapSwizzle swz = span == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
-                                   : span == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                                : CU_TENSOR_MAP_SWIZZLE_32B;
-    const CUresult r = fn(m, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          swz, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS)
-        return dn_fail_str(DN_ERR_CUDA, "linear8: cuTensorMapEncodeTiled failed (" + std::to_string(r) + ")");
-    return DN_OK;
-}
-
 template <typename T, int NT>
 int run(TcArgs& g, int sms, cudaStream_t s) {
     const ProductArgs& p = g.p;
@@ -341,15 +269,15 @@ int run(TcArgs& g, int sms, cudaStream_t s) {
     g.m_tiles = static_cast<int>((p.rows + kRows - 1) / kRows);
     g.n_tiles = (p.n_out + out_cols - 1) / out_cols;
     g.bufs = 2 * p.segs * NT <= 512 ? 2 : 1;
-    const bool al16 = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo * sizeof(T) % 16 == 0;
+    const bool al16 = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo * sizeof(T) % 16 == 0 && p.ldo >= p.n_out;
     // A TMA store moves 128 bytes of a row; narrower tiles and planes go directly.
     g.tma_out = !p.planes && al16 && out_cols * sizeof(T) >= 128;
     g.vec_out = !p.planes && al16;
     Maps maps{};
-    DN_TRY(encode(&maps.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.a, p.seg_c, p.a_rows, p.lda, g.kc, kRows));
-    DN_TRY(encode(&maps.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.ldw, p.cout, p.ldw, g.kc, p.gate ? NT / 2 : NT));
+    DN_TRY(linear8_map(&maps.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.a, p.seg_c, p.a_rows, p.lda, g.kc, kRows));
+    DN_TRY(linear8_map(&maps.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.ldw, p.cout, p.ldw, g.kc, p.gate ? NT / 2 : NT));
     if (g.tma_out)
-        DN_TRY(encode(&maps.out, sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+        DN_TRY(linear8_map(&maps.out, sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
                       sizeof(T), p.out, p.n_out, p.rows, p.ldo, 128 / sizeof(T), 32));
     const int64_t tiles = static_cast<int64_t>(g.m_tiles) * g.n_tiles;
     if (tiles >= (1LL << 30)) return dn_fail(DN_ERR_UNSUPPORTED, "linear8: the product has 2^30 tiles or more");
@@ -393,6 +321,25 @@ int run_type(TcArgs& g, int nt, int sms, cudaStream_t s) {
 }
 
 }  // namespace
+
+int linear8_map(CUtensorMap* m, CUtensorMapDataType type, int esz, const void* base, int64_t cols, int64_t rows,
+                int64_t ld, int box_cols, int box_rows) {
+    auto fn = tensor_map_encoder();
+    if (!fn) return dn_fail(DN_ERR_CUDA, "linear8: cuTensorMapEncodeTiled unavailable");
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * esz};
+    const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
+    const cuuint32_t estr[2] = {1, 1};
+    const int span = box_cols * esz;
+    const CUtensorMapSwizzle swz = span == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                   : span == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                : CU_TENSOR_MAP_SWIZZLE_32B;
+    const CUresult r = fn(m, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          swz, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return dn_fail_str(DN_ERR_CUDA, "linear8: cuTensorMapEncodeTiled failed (" + std::to_string(r) + ")");
+    return DN_OK;
+}
 
 int launch_product_tc(const ProductArgs& a, int out_dtype, int sms, cudaStream_t s) {
     TcArgs g{};

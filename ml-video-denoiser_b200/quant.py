@@ -19,7 +19,9 @@ from __future__ import annotations
 import contextlib
 import ctypes
 
-from . import DN_ERR_DTYPE, DN_ERR_INVALID_ARG, DenoiserError, InvalidArgumentError, Weights, check, lib
+import torch
+
+from . import DN_ERR_DEVICE, DN_ERR_DTYPE, DN_ERR_INVALID_ARG, DenoiserError, InvalidArgumentError, Weights, check, lib
 
 
 def _bad(msg: str):
@@ -28,18 +30,14 @@ def _bad(msg: str):
 
 def _code(dtype, what: str) -> int:
     """The C-ABI's number of a torch dtype."""
-    import torch
-
-    if dtype == torch.float16:
+    if dtype is torch.float16:
         return 1
-    if dtype == torch.float32:
+    if dtype is torch.float32:
         return 0
     raise DenoiserError(DN_ERR_DTYPE, f"{what}: expected FP16 or FP32, got {dtype}")
 
 
 def _device_of(device) -> int:
-    import torch
-
     d = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
     if d.type != "cuda":
         _bad("the operators run on CUDA devices")
@@ -48,31 +46,41 @@ def _device_of(device) -> int:
 
 @contextlib.contextmanager
 def _on(device: int, stream):
-    """`device` and `stream` made current (so that what a call allocates
-    belongs to them); yields the cudaStream_t."""
-    import torch
-
+    """`device` and `stream` made current, so that what a call allocates
+    belongs to them. The methods below come back through here when they are
+    not on their device, or were given a stream."""
     with torch.cuda.device(device):
         s = stream if stream is not None else torch.cuda.current_stream(device)
         if s.device.index != device:
             _bad(f"the stream is of device {s.device.index}, the operator of device {device}")
         with torch.cuda.stream(s):
-            yield s.cuda_stream
+            yield
+
+
+def _elsewhere(device: int, stream) -> bool:
+    return stream is not None or torch.cuda.current_device() != device
+
+
+def _stream(device: int) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def _on_device(t, device: int, what: str) -> None:
-    if not t.is_cuda or t.device.index != device:
+    if t.get_device() != device:
         _bad(f"{what} must be a tensor on cuda:{device}")
 
 
 def _matrix(t, rows: int | None, cols: int, device: int, what: str) -> int:
     """Row stride of a 2-D tensor with unit column stride."""
-    _on_device(t, device, what)
-    if t.dim() != 2 or t.shape[1] != cols or (rows is not None and t.shape[0] != rows):
-        _bad(f"{what} must be ({'rows' if rows is None else rows}, {cols}), got {tuple(t.shape)}")
-    if cols > 1 and t.shape[0] > 0 and t.stride(1) != 1:
+    if t.get_device() != device:
+        _bad(f"{what} must be a tensor on cuda:{device}")
+    shape = t.shape
+    if len(shape) != 2 or shape[1] != cols or (rows is not None and shape[0] != rows):
+        _bad(f"{what} must be ({'rows' if rows is None else rows}, {cols}), got {tuple(shape)}")
+    ld, one = t.stride()
+    if one != 1 and cols > 1 and shape[0] > 0:
         _bad(f"{what}: the columns must be adjacent (stride 1)")
-    return t.stride(0) if t.shape[0] > 1 else cols
+    return ld if shape[0] > 1 else cols
 
 
 class RowCache:
@@ -81,8 +89,6 @@ class RowCache:
     and ``scales`` are the tensors it is held in; new rows read as zeros."""
 
     def __init__(self, pages: int, page_rows: int, cols: int, bits: int = 8, group: int = 0, device=0):
-        import torch
-
         if pages < 0 or page_rows < 1 or cols < 1:
             _bad("RowCache: pages >= 0, page_rows >= 1 and cols >= 1 are needed")
         if bits not in (8, 4):
@@ -100,15 +106,12 @@ class RowCache:
         self.codes = torch.zeros(self.capacity, row, dtype=torch.uint8, device=d)
         self.scales = torch.zeros(self.capacity, cols // group, dtype=torch.float32, device=d)
         self._err = torch.zeros(1, dtype=torch.int32, device=d)
-
-    def _held(self):
-        return self.codes.data_ptr(), self.codes.shape[1], self.scales.data_ptr(), self.capacity
+        self._held = (self.codes.data_ptr(), row, self.scales.data_ptr(), self.capacity)
+        self._err_ptr = self._err.data_ptr()
 
     def _slots(self, slots, rows: int | None):
-        import torch
-
         _on_device(slots, self.device, "RowCache: slots")
-        if slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
+        if slots.dtype is not torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
             _bad("RowCache: slots must be a contiguous 1-D int64 tensor")
         if rows is not None and slots.shape[0] != rows:
             _bad(f"RowCache: {slots.shape[0]} slots for {rows} rows")
@@ -120,35 +123,38 @@ class RowCache:
         Rows with a negative slot are skipped; a slot at or behind the capacity
         is skipped and reported by ``sync``. Of rows with the same slot the
         last one is held."""
+        if _elsewhere(self.device, stream):
+            with _on(self.device, stream):
+                return self.write(x, slots, row0)
         dtype = _code(x.dtype, "RowCache.write")
         ldx = _matrix(x, None, self.cols, self.device, "RowCache.write: x")
-        p = None if slots is None else self._slots(slots, x.shape[0])
-        codes, ld, scales, cap = self._held()
-        with _on(self.device, stream) as s:
-            check(lib().dn_launch_cache_write(x.data_ptr(), dtype, ldx, x.shape[0], self.cols, p, row0, codes, ld,
-                                              scales, cap, self.bits, self.group, self._err.data_ptr(), s))
+        rows = x.shape[0]
+        codes, ld, scales, cap = self._held
+        check(lib().dn_launch_cache_write(
+            x.data_ptr(), dtype, ldx, rows, self.cols, None if slots is None else self._slots(slots, rows), row0, codes,
+            ld, scales, cap, self.bits, self.group, self._err_ptr, _stream(self.device)))
 
     def read_rows(self, slots=None, row0: int = 0, rows: int | None = None, out=None, dtype=None, stream=None):
         """Cache rows ``slots`` (int64 CUDA tensor), or the ``rows`` rows from
         ``row0`` on -> (rows, cols) in ``dtype`` (default FP16) or into
         ``out``. Out rows of a skipped slot (see ``write``) stay as they were;
         without ``out`` they are zeros."""
-        import torch
-
-        if slots is None and rows is None:
-            _bad("RowCache.read_rows: slots or rows is needed")
-        n = rows if slots is None else slots.shape[0]
-        if n < 0:
-            _bad("RowCache.read_rows: rows is negative")
-        p = None if slots is None else self._slots(slots, rows)
-        codes, ld, scales, cap = self._held()
-        with _on(self.device, stream) as s:
-            if out is None:
-                out = torch.zeros(n, self.cols, dtype=dtype or torch.float16, device=self.codes.device)
-            code = _code(out.dtype, "RowCache.read_rows")
-            ldo = _matrix(out, n, self.cols, self.device, "RowCache.read_rows: out")
-            check(lib().dn_launch_cache_read_rows(codes, ld, scales, cap, self.cols, self.bits, self.group, p, row0, n,
-                                                  out.data_ptr(), code, ldo, self._err.data_ptr(), s))
+        if _elsewhere(self.device, stream):
+            with _on(self.device, stream):
+                return self.read_rows(slots, row0, rows, out, dtype)
+        if slots is None:
+            if rows is None or rows < 0:
+                _bad("RowCache.read_rows: slots, or rows >= 0, is needed")
+            p, n = None, rows
+        else:
+            p, n = self._slots(slots, rows), slots.shape[0]
+        if out is None:
+            out = torch.zeros(n, self.cols, dtype=dtype or torch.float16, device=self.codes.device)
+        code = _code(out.dtype, "RowCache.read_rows")
+        ldo = _matrix(out, n, self.cols, self.device, "RowCache.read_rows: out")
+        codes, ld, scales, cap = self._held
+        check(lib().dn_launch_cache_read_rows(codes, ld, scales, cap, self.cols, self.bits, self.group, p, row0, n,
+                                              out.data_ptr(), code, ldo, self._err_ptr, _stream(self.device)))
         return out
 
     def read(self, table, lengths=None, out=None, dtype=None, stream=None):
@@ -159,46 +165,43 @@ class RowCache:
         i < lengths[b] (int32 CUDA tensor; default: all). What lies behind a
         sequence's length, and rows of a negative page, stay as they were;
         without ``out`` they are zeros."""
-        import torch
-
+        if _elsewhere(self.device, stream):
+            with _on(self.device, stream):
+                return self.read(table, lengths, out, dtype)
         _on_device(table, self.device, "RowCache.read: table")
-        if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        if table.dtype is not torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
             _bad("RowCache.read: table must be a 2-D int32 tensor with adjacent columns")
         b, n = table.shape
         if lengths is not None:
             _on_device(lengths, self.device, "RowCache.read: lengths")
-            if lengths.dtype != torch.int32 or lengths.shape != (b,) or not lengths.is_contiguous():
+            if lengths.dtype is not torch.int32 or lengths.shape != (b,) or not lengths.is_contiguous():
                 _bad(f"RowCache.read: lengths must be a contiguous int32 tensor ({b},)")
-        codes, ld, scales, cap = self._held()
-        with _on(self.device, stream) as s:
-            if out is None:
-                out = torch.zeros(b, n * self.page_rows, self.cols, dtype=dtype or torch.float16,
-                                  device=self.codes.device)
-            code = _code(out.dtype, "RowCache.read")
-            _on_device(out, self.device, "RowCache.read: out")
-            if out.dim() != 3 or out.shape[0] != b or out.shape[2] != self.cols:
-                _bad(f"RowCache.read: out must be ({b}, rows, {self.cols}), got {tuple(out.shape)}")
-            if self.cols > 1 and out.numel() and out.stride(2) != 1:
-                _bad("RowCache.read: out's columns must be adjacent (stride 1)")
-            check(lib().dn_launch_cache_read_pages(
-                codes, ld, scales, cap, self.cols, self.bits, self.group, self.page_rows, table.data_ptr(),
-                table.stride(0) if b > 1 else n, n, None if lengths is None else lengths.data_ptr(), b, out.shape[1],
-                out.data_ptr(), code, out.stride(0), out.stride(1) if out.shape[1] > 1 else self.cols,
-                self._err.data_ptr(), s))
+        if out is None:
+            out = torch.zeros(b, n * self.page_rows, self.cols, dtype=dtype or torch.float16, device=self.codes.device)
+        code = _code(out.dtype, "RowCache.read")
+        _on_device(out, self.device, "RowCache.read: out")
+        if out.dim() != 3 or out.shape[0] != b or out.shape[2] != self.cols:
+            _bad(f"RowCache.read: out must be ({b}, rows, {self.cols}), got {tuple(out.shape)}")
+        step, ldo, one = out.stride()
+        if one != 1 and self.cols > 1 and out.numel():
+            _bad("RowCache.read: out's columns must be adjacent (stride 1)")
+        codes, ld, scales, cap = self._held
+        check(lib().dn_launch_cache_read_pages(
+            codes, ld, scales, cap, self.cols, self.bits, self.group, self.page_rows, table.data_ptr(),
+            table.stride(0) if b > 1 else n, n, None if lengths is None else lengths.data_ptr(), b, out.shape[1],
+            out.data_ptr(), code, step, ldo if out.shape[1] > 1 else self.cols, self._err_ptr, _stream(self.device)))
         return out
 
     def sync(self, stream=None) -> None:
         """Synchronise the stream and raise if a call met a slot or page
         behind the cache since the last check."""
-        import torch
-
         with _on(self.device, stream):
             torch.cuda.current_stream(self.device).synchronize()
             word = int(self._err.item())
             if word:
                 self._err.zero_()
         if word:
-            raise DenoiserError(-7, f"RowCache: a slot or page lies behind the cache (device error word {word})")
+            raise DenoiserError(DN_ERR_DEVICE, f"RowCache: a slot or page lies behind the cache (error word {word:#x})")
 
 
 class Linear8:
@@ -233,10 +236,11 @@ class Linear8:
             _on_device(bias, self.device, "Linear8: bias")
             if bias.dtype != weight.dtype or bias.shape != (weight.shape[0],) or not bias.is_contiguous():
                 _bad(f"Linear8: bias must be a contiguous ({weight.shape[0]},) tensor of the weight's type")
-        with _on(self.device, stream) as s:
+        with _on(self.device, stream):
             check(lib().dn_linear8_create_device(weight.data_ptr(), dtype, ldw,
                                                  None if bias is None else bias.data_ptr(), weight.shape[0],
-                                                 weight.shape[1], int(gate), segments, self.device, s,
+                                                 weight.shape[1], int(gate), segments, self.device,
+                                                 _stream(self.device),
                                                  ctypes.byref(self._h)))
         self._info()
         return self
@@ -259,13 +263,12 @@ class Linear8:
         except Exception:
             pass
 
-    def _workspace(self, rows: int, dtype: int):
-        """Workspace of a call, from torch's allocator on the current stream:
-        the allocator keeps it from others until the stream is past the call."""
-        import torch
-
+    def _workspace(self, rows: int, dtype: int, nchw: int = 0):
+        """(address, bytes, tensor) of a call's workspace, from torch's
+        allocator on the current stream, which keeps it from others until the
+        stream is past the call."""
         n = ctypes.c_int64()
-        check(lib().dn_linear8_workspace(self._h, rows, dtype, ctypes.byref(n)))
+        check(lib().dn_linear8_workspace(self._h, rows, dtype, nchw, ctypes.byref(n)))
         if n.value == 0:
             return None, 0, None
         t = torch.empty(n.value, dtype=torch.uint8, device=torch.device("cuda", self.device))
@@ -274,19 +277,19 @@ class Linear8:
     def forward(self, x, out=None, out_dtype=None, stream=None):
         """Token rows x (rows, in_channels), FP16 or FP32, any row stride ->
         (rows, out_channels) in ``out_dtype`` (default: x's) or into ``out``."""
-        import torch
-
+        if _elsewhere(self.device, stream):
+            with _on(self.device, stream):
+                return self.forward(x, out, out_dtype)
         dtype = _code(x.dtype, "Linear8.forward")
         ldx = _matrix(x, None, self.in_channels, self.device, "Linear8.forward: x")
         rows = x.shape[0]
-        with _on(self.device, stream) as s:
-            if out is None:
-                out = torch.empty(rows, self.out_channels, dtype=out_dtype or x.dtype, device=x.device)
-            code = _code(out.dtype, "Linear8.forward: out")
-            ldo = _matrix(out, rows, self.out_channels, self.device, "Linear8.forward: out")
-            ws, n, _keep = self._workspace(rows, dtype)
-            check(lib().dn_linear8_forward(self._h, x.data_ptr(), dtype, ldx, rows, out.data_ptr(), code, ldo, ws, n,
-                                           s))
+        if out is None:
+            out = torch.empty(rows, self.out_channels, dtype=out_dtype or x.dtype, device=x.device)
+        code = _code(out.dtype, "Linear8.forward: out")
+        ldo = _matrix(out, rows, self.out_channels, self.device, "Linear8.forward: out")
+        ws, n, _keep = self._workspace(rows, dtype)
+        check(lib().dn_linear8_forward(self._h, x.data_ptr(), dtype, ldx, rows, out.data_ptr(), code, ldo, ws, n,
+                                       _stream(self.device)))
         return out
 
     __call__ = forward
@@ -294,31 +297,33 @@ class Linear8:
     def forward_nchw(self, x, out=None, stream=None):
         """A 1x1 convolution: x (N, in_channels, H, W) FP16 contiguous ->
         (N, out_channels, H, W) FP16, a scale for every pixel."""
-        import torch
-
-        if x.dtype != torch.float16:
+        if _elsewhere(self.device, stream):
+            with _on(self.device, stream):
+                return self.forward_nchw(x, out)
+        if x.dtype is not torch.float16:
             raise DenoiserError(DN_ERR_DTYPE, "Linear8.forward_nchw: expected FP16 input")
         _on_device(x, self.device, "Linear8.forward_nchw: x")
         if x.dim() != 4 or x.shape[1] != self.in_channels or not x.is_contiguous():
             _bad(f"Linear8.forward_nchw: x must be a contiguous (N, {self.in_channels}, H, W) tensor")
         n, _, h, w = x.shape
         shape = (n, self.out_channels, h, w)
-        with _on(self.device, stream) as s:
-            if out is None:
-                out = torch.empty(shape, dtype=torch.float16, device=x.device)
-            _on_device(out, self.device, "Linear8.forward_nchw: out")
-            if out.dtype != torch.float16 or tuple(out.shape) != shape or not out.is_contiguous():
-                _bad(f"Linear8.forward_nchw: out must be a contiguous FP16 tensor {shape}")
-            ws, nb, _keep = self._workspace(n * h * w, 1)
-            check(lib().dn_linear8_forward_nchw(self._h, x.data_ptr(), n, h, w, out.data_ptr(), ws, nb, s))
+        if out is None:
+            out = torch.empty(shape, dtype=torch.float16, device=x.device)
+        _on_device(out, self.device, "Linear8.forward_nchw: out")
+        if out.dtype is not torch.float16 or tuple(out.shape) != shape or not out.is_contiguous():
+            _bad(f"Linear8.forward_nchw: out must be a contiguous FP16 tensor {shape}")
+        ws, nb, _keep = self._workspace(n * h * w, 1, 1)
+        check(lib().dn_linear8_forward_nchw(self._h, x.data_ptr(), n, h, w, out.data_ptr(), ws, nb,
+                                            _stream(self.device)))
         return out
 
     def forward_cached(self, cache: RowCache, pages, rows: int | None = None, out=None, out_dtype=None, stream=None):
         """Straight from an 8-bit cache: ``segments`` pages (ints) side by
         side, the first ``rows`` rows of each (default: all) -> (rows,
         out_channels) in ``out_dtype`` (default FP16) or into ``out``."""
-        import torch
-
+        if _elsewhere(self.device, stream):
+            with _on(self.device, stream):
+                return self.forward_cached(cache, pages, rows, out, out_dtype)
         if cache.device != self.device:
             _bad("Linear8.forward_cached: cache and layer are on different devices")
         if cache.bits != 8 or cache.group != cache.cols:
@@ -330,19 +335,17 @@ class Linear8:
             rows = cache.page_rows
         if not 0 <= rows <= cache.page_rows:
             _bad(f"Linear8.forward_cached: {rows} rows of pages of {cache.page_rows}")
-        arr = (ctypes.c_int64 * len(pages))(*pages)
-        codes, ld, scales, cap = cache._held()
-        with _on(self.device, stream) as s:
-            if out is None:
-                out = torch.empty(rows, self.out_channels, dtype=out_dtype or torch.float16,
-                                  device=cache.codes.device)
-            code = _code(out.dtype, "Linear8.forward_cached: out")
-            ldo = _matrix(out, rows, self.out_channels, self.device, "Linear8.forward_cached: out")
-            check(lib().dn_linear8_forward_cached(self._h, codes, ld, scales, cap, cache.page_rows, arr, len(pages),
-                                                  rows, out.data_ptr(), code, ldo, s))
+        if out is None:
+            out = torch.empty(rows, self.out_channels, dtype=out_dtype or torch.float16, device=cache.codes.device)
+        code = _code(out.dtype, "Linear8.forward_cached: out")
+        ldo = _matrix(out, rows, self.out_channels, self.device, "Linear8.forward_cached: out")
+        codes, ld, scales, cap = cache._held
+        check(lib().dn_linear8_forward_cached(self._h, codes, ld, scales, cap, cache.page_rows,
+                                              (ctypes.c_int64 * len(pages))(*pages), len(pages), rows, out.data_ptr(),
+                                              code, ldo, _stream(self.device)))
         return out
 
     def sync(self, stream=None) -> None:
         """Synchronise the stream and raise if a kernel flagged a device error."""
-        with _on(self.device, stream) as s:
-            check(lib().dn_linear8_sync(self._h, s))
+        with _on(self.device, stream):
+            check(lib().dn_linear8_sync(self._h, _stream(self.device)))

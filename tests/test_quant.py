@@ -547,14 +547,14 @@ def test_calls_refuse(pkg, Q):
             f()
         assert e.value.code == pkg.DN_ERR_DTYPE
     lib, n = pkg.lib(), ctypes.c_int64()
-    big = torch.ones(600, 32, dtype=h, device="cuda")
+    big = torch.ones(600, 32, device="cuda")
     out = torch.empty(600, 6, dtype=h, device="cuda")
     for rows in (1, 600):
-        pkg.check(lib.dn_linear8_workspace(layer._h, rows, 1, ctypes.byref(n)))
+        pkg.check(lib.dn_linear8_workspace(layer._h, rows, 0, 0, ctypes.byref(n)))
         if n.value:
             ws = torch.empty(n.value + 16, dtype=torch.uint8, device="cuda")
             for p, size in ((None, n.value), (ws.data_ptr(), n.value - 1), (ws.data_ptr() + 4, n.value)):
-                assert lib.dn_linear8_forward(layer._h, big.data_ptr(), 1, 32, rows, out.data_ptr(), 1, 6, p, size,
+                assert lib.dn_linear8_forward(layer._h, big.data_ptr(), 0, 32, rows, out.data_ptr(), 1, 6, p, size,
                                               None) == pkg.DN_ERR_INVALID_ARG
 
 
