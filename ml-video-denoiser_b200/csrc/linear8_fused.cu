@@ -290,8 +290,13 @@ int run(FusedArgs& g, int sms, cudaStream_t s) {
     auto kernel = product_fused_kernel<T, PLANES, SG, NT>;
     if (e == cudaSuccess && per_sm == 0) {
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-        if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, S::kThreads, S::kSmem);
-        per_sm = std::max(1, std::min(per_sm, 512 / NT));  // an SM has 512 TMEM columns
+        cudaFuncAttributes at{};
+        if (e == cudaSuccess) e = cudaFuncGetAttributes(&at, kernel);
+        // By registers (allocated in eights a thread), shared memory (228 KB, 1 KB a CTA reserved) and TMEM (512
+        // columns); the occupancy query answers 1 for kernels that use TMEM.
+        const int by_regs = 65536 / (std::max(1, (at.numRegs + 7) / 8 * 8) * S::kThreads);
+        const int by_smem = 233472 / (S::kSmem + static_cast<int>(at.sharedSizeBytes) + 1024);
+        per_sm = std::max(1, std::min({by_regs, by_smem, 512 / NT}));
         if (e == cudaSuccess && device < 64) resident[device] = per_sm;
     }
     if (e == cudaSuccess)
