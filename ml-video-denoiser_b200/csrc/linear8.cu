@@ -48,9 +48,12 @@ __global__ void __launch_bounds__(256) quantise_planes_kernel(const __half* __re
     scales[m] = g.s;
 }
 
-__global__ void bias_kernel(const void* b, int dtype, float* out, int n) {
-    const int i = blockIdx.x * blockDim.x + threadIdx.x;
-    if (i < n) out[i] = dtype == 1 ? __half2float(static_cast<const __half*>(b)[i]) : static_cast<const float*>(b)[i];
+// par of ProductArgs from the weight rows' scales and the bias (may be null).
+__global__ void params_kernel(const float* ws, const void* b, int dtype, float2* par, int cout, int n_out, int npad) {
+    const int c = blockIdx.x * blockDim.x + threadIdx.x;
+    if (c >= cout) return;
+    const float v = !b ? 0.f : dtype == 1 ? __half2float(static_cast<const __half*>(b)[c]) : static_cast<const float*>(b)[c];
+    par[c < n_out ? c : npad + c - n_out] = make_float2(ws[c], v);
 }
 
 struct DeviceScope {
@@ -78,12 +81,12 @@ struct dn_linear8 {
     int cout = 0, cin = 0, gate = 0, segs = 1, seg_c = 0, seg_p = 0;
     int64_t ldw = 0;
     int sms = 148;
-    uint8_t* arena = nullptr;  // weight codes, scales, bias, error word
+    uint8_t* arena = nullptr;  // weight codes, channel parameters, error word
     int8_t* w = nullptr;
-    float* ws = nullptr;
-    float* bias = nullptr;  // null: none
+    float2* par = nullptr;
     uint32_t* err = nullptr;
     int n_out() const { return gate ? cout / 2 : cout; }
+    int npad() const { return (n_out() + 255) / 256 * 256; }
 };
 
 namespace {
@@ -101,31 +104,34 @@ int check_shape(int64_t cout, int64_t cin, int gate, int segments) {
 
 // The layer's own copy of the weight, quantised; the current device is the layer's.
 cudaError_t lay_out(dn_linear8* L, const void* weight, int dtype, int64_t ldw, const void* bias, cudaStream_t s, int& rc) {
-    const int64_t codes = L->cout * L->ldw;
-    const size_t total = static_cast<size_t>(round16(codes)) + static_cast<size_t>(L->cout) * 8 + 16;
+    const int64_t codes = round16(L->cout * L->ldw);
+    const size_t pars = static_cast<size_t>(L->npad()) * (L->gate ? 2 : 1) * sizeof(float2);
+    const size_t total = static_cast<size_t>(codes) + pars + 16;
     cudaError_t e = cudaMalloc(&L->arena, total);
     if (e != cudaSuccess) return e;
     L->w = reinterpret_cast<int8_t*>(L->arena);
-    L->ws = reinterpret_cast<float*>(L->arena + round16(codes));
-    float* b = L->ws + L->cout;
-    L->err = reinterpret_cast<uint32_t*>(b + L->cout);
+    L->par = reinterpret_cast<float2*>(L->arena + codes);
+    L->err = reinterpret_cast<uint32_t*>(L->arena + codes + pars);
     if ((e = cudaMemsetAsync(L->arena, 0, total, s)) != cudaSuccess) return e;
-    uint8_t* dense = L->arena;
-    const bool apart = L->segs > 1 && L->seg_p != L->seg_c;  // segments that are padded one by one
-    if (apart && (e = cudaMalloc(&dense, static_cast<size_t>(L->cout) * L->cin)) != cudaSuccess) return e;
-    rc = launch_cache_write(CacheWrite{weight, dtype, ldw, L->cout, L->cin, nullptr, 0, dense, apart ? L->cin : L->ldw,
-                                       L->ws, L->cout, 8, L->cin, nullptr},
+    // Segments that are padded one by one are quantised apart and copied.
+    const bool apart = L->segs > 1 && L->seg_p != L->seg_c;
+    const size_t dense_bytes = apart ? static_cast<size_t>(L->cout) * L->cin : 0;
+    uint8_t* tmp = nullptr;
+    if ((e = cudaMalloc(&tmp, static_cast<size_t>(L->cout) * sizeof(float) + dense_bytes)) != cudaSuccess) return e;
+    float* ws = reinterpret_cast<float*>(tmp);
+    uint8_t* dense = apart ? tmp + static_cast<size_t>(L->cout) * sizeof(float) : L->arena;
+    rc = launch_cache_write(CacheWrite{weight, dtype, ldw, L->cout, L->cin, nullptr, 0, dense, apart ? L->cin : L->ldw, ws,
+                                       L->cout, 8, L->cin, nullptr},
                             s);
     for (int t = 0; apart && rc == DN_OK && e == cudaSuccess && t < L->segs; ++t)
         e = cudaMemcpy2DAsync(L->w + t * L->seg_p, L->ldw, dense + t * L->seg_c, L->cin, L->seg_c, L->cout,
                               cudaMemcpyDeviceToDevice, s);
-    if (bias && rc == DN_OK && e == cudaSuccess) {
-        bias_kernel<<<(L->cout + 255) / 256, 256, 0, s>>>(bias, dtype, b, L->cout);
-        L->bias = b;
+    if (rc == DN_OK && e == cudaSuccess) {
+        params_kernel<<<(L->cout + 255) / 256, 256, 0, s>>>(ws, bias, dtype, L->par, L->cout, L->n_out(), L->npad());
         e = cudaGetLastError();
     }
     const cudaError_t e2 = cudaStreamSynchronize(s);
-    if (apart) cudaFree(dense);
+    cudaFree(tmp);
     return e != cudaSuccess ? e : e2;
 }
 
@@ -159,8 +165,8 @@ ProductArgs product_args(const dn_linear8* L) {
     a.seg_p = L->seg_p;
     a.w = L->w;
     a.ldw = L->ldw;
-    a.ws = L->ws;
-    a.bias = L->bias;
+    a.par = L->par;
+    a.npad = L->npad();
     a.cout = L->cout;
     a.n_out = L->n_out();
     a.gate = L->gate;

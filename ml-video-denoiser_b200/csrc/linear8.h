@@ -18,8 +18,11 @@ struct ProductArgs {
     int segs, seg_c, seg_p;      // segments, their channels, their bytes in a weight row (a multiple of 16)
     const int8_t* w;             // [cout][ldw]
     int64_t ldw;
-    const float* ws;             // [cout]
-    const float* bias;           // [cout], or null
+    // (scale, bias) of the channels: of output c at par[c], of a gated layer's
+    // second factor at par[npad + c]; npad = n_out rounded up to 256, zeros
+    // behind n_out, so that a tile's columns need no check.
+    const float2* par;
+    int npad;
     int cout, n_out, gate;
     int64_t rows;
     void* out;

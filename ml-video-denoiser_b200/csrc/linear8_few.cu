@@ -124,9 +124,11 @@ __global__ void __launch_bounds__(kThreads) product_few_kernel(const __grid_cons
     const int r = lane / CPW, j = lane % CPW;
     const int o = p.gate ? c0 + j / 2 : c0 + j;
     const bool in = r < R && o < p.n_out;
-    const int c = o + (p.gate && (j & 1) ? p.n_out : 0);
     float y = 0.f;
-    if (in) y = fmaf(static_cast<float>(mine) * s_scale[r], p.ws[c], p.bias ? p.bias[c] : 0.f);
+    if (in) {
+        const float2 wb = __ldg(p.par + o + (p.gate && (j & 1) ? p.npad : 0));
+        y = fmaf(static_cast<float>(mine) * s_scale[r], wb.x, wb.y);
+    }
     if (p.gate) y *= __shfl_down_sync(0xffffffffu, y, 1);
     if (in && r < rows && !(p.gate && (j & 1))) {
         if (g.out_f32)

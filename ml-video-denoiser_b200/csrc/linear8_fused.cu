@@ -101,10 +101,7 @@ __global__ void __launch_bounds__(Shape<PLANES, SG, NT>::kThreads) product_fused
         constexpr int kPer = S::kSpan / 16;
         *reinterpret_cast<uint4*>(sb + (j / kPer) * (NT * S::kSpan) + sw_offset(r, j % kPer, S::kSpan)) = v;
     }
-    for (int r = tid; r < NT; r += S::kThreads) {
-        const int c = weight_row(r);
-        s_par[r] = c >= 0 ? make_float2(p.ws[c], p.bias ? p.bias[c] : 0.f) : make_float2(0.f, 0.f);
-    }
+    for (int r = tid; r < NT; r += S::kThreads) s_par[r] = __ldg(p.par + (p.gate && r >= half ? p.npad + r - half : r));
     tc_fence_before();
     __syncthreads();
     tc_fence_after();

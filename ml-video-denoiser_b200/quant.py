@@ -61,8 +61,11 @@ def _elsewhere(device: int, stream) -> bool:
     return stream is not None or torch.cuda.current_device() != device
 
 
-def _stream(device: int) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+try:  # the current stream's handle without a Stream object: a microsecond of a call's eight
+    from torch._C import _cuda_getCurrentRawStream as _stream
+except ImportError:
+    def _stream(device: int) -> int:
+        return torch.cuda.current_stream(device).cuda_stream
 
 
 def _on_device(t, device: int, what: str) -> None:
@@ -250,6 +253,7 @@ class Linear8:
         check(lib().dn_linear8_info(self._h, *[ctypes.byref(v) for v in vals]))
         self.out_channels, self.in_channels = vals[0].value, vals[1].value
         self.gate, self.segments = bool(vals[2].value), vals[3].value
+        self._need = {}  # workspace bytes of the sizes met
 
     def close(self) -> None:
         h = getattr(self, "_h", None)
@@ -267,12 +271,17 @@ class Linear8:
         """(address, bytes, tensor) of a call's workspace, from torch's
         allocator on the current stream, which keeps it from others until the
         stream is past the call."""
-        n = ctypes.c_int64()
-        check(lib().dn_linear8_workspace(self._h, rows, dtype, nchw, ctypes.byref(n)))
-        if n.value == 0:
+        need = self._need.get((rows, dtype, nchw))
+        if need is None:
+            n = ctypes.c_int64()
+            check(lib().dn_linear8_workspace(self._h, rows, dtype, nchw, ctypes.byref(n)))
+            if len(self._need) > 256:
+                self._need.clear()
+            need = self._need[rows, dtype, nchw] = n.value
+        if need == 0:
             return None, 0, None
-        t = torch.empty(n.value, dtype=torch.uint8, device=torch.device("cuda", self.device))
-        return t.data_ptr(), n.value, t
+        t = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", self.device))
+        return t.data_ptr(), need, t
 
     def forward(self, x, out=None, out_dtype=None, stream=None):
         """Token rows x (rows, in_channels), FP16 or FP32, any row stride ->
@@ -284,7 +293,7 @@ class Linear8:
         ldx = _matrix(x, None, self.in_channels, self.device, "Linear8.forward: x")
         rows = x.shape[0]
         if out is None:
-            out = torch.empty(rows, self.out_channels, dtype=out_dtype or x.dtype, device=x.device)
+            out = x.new_empty((rows, self.out_channels), dtype=out_dtype)
         code = _code(out.dtype, "Linear8.forward: out")
         ldo = _matrix(out, rows, self.out_channels, self.device, "Linear8.forward: out")
         ws, n, _keep = self._workspace(rows, dtype)
