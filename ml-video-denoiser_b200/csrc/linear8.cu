@@ -339,7 +339,9 @@ int dn_linear8_forward_nchw(dn_linear8* L, const void* input, int N, int H, int 
     DN_TRY(check_workspace(workspace_bytes_of(a, 1), workspace, workspace_bytes, name));
     DeviceScope scope(L->device);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (path_of(a, 1) == Path::kFused) return launch_product_fused(a, input, 0, 1, L->sms, s);
+    if (path_of(a, 1) == Path::kFused)
+        return product_planes_takes(a, input) ? launch_product_planes(a, input, L->sms, s)
+                                              : launch_product_fused(a, input, 0, 1, L->sms, s);
     a.lda = round16(L->cin);
     auto* codes = static_cast<uint8_t*>(workspace);
     auto* scales = reinterpret_cast<float*>(codes + rows * a.lda);

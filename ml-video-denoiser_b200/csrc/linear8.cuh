@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "sm100.cuh"
@@ -17,6 +18,30 @@ namespace dnb {
 // 128 bytes). Base and row stride are multiples of 16 bytes.
 int linear8_map(CUtensorMap* m, CUtensorMapDataType type, int esz, const void* base, int64_t cols, int64_t rows,
                 int64_t ld, int box_cols, int box_rows);
+
+PFN_cuTensorMapEncodeTiled_v12000 linear8_encoder();
+
+// CTAs per SM of a kernel that allocates tmem_cols TMEM columns: by registers
+// (allocated in eights a thread), shared memory (228 KB, 1 KB a CTA reserved)
+// and TMEM (512 columns). The occupancy query answers 1 for kernels that use
+// TMEM. `cache` (per device) keeps the answer; sets the kernel's shared-memory
+// limit on the first call.
+template <typename Kernel>
+cudaError_t tmem_kernel_ctas(Kernel kernel, int threads, int smem, int tmem_cols, int (&cache)[64], int* per_sm) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    *per_sm = e == cudaSuccess && device < 64 ? cache[device] : 0;
+    if (e != cudaSuccess || *per_sm > 0) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaFuncAttributes at{};
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&at, kernel);
+    if (e != cudaSuccess) return e;
+    const int by_regs = 65536 / (std::max(1, (at.numRegs + 7) / 8 * 8) * threads);
+    const int by_smem = 233472 / (smem + static_cast<int>(at.sharedSizeBytes) + 1024);
+    *per_sm = std::max(1, std::min({by_regs, by_smem, 512 / tmem_cols}));
+    if (device < 64) cache[device] = *per_sm;
+    return e;
+}
 
 __host__ __device__ constexpr uint32_t idesc_s8(int M, int N) {
     return (2u << 4)                                 // D: s32

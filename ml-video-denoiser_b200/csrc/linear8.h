@@ -40,6 +40,14 @@ int launch_product_tc(const ProductArgs& a, int out_dtype, int sms, cudaStream_t
 bool product_fused_takes(const ProductArgs& a);
 int launch_product_fused(const ProductArgs& a, const void* x, int64_t ldx, int out_dtype, int sms, cudaStream_t s);
 
+// Tile columns that hold all channels of a layer (gated ones need whole
+// 32-column runs of each factor); the one-pass kernels take up to 256.
+inline int fused_width(const ProductArgs& a) { return a.gate ? 2 * ((a.n_out + 31) / 32 * 32) : a.cout; }
+
+// One pass over planes that TMA can address.
+bool product_planes_takes(const ProductArgs& a, const void* x);
+int launch_product_planes(const ProductArgs& a, const void* x, int sms, cudaStream_t s);
+
 // One pass over a few token rows.
 bool product_few_takes(const ProductArgs& a);
 int launch_product_few(const ProductArgs& a, const void* x, int dtype, int64_t ldx, int out_dtype, int sms,

@@ -280,22 +280,10 @@ int run(FusedArgs& g, int sms, cudaStream_t s) {
     if (g.tma_out)
         DN_TRY(linear8_map(&map, sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
                            sizeof(T), p.out, p.n_out, p.rows, p.ldo, g.unit, 32));
-    static int resident[64] = {};  // CTAs per SM, per device
-    int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    int per_sm = device < 64 ? resident[device] : 0;
+    static int resident[64] = {};
+    int per_sm = 0;
     auto kernel = product_fused_kernel<T, PLANES, SG, NT>;
-    if (e == cudaSuccess && per_sm == 0) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-        cudaFuncAttributes at{};
-        if (e == cudaSuccess) e = cudaFuncGetAttributes(&at, kernel);
-        // By registers (allocated in eights a thread), shared memory (228 KB, 1 KB a CTA reserved) and TMEM (512
-        // columns); the occupancy query answers 1 for kernels that use TMEM.
-        const int by_regs = 65536 / (std::max(1, (at.numRegs + 7) / 8 * 8) * S::kThreads);
-        const int by_smem = 233472 / (S::kSmem + static_cast<int>(at.sharedSizeBytes) + 1024);
-        per_sm = std::max(1, std::min({by_regs, by_smem, 512 / NT}));
-        if (e == cudaSuccess && device < 64) resident[device] = per_sm;
-    }
+    cudaError_t e = tmem_kernel_ctas(kernel, S::kThreads, S::kSmem, NT, resident, &per_sm);
     if (e == cudaSuccess)
         e = launch_pdl(kernel, dim3(static_cast<unsigned>(std::min(g.m_tiles, per_sm * sms))), dim3(S::kThreads), S::kSmem,
                        s, g, map);
@@ -304,8 +292,7 @@ int run(FusedArgs& g, int sms, cudaStream_t s) {
 
 template <typename T, bool PLANES, int SG>
 int run_nt(FusedArgs& g, int sms, cudaStream_t s) {
-    // A tile holds the whole layer; gated ones need whole 32-column runs of each factor.
-    const int need = g.p.gate ? 2 * ((g.p.n_out + 31) / 32 * 32) : g.p.cout;
+    const int need = fused_width(g.p);
     if (need <= 32) return run<T, PLANES, SG, 32>(g, sms, s);
     if (need <= 64) return run<T, PLANES, SG, 64>(g, sms, s);
     if (need <= 128) return run<T, PLANES, SG, 128>(g, sms, s);
@@ -326,8 +313,7 @@ int run_k(FusedArgs& g, int sms, cudaStream_t s) {
 }  // namespace
 
 bool product_fused_takes(const ProductArgs& a) {
-    const int need = a.gate ? 2 * ((a.n_out + 31) / 32 * 32) : a.cout;
-    return need <= 256 && a.segs == 1 && a.seg_c <= (a.planes ? 128 : 256);
+    return fused_width(a) <= 256 && a.segs == 1 && a.seg_c <= (a.planes ? 128 : 256);
 }
 
 int launch_product_fused(const ProductArgs& a, const void* x, int64_t ldx, int out_dtype, int sms, cudaStream_t s) {

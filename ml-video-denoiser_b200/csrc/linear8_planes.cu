@@ -1,0 +1,312 @@
+// The 8-bit product over NCHW planes of narrow layers (Cin <= 128, Cout <= 256)
+// whose planes TMA can address (H * W a multiple of 8, 16-byte aligned): one
+// pass, bound by HBM (2 Cin + 2 Cout bytes a pixel).
+//
+// Planes are channel-major and the operand of the MMA is pixel-major. The
+// transposes cost one instruction per 8 x 32 values each way:
+//   in    TMA brings [KP channels][64 pixels] boxes (128-byte swizzle);
+//         ldmatrix.trans hands lane t of a warp, for pixel t / 4, the channels
+//         8 m + 2 (t % 4) + {0, 1} of four 8-channel groups m. A lane quantises
+//         these 8 values (the pixel's maximum is two shuffles) and writes them
+//         as 8 adjacent bytes: the K order of the operand is a permutation of
+//         the channels within each 32, and the weight is laid out in the same
+//         one, so the sums are those of the definition;
+//   out   tcgen05.ld 16x256b returns the accumulator in the layout whose
+//         packed pairs stmatrix.trans stores channel-major; TMA stores boxes
+//         of 32 channels x 32 pixels.
+// A CTA of four warps takes tiles of 128 pixels of one image, keeps the weight
+// in shared memory and two tiles' loads in flight; several CTAs per SM overlap
+// each other's phases.
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <string>
+
+#include "denoiser_b200.h"
+#include "launch.cuh"
+#include "linear8.cuh"
+#include "linear8.h"
+#include "quant.cuh"
+#include "status.h"
+
+namespace dnb {
+namespace {
+
+constexpr int kRows = 128;
+constexpr int kThreads = 128;
+
+struct PlanesArgs {
+    ProductArgs p;
+    int tiles_per_image, tiles;
+};
+
+template <int KP, int NT>
+struct Shape {
+    static constexpr int kBox = KP * 128;            // 64 pixels of KP channels
+    static constexpr int kIn = 2 * kBox;             // a tile
+    static constexpr int kA = kRows * KP, kB = NT * KP;
+    static constexpr int kStgWarp = 2 * 32 * 64;     // two boxes of 32 channels x 32 pixels
+    static constexpr int kSmem = 1024 + 2 * kIn + kA + kB + 4 * kStgWarp;
+};
+
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void stmatrix4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
+                 "r"(d)
+                 : "memory");
+}
+// 16 lanes x 32 columns: r[4 k + i] is (lane t / 4 + 8 (i / 2), column 8 k + 2 (t % 4) + i % 2).
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, int (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+
+template <int KP, int NT>
+__global__ void __launch_bounds__(kThreads) product_planes_kernel(const __grid_constant__ PlanesArgs g,
+                                                                  const __grid_constant__ CUtensorMap in_map,
+                                                                  const __grid_constant__ CUtensorMap out_map) {
+    using S = Shape<KP, NT>;
+    using Q = QuantOf<__half>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    __shared__ uint64_t bar, bar_in[2];
+    __shared__ uint32_t tslot;
+    __shared__ volatile int s_abort;
+    __shared__ float s_x[2][kRows];
+    __shared__ __align__(16) float2 s_par[NT];
+    const ProductArgs& p = g.p;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint8_t* s_in = smem;
+    uint8_t* sa = smem + 2 * S::kIn;
+    uint8_t* sb = sa + S::kA;
+    uint8_t* stg = sb + S::kB + warp * S::kStgWarp;
+    constexpr int half = NT / 2;
+    constexpr uint32_t kCols = NT < 32 ? 32 : NT;
+
+    if (warp == 0) {
+        tmem_alloc(&tslot, kCols);
+        tmem_relinquish();
+    }
+    if (tid == 0) {
+        mbar_init(&bar, 1);
+        mbar_init(&bar_in[0], 1);
+        mbar_init(&bar_in[1], 1);
+        s_abort = 0;
+        fence_mbar_init();
+        prefetch_tmap(&in_map);
+        prefetch_tmap(&out_map);
+    }
+    // The weight, its channels in the operand's order: byte position 32 v +
+    // 8 j + 2 m + e holds channel 32 v + 8 m + 2 j + e.
+    for (int i = tid; i < NT * (KP / 16); i += kThreads) {
+        const int r = i / (KP / 16), q = i % (KP / 16);
+        int c;
+        if (!p.gate)
+            c = r < p.cout ? r : -1;
+        else
+            c = r < half ? (r < p.n_out ? r : -1) : (r - half < p.n_out ? p.n_out + r - half : -1);
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int h = 0; h < 8; ++h) {  // pairs of adjacent channels
+            const int pos = q * 16 + 2 * h;
+            const int ch = (pos & ~31) + ((pos & 7) >> 1) * 8 + ((pos >> 3) & 3) * 2;
+            if (c >= 0 && ch < p.ldw)
+                w[h >> 1] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p.w + c * p.ldw + ch)) << ((h & 1) * 16);
+        }
+        *reinterpret_cast<uint4*>(sb + sw_offset(r, q, KP)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    for (int r = tid; r < NT; r += kThreads) s_par[r] = __ldg(p.par + (p.gate && r >= half ? p.npad + r - half : r));
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tslot;
+    pdl_trigger();
+    pdl_wait();
+
+    auto load = [&](int tile, int b) {
+        const int img = tile / g.tiles_per_image, x0 = (tile - img * g.tiles_per_image) * kRows;
+        mbar_arrive_expect_tx(&bar_in[b], S::kIn);
+        tma_load_3d(s_in + b * S::kIn, &in_map, x0, 0, img, &bar_in[b]);
+        tma_load_3d(s_in + b * S::kIn + S::kBox, &in_map, x0 + 64, 0, img, &bar_in[b]);
+    };
+    if (tid == 0) {
+        if (static_cast<int>(blockIdx.x) < g.tiles) load(blockIdx.x, 0);
+        if (static_cast<int>(blockIdx.x + gridDim.x) < g.tiles) load(blockIdx.x + gridDim.x, 1);
+    }
+    const uint64_t ad0 = sdesc_kmajor_sw(smem_u32(sa), KP), bd0 = sdesc_kmajor_sw(smem_u32(sb), KP);
+    const int steps = (p.seg_c + 31) / 32;
+    const int out_cols = p.gate ? half : NT;
+    const int j4 = lane & 3, px = lane >> 2;  // a lane's channel pair and pixel of 8
+    int n = 0;
+    uint32_t stores = 0;
+    for (int tile = blockIdx.x; tile < g.tiles; tile += gridDim.x, ++n) {
+        const int b = n & 1;
+        float* sx = s_x[b];
+        wait_or_abort(&bar_in[b], (n >> 1) & 1, &s_abort, p.err, 0x75);
+        __syncwarp();
+        // This warp's 32 pixels: half of a 64-pixel box, four groups of 8.
+        const uint32_t box = smem_u32(s_in + b * S::kIn + (warp >> 1) * S::kBox);
+#pragma unroll
+        for (int pg = 0; pg < 4; ++pg) {
+            const uint32_t chunk = (warp & 1) * 4 + pg;
+            typename Q::Vec v[KP / 32];
+            uint32_t mag = 0;
+#pragma unroll
+            for (int k = 0; k < KP / 32; ++k) {
+                uint32_t r[4];
+                ldmatrix4_trans(r, box + (k * 32 + lane) * 128 + ((chunk ^ (lane & 7)) << 4));
+                v[k].v = make_uint4(r[0], r[1], r[2], r[3]);
+                mag = max(mag, Q::mag(v[k]));
+            }
+            mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, 1));
+            mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, 2));
+            const GroupScale q = group_scale<__half>(mag, 127.f);
+            const bool fix = __any_sync(0xffffffffu, q.fix != 0.f);
+            const int r = warp * 32 + pg * 8 + px;
+#pragma unroll
+            for (int k = 0; k < KP / 32; ++k)
+                *reinterpret_cast<uint2*>(sa + sw_offset(r, k * 2 + (j4 >> 1), KP) + (j4 & 1) * 8) =
+                    codes8<__half>(v[k], q, fix);
+            if (j4 == 0) sx[r] = q.s;
+        }
+        fence_async_smem();
+        tc_fence_before();
+        __syncthreads();  // the operand is complete; this input buffer and the accumulator are free
+        if (tid == 0) {
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < KP / 32; ++k)
+                if (k < steps) mma_s8(tmem, ad0 + 2 * k, bd0 + 2 * k, idesc_s8(kRows, NT), k > 0 ? 1u : 0u);
+            mma_commit(&bar);
+            const int64_t next = static_cast<int64_t>(tile) + 2 * static_cast<int64_t>(gridDim.x);
+            if (next < g.tiles) load(static_cast<int>(next), b);
+        }
+        wait_or_abort(&bar, n & 1, &s_abort, p.err, 0x76);
+        __syncwarp();
+        tc_fence_after();
+
+        const int img = tile / g.tiles_per_image, x0 = (tile - img * g.tiles_per_image) * kRows + warp * 32;
+        const uint32_t acc = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+        float s[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = sx[warp * 32 + i * 8 + px];
+        // y[k][pg][e]: tile column c + 8 k + 2 j4 + e of pixel 8 pg + px.
+        auto scaled = [&](int c, float (&y)[4][4][2]) {
+            int a[2][16];
+            tmem_ld_16x32(acc + c, a[0]);
+            tmem_ld_16x32(acc + (16u << 16) + c, a[1]);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float4 w = *reinterpret_cast<const float4*>(&s_par[c + 8 * k + 2 * j4]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    y[k][i][0] = fmaf(static_cast<float>(a[i >> 1][4 * k + 2 * (i & 1)]) * s[i], w.x, w.y);
+                    y[k][i][1] = fmaf(static_cast<float>(a[i >> 1][4 * k + 2 * (i & 1) + 1]) * s[i], w.z, w.w);
+                }
+            }
+        };
+        for (int c = 0; c < out_cols && c < p.n_out; c += 32, ++stores) {
+            float y[4][4][2];
+            scaled(c, y);
+            if (p.gate) {
+                float z[4][4][2];
+                scaled(half + c, z);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[k][i][0] *= z[k][i][0], y[k][i][1] *= z[k][i][1];
+            }
+            // The box stored two boxes ago has been read.
+            uint8_t* dst = stg + (stores & 1) * (32 * 64);
+            if (lane == 0) bulk_wait_read1();
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                stmatrix4_trans(smem_u32(dst) + sw_offset(8 * k + (lane & 7), lane >> 3, 64), pack_half2(y[k][0][0], y[k][0][1]),
+                                pack_half2(y[k][1][0], y[k][1][1]), pack_half2(y[k][2][0], y[k][2][1]),
+                                pack_half2(y[k][3][0], y[k][3][1]));
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                if (x0 < p.ldo) tma_store_3d(&out_map, x0, c, img, dst);
+                bulk_commit();
+            }
+        }
+    }
+    if (lane == 0) bulk_wait_read0();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) tmem_dealloc(tmem, kCols);
+}
+
+// Planes [images][channels][pixels] with boxes of box_px x box_ch.
+int planes_map(CUtensorMap* m, const void* base, int64_t pixels, int64_t channels, int64_t images, int box_px, int box_ch) {
+    auto fn = linear8_encoder();
+    if (!fn) return dn_fail(DN_ERR_CUDA, "linear8: cuTensorMapEncodeTiled unavailable");
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(pixels), static_cast<cuuint64_t>(channels),
+                                static_cast<cuuint64_t>(images)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(pixels) * 2, static_cast<cuuint64_t>(pixels * channels) * 2};
+    const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_px), static_cast<cuuint32_t>(box_ch), 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, box_px == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return dn_fail_str(DN_ERR_CUDA, "linear8: cuTensorMapEncodeTiled failed (" + std::to_string(r) + ")");
+    return DN_OK;
+}
+
+template <int KP, int NT>
+int run(PlanesArgs& g, const void* x, int sms, cudaStream_t s) {
+    using S = Shape<KP, NT>;
+    const ProductArgs& p = g.p;
+    const int64_t images = p.rows / p.ldo;
+    CUtensorMap in{}, out{};
+    DN_TRY(planes_map(&in, x, p.ldo, p.seg_c, images, 64, KP));
+    DN_TRY(planes_map(&out, p.out, p.ldo, p.n_out, images, 32, 32));
+    static int resident[64] = {};
+    int per_sm = 0;
+    cudaError_t e = tmem_kernel_ctas(product_planes_kernel<KP, NT>, kThreads, S::kSmem, NT, resident, &per_sm);
+    if (e == cudaSuccess)
+        e = launch_pdl(product_planes_kernel<KP, NT>, dim3(static_cast<unsigned>(std::min(g.tiles, per_sm * sms))),
+                       dim3(kThreads), S::kSmem, s, g, in, out);
+    return e == cudaSuccess ? DN_OK : dn_cuda_fail(e, "linear8: planes launch");
+}
+
+template <int KP>
+int run_nt(PlanesArgs& g, const void* x, int sms, cudaStream_t s) {
+    const int need = fused_width(g.p);
+    if (need <= 32) return run<KP, 32>(g, x, sms, s);
+    if (need <= 64) return run<KP, 64>(g, x, sms, s);
+    if (need <= 128) return run<KP, 128>(g, x, sms, s);
+    return run<KP, 256>(g, x, sms, s);
+}
+
+}  // namespace
+
+bool product_planes_takes(const ProductArgs& a, const void* x) {
+    return a.planes && fused_width(a) <= 256 && a.segs == 1 && a.seg_c <= 128 && a.ldo % 8 == 0 &&
+           reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
+}
+
+int launch_product_planes(const ProductArgs& a, const void* x, int sms, cudaStream_t s) {
+    PlanesArgs g{};
+    g.p = a;
+    g.tiles_per_image = static_cast<int>((a.ldo + kRows - 1) / kRows);
+    g.tiles = static_cast<int>(g.tiles_per_image * (a.rows / a.ldo));
+    if (a.seg_c <= 32) return run_nt<32>(g, x, sms, s);
+    if (a.seg_c <= 64) return run_nt<64>(g, x, sms, s);
+    return run_nt<128>(g, x, sms, s);
+}
+
+}  // namespace dnb

@@ -390,6 +390,8 @@ int run_type(TcArgs& g, int sms, cudaStream_t s) {
 
 }  // namespace
 
+PFN_cuTensorMapEncodeTiled_v12000 linear8_encoder() { return tensor_map_encoder(); }
+
 int linear8_map(CUtensorMap* m, CUtensorMapDataType type, int esz, const void* base, int64_t cols, int64_t rows,
                 int64_t ld, int box_cols, int box_rows) {
     auto fn = tensor_map_encoder();
