@@ -36,14 +36,14 @@ __global__ void __launch_bounds__(256) quantise_planes_kernel(const __half* __re
     uint32_t mag = 0;
     for (int k = 0; k < K; ++k) mag = max(mag, static_cast<uint32_t>(__half_as_ushort(src[k * hw])) & 0x7fffu);
     const GroupScale g = group_scale<__half>(mag, 127.f);
-    const bool fix = __any_sync(0xffffffffu, g.fix != 0.f);
+    const bool rare = __any_sync(0xffffffffu, g.rare);
     if (!live) return;
     for (int k = 0; k < K; k += 8) {
         uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (k + i < K) w[i >> 1] |= static_cast<uint32_t>(__half_as_ushort(src[(k + i) * hw])) << ((i & 1) * 16);
-        *reinterpret_cast<uint2*>(codes + m * ldc + k) = codes8<__half>(Q::Vec{make_uint4(w[0], w[1], w[2], w[3])}, g, fix);
+        *reinterpret_cast<uint2*>(codes + m * ldc + k) = codes8<__half>(Q::Vec{make_uint4(w[0], w[1], w[2], w[3])}, g, rare);
     }
     scales[m] = g.s;
 }

@@ -25,14 +25,15 @@ PFN_cuTensorMapEncodeTiled_v12000 linear8_encoder();
 // (allocated in eights a thread), shared memory (228 KB, 1 KB a CTA reserved)
 // and TMEM (512 columns). The occupancy query answers 1 for kernels that use
 // TMEM. `cache` (per device) keeps the answer; sets the kernel's shared-memory
-// limit on the first call.
+// limit, smem_limit, on the first call.
 template <typename Kernel>
-cudaError_t tmem_kernel_ctas(Kernel kernel, int threads, int smem, int tmem_cols, int (&cache)[64], int* per_sm) {
+cudaError_t tmem_kernel_ctas(Kernel kernel, int threads, int smem, int smem_limit, int tmem_cols, int (&cache)[64],
+                             int* per_sm) {
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
     *per_sm = e == cudaSuccess && device < 64 ? cache[device] : 0;
     if (e != cudaSuccess || *per_sm > 0) return e;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_limit);
     cudaFuncAttributes at{};
     if (e == cudaSuccess) e = cudaFuncGetAttributes(&at, kernel);
     if (e != cudaSuccess) return e;

@@ -81,10 +81,10 @@ __global__ void __launch_bounds__(kThreads) product_few_kernel(const __grid_cons
     for (int r = 0; r < R; ++r) {
         const GroupScale q = group_scale<T>(r < rows ? s_mag[r] : 0u, 127.f);
         if (tid == 0) s_scale[r] = q.s;
-        const bool fix = !Q::kF32 && q.fix != 0.f;  // the same on every thread
+        const bool rare = q.rare;  // the same on every thread
         for (int k = tid; k < vecs * 2; k += kThreads)
             *reinterpret_cast<uint2*>(s_codes + r * p.ldw + k * 8) =
-                codes8<T>(r < rows && k < groups ? load(r, k) : Q::zero(), q, fix);
+                codes8<T>(r < rows && k < groups ? load(r, k) : Q::zero(), q, rare);
     }
     __syncthreads();
 

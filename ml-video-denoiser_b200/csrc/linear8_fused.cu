@@ -46,7 +46,12 @@ struct FusedArgs {
 // channels.
 template <bool PLANES, int SG, int NT>
 struct Shape {
-    static constexpr int kWarps = SG == 32 ? 8 : 4;
+    // Planes: a lane per pixel. Token rows: as many warps as keep 8 vectors a
+    // lane in registers (130560 x 256 -> 256: 36 us with 16 warps, 57 with 8;
+    // 522240 x 64 -> 128: 42 us with 4, 45 with 8), and 8 where TMEM leaves
+    // room for two CTAs only (130560 x 128 -> 256: 29 us, 49 with 4).
+    static constexpr int kWarps = PLANES ? 4 : SG == 32 ? 16 : SG == 16 || NT == 256 ? 8 : 4;
+    static constexpr int kGroups = kWarps / 4;                              // warps that share a TMEM quadrant
     static constexpr int kThreads = kWarps * 32;
     static constexpr int kVecs = PLANES ? SG : (kRows / kWarps) * SG / 32;  // 8-value vectors of a lane
     static constexpr int kBytesK = SG <= 4 ? 32 : SG * 8;                   // bytes of an operand row
@@ -161,25 +166,40 @@ __global__ void __launch_bounds__(Shape<PLANES, SG, NT>::kThreads) product_fused
 #pragma unroll
             for (int i = 1; i < S::kVecs; ++i) mag = max(mag, Q::mag(v[i]));
             const GroupScale q = group_scale<__half>(mag, 127.f);
-            const bool fix = __any_sync(0xffffffffu, q.fix != 0.f);
+            const bool rare = __any_sync(0xffffffffu, q.rare);
             const int r = warp * 32 + lane;
 #pragma unroll
             for (int i = 0; i < S::kVecs; i += 2) {
-                const uint2 lo = codes8<__half>(v[i], q, fix), hi = codes8<__half>(v[i + 1], q, fix);
+                const uint2 lo = codes8<__half>(v[i], q, rare), hi = codes8<__half>(v[i + 1], q, rare);
                 *reinterpret_cast<uint4*>(a_chunk(r, i / 2)) = make_uint4(lo.x, lo.y, hi.x, hi.y);
             }
             sx[r] = q.s;
         } else {
-#pragma unroll
-            for (int i = 0; i < S::kVecs; ++i) {
+            auto scale_of = [&](int i) {
                 uint32_t mag = Q::mag(v[i]);
 #pragma unroll
                 for (int d = SG / 2; d > 0; d >>= 1) mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, d));
-                const GroupScale q = group_scale<__half>(mag, 127.f);
-                const bool fix = __any_sync(0xffffffffu, q.fix != 0.f);
-                const int r = warp * kWarpRows + i * kPer + sub;
-                *reinterpret_cast<uint2*>(a_chunk(r, l / 2) + (l & 1) * 8) = codes8<__half>(v[i], q, fix);
-                if (l == 0) sx[r] = q.s;
+                return group_scale<__half>(mag, 127.f);
+            };
+            auto code_at = [&](int i) {
+                return reinterpret_cast<uint2*>(a_chunk(warp * kWarpRows + i * kPer + sub, l / 2) + (l & 1) * 8);
+            };
+            // One vote for the warp's rows (a fifth of 32 rows has a rare one).
+            float r[S::kVecs];
+            bool rare = false;
+#pragma unroll
+            for (int i = 0; i < S::kVecs; ++i) {
+                const GroupScale q = scale_of(i);
+                r[i] = q.r;
+                rare = rare || q.rare;
+                if (l == 0) sx[warp * kWarpRows + i * kPer + sub] = q.s;
+            }
+            if (!__any_sync(0xffffffffu, rare)) {
+#pragma unroll
+                for (int i = 0; i < S::kVecs; ++i) *code_at(i) = codes8_fast(v[i], r[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < S::kVecs; ++i) *code_at(i) = codes8_rare<__half>(v[i], scale_of(i));
             }
         }
         fence_async_smem();
@@ -218,13 +238,16 @@ __global__ void __launch_bounds__(Shape<PLANES, SG, NT>::kThreads) product_fused
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
                 const float4 w = *reinterpret_cast<const float4*>(&s_par[c + i]);  // two rows' (scale, bias)
-                y[i] = fmaf(static_cast<float>(a[i]) * s, w.x, w.y);
-                y[i + 1] = fmaf(static_cast<float>(a[i + 1]) * s, w.z, w.w);
+                const float2 t = ffma2(make_float2(static_cast<float>(a[i]), static_cast<float>(a[i + 1])), make_float2(s, s),
+                                       make_float2(0.f, 0.f));
+                const float2 z = ffma2(t, make_float2(w.x, w.z), make_float2(w.y, w.w));
+                y[i] = z.x;
+                y[i + 1] = z.y;
             }
         };
         const int unit = !PLANES && g.tma_out ? g.unit : 32;
         for (int c0 = 0, u = 0; c0 < out_cols && c0 < p.n_out; c0 += unit, ++u) {
-            if (S::kWarps == 8 && (u & 1) != group) continue;
+            if (u % S::kGroups != group) continue;
             if (!PLANES && g.tma_out) {
                 if (lane == 0) bulk_wait_read0();
                 __syncwarp();
@@ -275,7 +298,9 @@ int run(FusedArgs& g, int sms, cudaStream_t s) {
     const bool al16 = !PLANES && reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo * sizeof(T) % 16 == 0 &&
                       p.ldo >= p.n_out;
     g.tma_out = g.vec_out = al16;
-    g.unit = std::min<int>(128 / sizeof(T), out_cols);
+    // Staging rows of 128 bytes, or shorter ones so that every group of four
+    // warps has columns to finish.
+    g.unit = std::max(32, std::min<int>(128 / sizeof(T), out_cols / S::kGroups));
     CUtensorMap map{};
     if (g.tma_out)
         DN_TRY(linear8_map(&map, sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
@@ -283,7 +308,7 @@ int run(FusedArgs& g, int sms, cudaStream_t s) {
     static int resident[64] = {};
     int per_sm = 0;
     auto kernel = product_fused_kernel<T, PLANES, SG, NT>;
-    cudaError_t e = tmem_kernel_ctas(kernel, S::kThreads, S::kSmem, NT, resident, &per_sm);
+    cudaError_t e = tmem_kernel_ctas(kernel, S::kThreads, S::kSmem, S::kSmem, NT, resident, &per_sm);
     if (e == cudaSuccess)
         e = launch_pdl(kernel, dim3(static_cast<unsigned>(std::min(g.m_tiles, per_sm * sms))), dim3(S::kThreads), S::kSmem,
                        s, g, map);

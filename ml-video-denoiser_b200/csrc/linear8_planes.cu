@@ -13,7 +13,7 @@
 //         one, so the sums are those of the definition;
 //   out   tcgen05.ld 16x256b returns the accumulator in the layout whose
 //         packed pairs stmatrix.trans stores channel-major; TMA stores boxes
-//         of 32 channels x 32 pixels.
+//         of all channels x 64 pixels, each filled by two warps.
 // A CTA of four warps takes tiles of 128 pixels of one image, keeps the weight
 // in shared memory and two tiles' loads in flight; several CTAs per SM overlap
 // each other's phases.
@@ -46,8 +46,8 @@ struct Shape {
     static constexpr int kBox = KP * 128;            // 64 pixels of KP channels
     static constexpr int kIn = 2 * kBox;             // a tile
     static constexpr int kA = kRows * KP, kB = NT * KP;
-    static constexpr int kStgWarp = 2 * 32 * 64;     // two boxes of 32 channels x 32 pixels
-    static constexpr int kSmem = 1024 + 2 * kIn + kA + kB + 4 * kStgWarp;
+    // The output tile, two boxes of 64 pixels: a gated layer uses half of it.
+    static int smem(bool gate) { return 1024 + 2 * kIn + kA + kB + (gate ? NT / 2 : NT) * 256; }
 };
 
 __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
@@ -88,8 +88,9 @@ __global__ void __launch_bounds__(kThreads) product_planes_kernel(const __grid_c
     uint8_t* s_in = smem;
     uint8_t* sa = smem + 2 * S::kIn;
     uint8_t* sb = sa + S::kA;
-    uint8_t* stg = sb + S::kB + warp * S::kStgWarp;
     constexpr int half = NT / 2;
+    const int out_cols = p.gate ? half : NT;
+    uint8_t* stg = sb + S::kB + (warp >> 1) * (out_cols * 128);  // this warp's 64-pixel box of the output tile
     constexpr uint32_t kCols = NT < 32 ? 32 : NT;
 
     if (warp == 0) {
@@ -144,10 +145,12 @@ __global__ void __launch_bounds__(kThreads) product_planes_kernel(const __grid_c
     }
     const uint64_t ad0 = sdesc_kmajor_sw(smem_u32(sa), KP), bd0 = sdesc_kmajor_sw(smem_u32(sb), KP);
     const int steps = (p.seg_c + 31) / 32;
-    const int out_cols = p.gate ? half : NT;
     const int j4 = lane & 3, px = lane >> 2;  // a lane's channel pair and pixel of 8
     int n = 0;
-    uint32_t stores = 0;
+    // The tile's image and place in it, stepped along with the tile.
+    const int step_img = gridDim.x / g.tiles_per_image, step_x = gridDim.x - step_img * g.tiles_per_image;
+    int img = blockIdx.x / g.tiles_per_image, xt = blockIdx.x - img * g.tiles_per_image;
+    const bool issues = tid == 32;  // this thread stores the output tiles
     for (int tile = blockIdx.x; tile < g.tiles; tile += gridDim.x, ++n) {
         const int b = n & 1;
         float* sx = s_x[b];
@@ -155,32 +158,45 @@ __global__ void __launch_bounds__(kThreads) product_planes_kernel(const __grid_c
         __syncwarp();
         // This warp's 32 pixels: half of a 64-pixel box, four groups of 8.
         const uint32_t box = smem_u32(s_in + b * S::kIn + (warp >> 1) * S::kBox);
+        typename Q::Vec v[4][KP / 32];
+        GroupScale q[4];
+        bool rare = false;
 #pragma unroll
         for (int pg = 0; pg < 4; ++pg) {
             const uint32_t chunk = (warp & 1) * 4 + pg;
-            typename Q::Vec v[KP / 32];
             uint32_t mag = 0;
 #pragma unroll
             for (int k = 0; k < KP / 32; ++k) {
                 uint32_t r[4];
                 ldmatrix4_trans(r, box + (k * 32 + lane) * 128 + ((chunk ^ (lane & 7)) << 4));
-                v[k].v = make_uint4(r[0], r[1], r[2], r[3]);
-                mag = max(mag, Q::mag(v[k]));
+                v[pg][k].v = make_uint4(r[0], r[1], r[2], r[3]);
+                mag = max(mag, Q::mag(v[pg][k]));
             }
             mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, 1));
             mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, 2));
-            const GroupScale q = group_scale<__half>(mag, 127.f);
-            const bool fix = __any_sync(0xffffffffu, q.fix != 0.f);
-            const int r = warp * 32 + pg * 8 + px;
+            q[pg] = group_scale<__half>(mag, 127.f);
+            rare = rare || q[pg].rare;
+            if (j4 == 0) sx[warp * 32 + pg * 8 + px] = q[pg].s;
+        }
+        auto code_at = [&](int pg, int k) {
+            return reinterpret_cast<uint2*>(sa + sw_offset(warp * 32 + pg * 8 + px, k * 2 + (j4 >> 1), KP) + (j4 & 1) * 8);
+        };
+        // One vote for the warp's 32 pixels (a fifth of the warps has a rare one).
+        if (!__any_sync(0xffffffffu, rare)) {
 #pragma unroll
-            for (int k = 0; k < KP / 32; ++k)
-                *reinterpret_cast<uint2*>(sa + sw_offset(r, k * 2 + (j4 >> 1), KP) + (j4 & 1) * 8) =
-                    codes8<__half>(v[k], q, fix);
-            if (j4 == 0) sx[r] = q.s;
+            for (int pg = 0; pg < 4; ++pg)
+#pragma unroll
+                for (int k = 0; k < KP / 32; ++k) *code_at(pg, k) = codes8_fast(v[pg][k], q[pg].r);
+        } else {
+#pragma unroll
+            for (int pg = 0; pg < 4; ++pg)
+#pragma unroll
+                for (int k = 0; k < KP / 32; ++k) *code_at(pg, k) = codes8_rare<__half>(v[pg][k], q[pg]);
         }
         fence_async_smem();
         tc_fence_before();
-        __syncthreads();  // the operand is complete; this input buffer and the accumulator are free
+        if (issues) bulk_wait_read0();
+        __syncthreads();  // the operand is complete; this input buffer, the accumulator and the output tile are free
         if (tid == 0) {
             tc_fence_after();
 #pragma unroll
@@ -194,13 +210,12 @@ __global__ void __launch_bounds__(kThreads) product_planes_kernel(const __grid_c
         __syncwarp();
         tc_fence_after();
 
-        const int img = tile / g.tiles_per_image, x0 = (tile - img * g.tiles_per_image) * kRows + warp * 32;
         const uint32_t acc = tmem + (static_cast<uint32_t>(warp * 32) << 16);
         float s[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[i] = sx[warp * 32 + i * 8 + px];
-        // y[k][pg][e]: tile column c + 8 k + 2 j4 + e of pixel 8 pg + px.
-        auto scaled = [&](int c, float (&y)[4][4][2]) {
+        // y[k][pg]: tile columns c + 8 k + 2 j4 and the next of pixel 8 pg + px.
+        auto scaled = [&](int c, float2 (&y)[4][4]) {
             int a[2][16];
             tmem_ld_16x32(acc + c, a[0]);
             tmem_ld_16x32(acc + (16u << 16) + c, a[1]);
@@ -210,56 +225,66 @@ __global__ void __launch_bounds__(kThreads) product_planes_kernel(const __grid_c
                 const float4 w = *reinterpret_cast<const float4*>(&s_par[c + 8 * k + 2 * j4]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    y[k][i][0] = fmaf(static_cast<float>(a[i >> 1][4 * k + 2 * (i & 1)]) * s[i], w.x, w.y);
-                    y[k][i][1] = fmaf(static_cast<float>(a[i >> 1][4 * k + 2 * (i & 1) + 1]) * s[i], w.z, w.w);
+                    const int* v = &a[i >> 1][4 * k + 2 * (i & 1)];
+                    const float2 t = ffma2(make_float2(static_cast<float>(v[0]), static_cast<float>(v[1])),
+                                           make_float2(s[i], s[i]), make_float2(0.f, 0.f));
+                    y[k][i] = ffma2(t, make_float2(w.x, w.z), make_float2(w.y, w.w));
                 }
             }
         };
-        for (int c = 0; c < out_cols && c < p.n_out; c += 32, ++stores) {
-            float y[4][4][2];
+        for (int c = 0; c < out_cols && c < p.n_out; c += 32) {
+            float2 y[4][4];
             scaled(c, y);
             if (p.gate) {
-                float z[4][4][2];
+                float2 z[4][4];
                 scaled(half + c, z);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) y[k][i][0] *= z[k][i][0], y[k][i][1] *= z[k][i][1];
+                    for (int i = 0; i < 4; ++i) y[k][i].x *= z[k][i].x, y[k][i].y *= z[k][i].y;
             }
-            // The box stored two boxes ago has been read.
-            uint8_t* dst = stg + (stores & 1) * (32 * 64);
-            if (lane == 0) bulk_wait_read1();
-            __syncwarp();
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                stmatrix4_trans(smem_u32(dst) + sw_offset(8 * k + (lane & 7), lane >> 3, 64), pack_half2(y[k][0][0], y[k][0][1]),
-                                pack_half2(y[k][1][0], y[k][1][1]), pack_half2(y[k][2][0], y[k][2][1]),
-                                pack_half2(y[k][3][0], y[k][3][1]));
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                if (x0 < p.ldo) tma_store_3d(&out_map, x0, c, img, dst);
-                bulk_commit();
-            }
+                stmatrix4_trans(smem_u32(stg) + sw_offset(c + 8 * k + (lane & 7), (warp & 1) * 4 + (lane >> 3), 128),
+                                pack_half2(y[k][0].x, y[k][0].y), pack_half2(y[k][1].x, y[k][1].y),
+                                pack_half2(y[k][2].x, y[k][2].y), pack_half2(y[k][3].x, y[k][3].y));
+        }
+        fence_async_smem();
+        __syncthreads();
+        if (issues) {
+            const int x0 = xt * kRows;
+            tma_store_3d(&out_map, x0, 0, img, stg);
+            if (x0 + 64 < p.ldo) tma_store_3d(&out_map, x0 + 64, 0, img, stg + out_cols * 128);
+            bulk_commit();
+        }
+        img += step_img;
+        xt += step_x;
+        if (xt >= g.tiles_per_image) {
+            xt -= g.tiles_per_image;
+            ++img;
         }
     }
-    if (lane == 0) bulk_wait_read0();
+    if (issues) bulk_wait_read0();
     tc_fence_before();
     __syncthreads();
     if (warp == 0) tmem_dealloc(tmem, kCols);
 }
 
-// Planes [images][channels][pixels] with boxes of box_px x box_ch.
-int planes_map(CUtensorMap* m, const void* base, int64_t pixels, int64_t channels, int64_t images, int box_px, int box_ch) {
+// Planes [images][channels][pixels] with boxes of 64 pixels x box_ch. (Output
+// boxes of 32 pixels, one per warp, cost 157 us instead of 93 at 32 -> 64
+// channels, 1088x1920: half lines, and twice the address translations where
+// the planes are megabytes apart. 16 images of 272x480, the same bytes in
+// nearer planes, take 78 us.)
+int planes_map(CUtensorMap* m, const void* base, int64_t pixels, int64_t channels, int64_t images, int box_ch) {
     auto fn = linear8_encoder();
     if (!fn) return dn_fail(DN_ERR_CUDA, "linear8: cuTensorMapEncodeTiled unavailable");
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(pixels), static_cast<cuuint64_t>(channels),
                                 static_cast<cuuint64_t>(images)};
     const cuuint64_t strides[2] = {static_cast<cuuint64_t>(pixels) * 2, static_cast<cuuint64_t>(pixels * channels) * 2};
-    const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_px), static_cast<cuuint32_t>(box_ch), 1};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_ch), 1};
     const cuuint32_t estr[3] = {1, 1, 1};
     const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, box_px == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
         return dn_fail_str(DN_ERR_CUDA, "linear8: cuTensorMapEncodeTiled failed (" + std::to_string(r) + ")");
@@ -272,14 +297,16 @@ int run(PlanesArgs& g, const void* x, int sms, cudaStream_t s) {
     const ProductArgs& p = g.p;
     const int64_t images = p.rows / p.ldo;
     CUtensorMap in{}, out{};
-    DN_TRY(planes_map(&in, x, p.ldo, p.seg_c, images, 64, KP));
-    DN_TRY(planes_map(&out, p.out, p.ldo, p.n_out, images, 32, 32));
-    static int resident[64] = {};
+    DN_TRY(planes_map(&in, x, p.ldo, p.seg_c, images, KP));
+    DN_TRY(planes_map(&out, p.out, p.ldo, p.n_out, images, p.gate ? NT / 2 : NT));
+    static int resident[2][64] = {};
+    const int smem = S::smem(p.gate);
     int per_sm = 0;
-    cudaError_t e = tmem_kernel_ctas(product_planes_kernel<KP, NT>, kThreads, S::kSmem, NT, resident, &per_sm);
+    cudaError_t e = tmem_kernel_ctas(product_planes_kernel<KP, NT>, kThreads, smem, S::smem(false), NT,
+                                     resident[p.gate ? 1 : 0], &per_sm);
     if (e == cudaSuccess)
         e = launch_pdl(product_planes_kernel<KP, NT>, dim3(static_cast<unsigned>(std::min(g.tiles, per_sm * sms))),
-                       dim3(kThreads), S::kSmem, s, g, in, out);
+                       dim3(kThreads), smem, s, g, in, out);
     return e == cudaSuccess ? DN_OK : dn_cuda_fail(e, "linear8: planes launch");
 }
 

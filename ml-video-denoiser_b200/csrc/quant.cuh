@@ -5,20 +5,22 @@
 // The codes are exact: x_k and s are taken as they are, and the quotient is
 // never rounded to the wrong side of a border between two codes.
 //
-//   FP32 rows. q0 = rint(x * fl32(1/s)) is off by at most one, and
-//   r = fma(-q0, s, x) is exact (x - q0 s is a multiple of ulp(s)/2 below
-//   0.51 s), so comparing 2|r| with s settles it.
+//   FP32 rows. q0 = rint(x * r), r = 1/s to 2^-22, is off by at most one, and
+//   x - q0 s = fma(-q0, s, x) is exact (a multiple of ulp(s)/2 below 0.51 s),
+//   so comparing twice its magnitude with s settles it.
 //
 //   FP16 rows. x / s = (qmax x / a)(1 + d) with |d| < 2^-22, and qmax x / a
 //   is a quotient of whole numbers (11-bit significands): it is a half, or at
-//   least 2^-19 (relative) away from one. So x * fl32(1/s) is on the right
-//   side but where qmax x / a is a half exactly. Then the sign of
-//   s - a / qmax decides, which fma(s, qmax, -a) gives exactly: scaling 1/s
-//   by 1 -+ 2^-21 moves those products to the side they belong to and no
-//   other one across a border. Where s = a / qmax exactly, the quotient can
-//   be a half, and one correction step, t + fma(-t, s, x) / s, returns it
-//   correctly rounded. This was checked for all pairs of significands; it
-//   costs a multiply and an add per value instead of a division.
+//   least 2^-19 (relative) away from one. So x * r, r = 1/s to 2^-22, is on
+//   the right side but where qmax x / a is a half exactly. Then the sign of
+//   s - a / qmax decides, which fma(s, qmax, -a) gives exactly: scaling r by
+//   1 -+ 2^-21 moves those products to the side they belong to and no other
+//   one across a border. Where s = a / qmax exactly (8 of 1024 significands
+//   at 8 bits), the quotient can be a half, and one correction step, t +
+//   fma(-t, s, x) * r, returns it correctly rounded. It was checked for all
+//   pairs of significands, and costs a multiply and an add per value instead
+//   of a division; the rare groups (that case, and groups that are not finite)
+//   take a slower path together with their warp.
 #pragma once
 
 #include <cstdint>
@@ -33,11 +35,16 @@ constexpr float kRint = 12582912.f;            // 1.5 * 2^23: adding it rounds t
 
 // One group's scale and what the codes are made with.
 struct GroupScale {
-    float s;
-    float inv;      // 0 for a group that holds a NaN or an infinity
-    float fix;      // fl32(1/s) where the correction step is needed, else 0
-    uint32_t mask;  // all ones, or 0 for such a group: its codes are 0
+    float s;    // NaN for a group that holds a NaN or an infinity
+    float r;    // 1 / s, biased (FP16)
+    bool rare;  // the codes need codes8_rare
 };
+
+__device__ __forceinline__ float reciprocal(float x) {  // to 1 ulp
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 
 // Magnitude bits of 8 packed fp16 values / of fp32 values: the unsigned
 // maximum orders finite < infinity < NaN.
@@ -109,56 +116,77 @@ template <typename T>
 __device__ __forceinline__ GroupScale group_scale(uint32_t mag, float qmax) {
     const float a = QuantOf<T>::mag_value(mag);
     GroupScale g;
-    g.mask = a <= 3.402823466e38f ? 0xffffffffu : 0u;
-    g.s = g.mask ? fmaxf(__fmul_rn(a, qmax == 127.f ? 1.f / 127.f : 1.f / 7.f), kTinyScale) : __uint_as_float(0x7fc00000u);
-    g.inv = g.mask ? __frcp_rn(g.s) : 0.f;
-    g.fix = 0.f;
-    if (!QuantOf<T>::kF32) {
+    g.s = fmaxf(__fmul_rn(a, qmax == 127.f ? 1.f / 127.f : 1.f / 7.f), kTinyScale);
+    g.r = reciprocal(g.s);
+    if (QuantOf<T>::kF32) {
+        g.rare = true;
+    } else {
         const float d = fmaf(g.s, qmax, -a);  // exact sign of s - a / qmax
-        if (d == 0.f)
-            g.fix = g.inv;
-        else
-            g.inv *= d > 0.f ? 1.f - 4.76837158e-7f : 1.f + 4.76837158e-7f;
+        g.r *= d > 0.f ? 1.f - 4.76837158e-7f : 1.f + 4.76837158e-7f;
+        g.rare = !(d > 0.f || d < 0.f);  // exact, or not finite
     }
+    if (!(a <= 3.402823466e38f)) g.s = __uint_as_float(0x7fc00000u);
     return g;
 }
 
-// Codes of 8 values, one a byte. `fix`: whether any lane of the warp has
-// g.fix != 0 (FP16 only; warp-uniform).
+// The low byte of each of 8 words.
+__device__ __forceinline__ uint2 low_bytes(const uint32_t (&u)[8]) {
+    uint2 w;
+    w.x = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+    w.y = __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410);
+    return w;
+}
+
+// Codes of 8 FP16 values of a group that is not rare, one a byte.
+__device__ __forceinline__ uint2 codes8_fast(const QuantOf<__half>::Vec& x, float r) {
+    float f[8];
+    QuantOf<__half>::unpack(x, f);
+    const float2 r2 = make_float2(r, r), zero2 = make_float2(0.f, 0.f);
+    const float2 magic2 = make_float2(kRint, kRint), one2 = make_float2(1.f, 1.f);
+    uint32_t u[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 t = ffma2(ffma2(make_float2(f[2 * i], f[2 * i + 1]), r2, zero2), one2, magic2);
+        u[2 * i] = __float_as_uint(t.x);
+        u[2 * i + 1] = __float_as_uint(t.y);
+    }
+    return low_bytes(u);
+}
+
+// Codes of 8 values of any group.
 template <typename T>
-__device__ __forceinline__ uint2 codes8(const typename QuantOf<T>::Vec& x, const GroupScale& g, bool fix) {
+__device__ __forceinline__ uint2 codes8_rare(const typename QuantOf<T>::Vec& x, const GroupScale& g) {
     float f[8];
     QuantOf<T>::unpack(x, f);
     uint32_t u[8];
-    if (QuantOf<T>::kF32) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float v = g.mask ? f[i] : 0.f;  // a group that is not finite: codes 0
-            const float q0 = __fsub_rn(__fmaf_rn(v, g.inv, kRint), kRint);
-            const float r = __fmaf_rn(-q0, g.s, v);
-            const float r2 = 2.f * fabsf(r);  // exact; infinite for no finite group (r < 0.51 s)
+    for (int i = 0; i < 8; ++i) {
+        const float v = g.s == g.s ? f[i] : 0.f;  // a group that is not finite: codes 0
+        if (QuantOf<T>::kF32) {
+            const float q0 = __fsub_rn(__fmaf_rn(v, g.r, kRint), kRint);
+            const float rest = __fmaf_rn(-q0, g.s, v);
+            const float two = 2.f * fabsf(rest);
             const int q = static_cast<int>(q0);
-            const bool over = r2 > g.s || (r2 == g.s && (q & 1));
-            u[i] = static_cast<uint32_t>(over ? q + (r > 0.f ? 1 : -1) : q);
-        }
-    } else {
-        const float2 inv2 = make_float2(g.inv, g.inv), zero2 = make_float2(0.f, 0.f);
-        const float2 magic2 = make_float2(kRint, kRint), one2 = make_float2(1.f, 1.f);
-        const float2 ns2 = make_float2(-g.s, -g.s), fix2 = make_float2(g.fix, g.fix);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 v = make_float2(f[2 * i], f[2 * i + 1]);
-            float2 t = ffma2(v, inv2, zero2);
-            if (fix) t = ffma2(ffma2(t, ns2, v), fix2, t);
-            t = ffma2(t, one2, magic2);
-            u[2 * i] = __float_as_uint(t.x);
-            u[2 * i + 1] = __float_as_uint(t.y);
+            const bool over = two > g.s || (two == g.s && (q & 1));
+            u[i] = g.s == g.s ? static_cast<uint32_t>(over ? q + (rest > 0.f ? 1 : -1) : q) : 0u;
+        } else {
+            float t = __fmul_rn(v, g.r);
+            if (g.rare) t = fmaf(fmaf(-t, g.s, v), g.r, t);
+            u[i] = g.s == g.s ? __float_as_uint(__fadd_rn(t, kRint)) : 0u;
         }
     }
-    uint2 w;
-    w.x = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410) & g.mask;
-    w.y = __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410) & g.mask;
-    return w;
+    return low_bytes(u);
+}
+
+// Codes of 8 values; `rare`: whether a lane of the warp has a rare group
+// (warp-uniform; always for FP32).
+template <typename T>
+__device__ __forceinline__ uint2 codes8(const typename QuantOf<T>::Vec& x, const GroupScale& g, bool rare) {
+    if constexpr (QuantOf<T>::kF32) {
+        return codes8_rare<T>(x, g);
+    } else {
+        return rare ? codes8_rare<T>(x, g) : codes8_fast(x, g.r);
+    }
 }
 
 // 8 byte codes -> 8 nibbles (the even one in the low half of each byte).

@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kThreads) write_vec_kernel(const WriteArgs a) 
 #pragma unroll
         for (int d = SG / 2; d > 0; d >>= 1) mag = max(mag, __shfl_xor_sync(0xffffffffu, mag, d));
         const GroupScale g = group_scale<T>(mag, qmax);
-        const bool fix = !Q::kF32 && __any_sync(0xffffffffu, g.fix != 0.f);
+        const bool rare = __any_sync(0xffffffffu, g.rare);
         const int64_t slot = there ? slot_of(a, row[i]) : -1;
         if (!wins<SG>(a, row[i], grp[i], slot, there)) continue;
         uint8_t* dst = a.p.codes + slot * a.p.ldc + static_cast<int64_t>(grp[i]) * a.p.group * a.p.bits / 8;
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(kThreads) write_vec_kernel(const WriteArgs a) 
         for (int k = 0; k < V; ++k) {
             const int c = l + k * SG;
             if (c < nv) {
-                const uint2 w = codes8<T>(v[i][k], g, fix);
+                const uint2 w = codes8<T>(v[i][k], g, rare);
                 if (a.p.bits == 8)
                     *reinterpret_cast<uint2*>(dst + c * 8) = w;
                 else
@@ -158,13 +158,13 @@ __global__ void __launch_bounds__(kThreads) write_any_kernel(const WriteArgs a) 
     for (int c = lane * 8; c < n; c += 256) mag = max(mag, Q::mag(Q::load_some(src + c, min(8, n - c))));
     mag = __reduce_max_sync(0xffffffffu, mag);
     const GroupScale g = group_scale<T>(mag, qmax);
-    const bool fix = !Q::kF32 && g.fix != 0.f;  // the same on every lane
+    const bool rare = g.rare;  // the same on every lane
     const int64_t slot = slot_of(a, row);
     if (!wins<32>(a, row, grp, slot, true)) return;
     uint8_t* dst = a.p.codes + slot * a.p.ldc + static_cast<int64_t>(grp) * n * a.p.bits / 8;
     for (int c = lane * 8; c < n; c += 256) {
         const int m = min(8, n - c);
-        const uint2 w = codes8<T>(Q::load_some(src + c, m), g, fix);
+        const uint2 w = codes8<T>(Q::load_some(src + c, m), g, rare);
         if (a.p.bits == 8) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
