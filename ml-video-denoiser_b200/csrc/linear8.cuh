@@ -72,6 +72,22 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, int (&r)[32]) {
         : "r"(taddr));
 }
 
+// One lane of a converged warp, always the same one. Roles of a single thread
+// run their loops with the whole warp and elect a lane around each MMA, commit
+// or copy only: the loop stays warp-uniform, so that descriptors, coordinates
+// and barrier addresses live in uniform registers. Under `if (lane == 0)` every
+// operand of an MMA was moved there one by one, and a loop of two MMAs took
+// 1100 cycles.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(e));
+    return e != 0;
+}
+
 __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 

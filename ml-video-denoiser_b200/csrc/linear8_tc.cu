@@ -44,11 +44,14 @@ constexpr int kEpiWarps = 8;
 constexpr int kStageA = kRows * 128;
 constexpr int kStgWarp = 32 * 128;  // staging tile of an epilogue warp: 32 rows x 128 bytes
 
+// Shared memory: the ring of operand stages (at most kStages), the resident
+// weight if there is one, the epilogue's staging tiles.
 template <int NT>
 struct Plan {
     static constexpr int kStage = kStageA + NT * 128;
-    static constexpr int kStages = NT == 256 ? 4 : NT == 128 ? 5 : 6;
-    static constexpr int kBytes = 1024 + kStages * kStage + kEpiWarps * kStgWarp;
+    static constexpr int kStages = NT == 256 ? 4 : NT == 128 ? 5 : 8;
+    static constexpr int kRing = NT == 256 ? 4 * kStage : NT == 128 ? 5 * kStage : 6 * (kStageA + 64 * 128);
+    static constexpr int kBytes = 1024 + kRing + kEpiWarps * kStgWarp;
 };
 
 struct Maps {
@@ -61,6 +64,10 @@ struct TcArgs {
     int m_tiles, n_tiles;
     int tma_out;         // 1: staged TMA stores
     int unit;            // columns of a staging tile
+    int resident;        // the whole weight stays in shared memory (one column tile)
+    int stage, stages;   // bytes and number of the ring's stages
+    int units;           // K chunks of a stage: 1, or (resident weight) all of a tile's
+    int seg_full;        // accumulators are handed over one by one, not a tile's together
     int vec_out;         // direct stores: 16-byte vectors of a row are aligned
 };
 
@@ -78,13 +85,15 @@ template <typename T, int NT, bool SEG>
 __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_constant__ TcArgs g,
                                                                  const __grid_constant__ Maps maps) {
     using P = Plan<NT>;
-    constexpr int kSt = P::kStages;
+    const int kSt = g.stages;  // stages of the ring
     constexpr int kVec = 16 / sizeof(T);      // values of 16 bytes
-    constexpr int kAcc = NT == 256 ? 2 : 4;   // accumulators of the ring
+    constexpr int kAcc = SEG ? 512 / NT : NT == 256 ? 2 : 4;  // accumulators of the ring
     constexpr uint32_t kCols = kAcc * NT;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    __shared__ uint64_t bar_full[kSt], bar_empty[kSt], bar_acc_full[kAcc], bar_acc_empty[kAcc];
+    __shared__ uint64_t bar_full[P::kStages], bar_empty[P::kStages], bar_b, bar_acc_full[kAcc], bar_acc_empty[kAcc], bar_tile[8];
+    // A tile's scales, [segment][token] per epilogue warp.
+    __shared__ float s_scale[SEG ? kEpiWarps : 1][SEG ? kMaxSegments : 1][32];
     __shared__ uint32_t tslot;
     __shared__ volatile int s_abort;
     const ProductArgs& p = g.p;
@@ -97,9 +106,13 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
     }
     if (tid == 0) {
         for (int s = 0; s < kSt; ++s) {
-            mbar_init(&bar_full[s], 2);
+            mbar_init(&bar_full[s], g.resident ? 1 : 2);
             mbar_init(&bar_empty[s], 1);
         }
+        mbar_init(&bar_b, 1);
+        // The ring holds at most four tiles of two segments, so that a tile's
+        // barrier is waited for before it comes round again.
+        for (int b = 0; b < 8; ++b) mbar_init(&bar_tile[b], 1);
         for (int b = 0; b < kAcc; ++b) {
             mbar_init(&bar_acc_full[b], 1);
             mbar_init(&bar_acc_empty[b], kEpiWarps);
@@ -120,67 +133,124 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
     constexpr int half = NT / 2;
     const int out_cols = p.gate ? half : NT;  // output columns of a tile
 
-    if (warp == 8 || warp == 9) {
-        if (lane == 0) {
-            const uint32_t bytes = static_cast<uint32_t>(warp == 8 ? kRows : NT) * g.kc;
-            int it = 0;
-            bool ok = true;
-            for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
-                const int m0 = (tile / g.n_tiles) * kRows, n0 = (tile % g.n_tiles) * out_cols;
-                for (int t = 0; ok && t < p.segs; ++t)
-                    for (int j = 0; j < g.chunks; ++j, ++it) {
-                        const int s = it % kSt;
-                        ok = wait_or_abort(&bar_empty[s], ((it / kSt) & 1) ^ 1, &s_abort, p.err, 0x70);
-                        if (!ok) break;
-                        uint8_t* sa = smem + s * P::kStage;
-                        mbar_arrive_expect_tx(&bar_full[s], bytes);
-                        if (warp == 8) {
-                            tma_load_2d(sa, &maps.a, j * g.kc, static_cast<int>(p.arow[t]) + m0, &bar_full[s]);
-                        } else {
-                            uint8_t* sb = sa + kStageA;
-                            const int k = t * p.seg_p + j * g.kc;
-                            tma_load_2d(sb, &maps.b, k, n0, &bar_full[s]);
-                            if (p.gate) tma_load_2d(sb + half * g.kc, &maps.b, k, p.n_out + n0, &bar_full[s]);
-                        }
-                    }
+    uint8_t* b_res = smem + kSt * g.stage;  // resident weight: its chunks one behind the other
+    const int seg_c = p.seg_c, segs = p.segs, chunks = g.chunks, kc = g.kc, units = g.units, stage = g.stage;
+    if (warp == 9 && g.resident) {
+        if (elect_one()) {
+            mbar_arrive_expect_tx(&bar_b, static_cast<uint32_t>(segs * chunks * NT * kc));
+            for (int i = 0; i < segs * chunks; ++i) {
+                uint8_t* sb = b_res + i * (NT * kc);
+                const int k = (i / chunks) * p.seg_p + (i % chunks) * kc;
+                tma_load_2d(sb, &maps.b, k, 0, &bar_b);
+                if (p.gate) tma_load_2d(sb + half * kc, &maps.b, k, p.n_out, &bar_b);
             }
-            // After a wait that ran out: the copies in flight land before the CTA leaves.
-            if (!ok)
-                for (int k = max(0, it - kSt); k < it; ++k) mbar_wait(&bar_full[k % kSt], (k / kSt) & 1, 100000000ull);
+            // It has landed before this CTA leaves, whatever became of the others.
+            wait_or_abort(&bar_b, 0, &s_abort, p.err, 0x77);
         }
-    } else if (warp == 10) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = idesc_s8(kRows, NT);
-            const uint32_t sm0 = smem_u32(smem);
-            const uint64_t ad0 = sdesc_kmajor_sw(sm0, g.kc), bd0 = sdesc_kmajor_sw(sm0 + kStageA, g.kc);
-            int it = 0, q = 0;
-            bool ok = true;
-            for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
-                for (int t = 0; ok && t < p.segs; ++t, ++q) {
-                    const int b = q % kAcc;
-                    ok = wait_or_abort(&bar_acc_empty[b], ((q / kAcc) & 1) ^ 1, &s_abort, p.err, 0x71);
+    } else if (warp == 8) {
+        const uint32_t bytes = static_cast<uint32_t>(kRows * kc * units);
+        int filled = 0, left = 0, s = 0;  // stages begun, chunks that the current one still takes
+        uint32_t ph = 1;
+        bool ok = true;
+        for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+            const int m0 = (tile / g.n_tiles) * kRows;
+            for (int t = 0; ok && t < segs; ++t) {
+                const int row = static_cast<int>(p.arow[t]) + m0;
+                for (int j = 0; j < chunks; ++j) {
+                    if (left == 0) {
+                        ok = wait_or_abort(&bar_empty[s], ph, &s_abort, p.err, 0x70);
+                        if (!ok) break;
+                        if (elect_one()) mbar_arrive_expect_tx(&bar_full[s], bytes);
+                        left = units;
+                        ++filled;
+                    }
+                    uint8_t* sa = smem + s * stage + (units - left) * (kRows * kc);
+                    if (elect_one()) tma_load_2d(sa, &maps.a, j * kc, row, &bar_full[s]);
+                    if (--left == 0 && ++s == kSt) s = 0, ph ^= 1;
+                }
+            }
+        }
+        // After a wait that ran out: the copies in flight land before the CTA leaves.
+        if (!ok)
+            for (int k = max(0, filled - kSt); k < filled; ++k) mbar_wait(&bar_full[k % kSt], (k / kSt) & 1, 100000000ull);
+    } else if (warp == 9) {
+        const uint32_t bytes = static_cast<uint32_t>(NT * kc);
+        int filled = 0, s = 0;
+        uint32_t ph = 1;
+        bool ok = true;
+        for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+            const int n0 = (tile % g.n_tiles) * out_cols;
+            for (int t = 0; ok && t < segs; ++t)
+                for (int j = 0; j < chunks; ++j) {
+                    ok = wait_or_abort(&bar_empty[s], ph, &s_abort, p.err, 0x70);
                     if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t acc = tmem + b * NT;
-                    for (int j = 0; j < g.chunks; ++j, ++it) {
-                        const int s = it % kSt;
-                        ok = wait_or_abort(&bar_full[s], (it / kSt) & 1, &s_abort, p.err, 0x72);
+                    uint8_t* sb = smem + s * stage + kStageA;
+                    const int k = t * p.seg_p + j * kc;
+                    if (elect_one()) {
+                        mbar_arrive_expect_tx(&bar_full[s], bytes);
+                        tma_load_2d(sb, &maps.b, k, n0, &bar_full[s]);
+                        if (p.gate) tma_load_2d(sb + half * kc, &maps.b, k, p.n_out + n0, &bar_full[s]);
+                    }
+                    ++filled;
+                    if (++s == kSt) s = 0, ph ^= 1;
+                }
+        }
+        if (!ok)
+            for (int k = max(0, filled - kSt); k < filled; ++k) mbar_wait(&bar_full[k % kSt], (k / kSt) & 1, 100000000ull);
+    } else if (warp == 10) {
+        constexpr uint32_t idesc = idesc_s8(kRows, NT);
+        const uint32_t sm0 = smem_u32(smem);
+        const uint64_t ad0 = sdesc_kmajor_sw(sm0, kc);
+        const uint64_t bd0 = sdesc_kmajor_sw(g.resident ? smem_u32(b_res) : sm0 + kStageA, kc);
+        const uint32_t a_unit = (kRows * kc) >> 4;                         // from chunk to chunk of a stage
+        const uint32_t b_unit = g.resident ? (NT * kc) >> 4 : 0;           // of the resident weight
+        const uint32_t b_stage = g.resident ? 0 : stage >> 4;              // from stage to stage
+        int s = 0, b = 0, n = 0, left = 0;
+        uint32_t ph = 0, acc_ph = 1;
+        uint64_t ad = ad0;
+        bool ok = !g.resident || wait_or_abort(&bar_b, 0, &s_abort, p.err, 0x78);
+        for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++n) {
+            uint64_t bd = bd0;  // of the chunk, but for the stage
+            for (int t = 0; ok && t < segs; ++t) {
+                ok = wait_or_abort(&bar_acc_empty[b], acc_ph, &s_abort, p.err, 0x71);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t acc = tmem + b * NT;
+                int steps_left = (seg_c + 31) / 32;
+                for (int j = 0; j < chunks; ++j) {
+                    if (left == 0) {
+                        ok = wait_or_abort(&bar_full[s], ph, &s_abort, p.err, 0x72);
                         if (!ok) break;
                         tc_fence_after();
-                        const uint64_t so = static_cast<uint64_t>(s) * (P::kStage >> 4);
-                        const int steps = min(g.kc, p.seg_c - j * g.kc + 31) / 32;
+                        left = units;
+                        ad = ad0 + static_cast<uint32_t>(s * (stage >> 4));
+                    }
+                    const uint64_t bs = bd + s * b_stage;
+                    if (elect_one()) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            if (k < steps) mma_s8(acc, ad0 + so + 2 * k, bd0 + so + 2 * k, idesc, (j > 0 || k > 0) ? 1u : 0u);
-                        mma_commit(&bar_empty[s]);
+                            if (k < steps_left && k * 32 < kc)
+                                mma_s8(acc, ad + 2 * k, bs + 2 * k, idesc, (j > 0 || k > 0) ? 1u : 0u);
+                        if (left == 1) mma_commit(&bar_empty[s]);
+                        if (j == chunks - 1) {
+                            if (g.seg_full)
+                                mma_commit(&bar_acc_full[b]);
+                            else if (t == segs - 1)
+                                mma_commit(&bar_tile[n & 7]);
+                        }
                     }
-                    if (ok) mma_commit(&bar_acc_full[b]);
+                    __syncwarp();
+                    steps_left -= kc / 32;
+                    ad += a_unit;
+                    bd += b_unit;
+                    if (--left == 0 && ++s == kSt) s = 0, ph ^= 1;
                 }
+                if (++b == kAcc) b = 0, acc_ph ^= 1;
             }
         }
     } else {
         const int quad = warp & 3, group = warp >> 2;
-        uint8_t* stg = smem + kSt * P::kStage + warp * kStgWarp;
+        uint8_t* stg = smem + P::kRing + warp * kStgWarp;
         const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16);
         T* out = static_cast<T*>(p.out);
         // 32 finished values of a lane's row, tile columns c .. c + 31; in a
@@ -211,9 +281,8 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
                 bulk_commit();
             }
         };
-        auto acc_wait = [&](int q) {
-            const bool ok =
-                lane == 0 ? wait_or_abort(&bar_acc_full[q % kAcc], (q / kAcc) & 1, &s_abort, p.err, 0x73) : true;
+        auto full_wait = [&](uint64_t* bar, int use) {
+            const bool ok = lane == 0 ? wait_or_abort(bar, use & 1, &s_abort, p.err, 0x73) : true;
             const bool all = __shfl_sync(0xffffffffu, ok, 0);
             tc_fence_after();
             return all;
@@ -223,8 +292,25 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar_acc_empty[q % kAcc]);
         };
+        // The scales of a lane's token, loaded a tile ahead: their latency would
+        // otherwise show in every tile.
+        constexpr int kScales = SEG ? kMaxSegments : 1;
+        float next[kScales];
+        auto load_scales = [&](int tile) {
+            const int64_t row = static_cast<int64_t>(tile / g.n_tiles) * kRows + quad * 32 + lane;
+#pragma unroll
+            for (int t = 0; t < kScales; ++t)
+                next[t] = t < p.segs && tile < tiles && row < p.rows ? __ldg(p.as + p.arow[t] + row) : 0.f;
+        };
         int q = 0, n = 0;
+        load_scales(blockIdx.x);
         for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
+            const float s = next[0];
+            if constexpr (SEG) {
+#pragma unroll
+                for (int t = 0; t < kScales; ++t) s_scale[warp][t][lane] = next[t];  // read by this lane alone
+            }
+            load_scales(tile + gridDim.x);
             const int64_t m0 = static_cast<int64_t>(tile / g.n_tiles) * kRows + quad * 32;
             const int n0 = (tile % g.n_tiles) * out_cols;
             const int64_t row = m0 + lane;
@@ -233,28 +319,27 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
                 // A warp takes 32-column blocks: NT/2 columns of its group of
                 // warps, or (gated, NT = 128) 32 of each factor.
                 constexpr int kBlocks = NT / 64;
-                float s[kMaxSegments];
-#pragma unroll
-                for (int t = 0; t < kMaxSegments; ++t)
-                    s[t] = t < p.segs && row < p.rows ? __ldg(p.as + p.arow[t] + row) : 0.f;
                 float y[kBlocks][32];
                 int col[kBlocks];
 #pragma unroll
                 for (int k = 0; k < kBlocks; ++k) col[k] = p.gate ? k * half + group * 32 : group * half + k * 32;
-                bool ok = true;
+                bool ok = g.seg_full || full_wait(&bar_tile[n & 7], n >> 3);
+                if (!ok) break;
 #pragma unroll
-                for (int t = 0; t < kMaxSegments; ++t) {
-                    if (t >= p.segs) break;
-                    ok = acc_wait(q);
-                    if (!ok) break;
+                for (int k = 0; k < kBlocks; ++k)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) y[k][i] = 0.f;
+#pragma unroll 1
+                for (int t = 0; t < p.segs; ++t) {
+                    const float st = s_scale[warp][t][lane];
+                    if (g.seg_full && !(ok = full_wait(&bar_acc_full[q % kAcc], q / kAcc))) break;
 #pragma unroll
                     for (int k = 0; k < kBlocks; ++k) {
                         int a[32];
                         tmem_ld32(lane_base + (q % kAcc) * NT + col[k], a);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            y[k][i] = t == 0 ? static_cast<float>(a[i]) * s[0] : fmaf(static_cast<float>(a[i]), s[t], y[k][i]);
+                        for (int i = 0; i < 32; ++i) y[k][i] = fmaf(static_cast<float>(a[i]), st, y[k][i]);
                     }
                     acc_done(q);
                     ++q;
@@ -280,8 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
                     }
                 }
             } else {
-                const float s = row < p.rows ? __ldg(p.as + p.arow[0] + row) : 0.f;
-                if (!acc_wait(q)) break;
+                if (!full_wait(&bar_acc_full[q % kAcc], q / kAcc)) break;
                 const uint32_t acc = lane_base + (q % kAcc) * NT;
                 auto scaled = [&](int c, const float2* par, float (&y)[32]) {
                     int a[32];
@@ -333,6 +417,20 @@ int run(TcArgs& g, int sms, cudaStream_t s) {
     g.n_tiles = (p.n_out + out_cols - 1) / out_cols;
     const bool al16 = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo * sizeof(T) % 16 == 0 && p.ldo >= p.n_out;
     g.tma_out = g.vec_out = !p.planes && al16;
+    // A weight of one column tile that leaves room for four stages of codes
+    // stays in shared memory.
+    const int64_t b_bytes = static_cast<int64_t>(p.segs) * g.chunks * NT * g.kc;
+    g.resident = g.n_tiles == 1 && b_bytes <= Plan<NT>::kRing - 4 * kStageA;
+    g.stage = g.resident ? kRows * g.kc : Plan<NT>::kStage;
+    const int ring = Plan<NT>::kRing - static_cast<int>(g.resident ? b_bytes : 0);
+    // With a resident weight all of a tile's chunks make one stage where three
+    // fit: fewer waits and commits.
+    const int tile_bytes = p.segs * g.chunks * g.stage;
+    g.units = g.resident && 3 * tile_bytes <= ring ? p.segs * g.chunks : 1;
+    g.stage *= g.units;
+    g.stages = std::min<int>(Plan<NT>::kStages, ring / g.stage);
+    // A tile's accumulators together where the ring holds them all.
+    g.seg_full = !SEG || p.segs > 512 / NT;
     // Staging tiles of 128-byte rows; 32 columns with segments (a warp's
     // blocks), and for direct stores.
     g.unit = SEG || !g.tma_out ? 32 : std::min<int>(128 / sizeof(T), out_cols);
