@@ -88,6 +88,9 @@ __device__ __forceinline__ bool elect_one() {
     return e != 0;
 }
 
+// The warp's index as a value that the compiler knows to be warp-uniform.
+__device__ __forceinline__ int warp_index() { return __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0); }
+
 __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 

@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(Shape<PLANES, SG, NT>::kThreads) product_fused
     __shared__ float s_x[2][kRows];       // the tokens' scales, of this and the previous tile
     __shared__ float2 s_par[NT];          // scale and bias of each weight row
     const ProductArgs& p = g.p;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
     uint8_t* sa = smem;
     uint8_t* sb = smem + S::kA;
     uint8_t* stg = smem + S::kA + S::kB + warp * 32 * 128;
@@ -205,17 +205,20 @@ __global__ void __launch_bounds__(Shape<PLANES, SG, NT>::kThreads) product_fused
         fence_async_smem();
         tc_fence_before();
         __syncthreads();  // the operand is complete, and every warp is done with the previous accumulator
-        if (tid == 0) {
+        if (warp == 0) {
             tc_fence_after();
+            if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < S::kBytesK / 32; ++k)
-                if (k < steps) {
-                    const uint32_t span_steps = S::kSpan / 32;
-                    const uint32_t s = k / span_steps, o = 2 * (k % span_steps);
-                    mma_s8(tmem, ad0 + s * ((kRows * S::kSpan) >> 4) + o, bd0 + s * ((NT * S::kSpan) >> 4) + o,
-                           idesc_s8(kRows, NT), k > 0 ? 1u : 0u);
-                }
-            mma_commit(&bar);
+                for (int k = 0; k < S::kBytesK / 32; ++k)
+                    if (k < steps) {
+                        const uint32_t span_steps = S::kSpan / 32;
+                        const uint32_t s = k / span_steps, o = 2 * (k % span_steps);
+                        mma_s8(tmem, ad0 + s * ((kRows * S::kSpan) >> 4) + o, bd0 + s * ((NT * S::kSpan) >> 4) + o,
+                               idesc_s8(kRows, NT), k > 0 ? 1u : 0u);
+                    }
+                mma_commit(&bar);
+            }
+            __syncwarp();
         }
         if (tile + static_cast<int>(gridDim.x) < g.m_tiles) load(tile + gridDim.x);
         // A wait that runs out marks the launch as failed and lets the CTA finish.

@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(kThreads) product_planes_kernel(const __grid_c
     __shared__ float s_x[2][kRows];
     __shared__ __align__(16) float2 s_par[NT];
     const ProductArgs& p = g.p;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
     uint8_t* s_in = smem;
     uint8_t* sa = smem + 2 * S::kIn;
     uint8_t* sb = sa + S::kA;
@@ -197,14 +197,17 @@ __global__ void __launch_bounds__(kThreads) product_planes_kernel(const __grid_c
         tc_fence_before();
         if (issues) bulk_wait_read0();
         __syncthreads();  // the operand is complete; this input buffer, the accumulator and the output tile are free
-        if (tid == 0) {
+        if (warp == 0) {
             tc_fence_after();
+            if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < KP / 32; ++k)
-                if (k < steps) mma_s8(tmem, ad0 + 2 * k, bd0 + 2 * k, idesc_s8(kRows, NT), k > 0 ? 1u : 0u);
-            mma_commit(&bar);
-            const int64_t next = static_cast<int64_t>(tile) + 2 * static_cast<int64_t>(gridDim.x);
-            if (next < g.tiles) load(static_cast<int>(next), b);
+                for (int k = 0; k < KP / 32; ++k)
+                    if (k < steps) mma_s8(tmem, ad0 + 2 * k, bd0 + 2 * k, idesc_s8(kRows, NT), k > 0 ? 1u : 0u);
+                mma_commit(&bar);
+                const int64_t next = static_cast<int64_t>(tile) + 2 * static_cast<int64_t>(gridDim.x);
+                if (next < g.tiles) load(static_cast<int>(next), b);
+            }
+            __syncwarp();
         }
         wait_or_abort(&bar, n & 1, &s_abort, p.err, 0x76);
         __syncwarp();

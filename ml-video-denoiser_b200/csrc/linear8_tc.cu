@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
     __shared__ uint32_t tslot;
     __shared__ volatile int s_abort;
     const ProductArgs& p = g.p;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
     const int tiles = g.m_tiles * g.n_tiles;
 
     if (warp == 10) {
