@@ -22,30 +22,58 @@ namespace {
 
 constexpr int kMaxK = 131072;  // 127 * 127 * 131072 < 2^31
 
-// Codes and scales of the pixels of NCHW planes: a thread per pixel.
+// Codes and scales of the pixels of NCHW planes (layers too wide for one pass):
+// a CTA of eight warps takes 32 pixels, a lane one of them and a warp 32
+// channels at a time, so that the loads of 32 channels are in flight and a
+// lane's codes are a whole 32-byte sector. Two passes over the planes; the
+// second finds them in L1 or L2.
 __global__ void __launch_bounds__(256) quantise_planes_kernel(const __half* __restrict__ x, int64_t rows, int K, int64_t hw,
                                                               uint8_t* __restrict__ codes, int64_t ldc,
                                                               float* __restrict__ scales) {
     using Q = QuantOf<__half>;
+    __shared__ uint32_t s_mag[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (threadIdx.x < 32) s_mag[threadIdx.x] = 0;
+    __syncthreads();
     pdl_trigger();
     pdl_wait();
-    const int64_t m = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t m = static_cast<int64_t>(blockIdx.x) * 32 + lane;
     const bool live = m < rows;
     const int64_t img = live ? m / hw : 0;
-    const __half* src = x + (img * K * hw + (live ? m - img * hw : 0));
-    uint32_t mag = 0;
-    for (int k = 0; k < K; ++k) mag = max(mag, static_cast<uint32_t>(__half_as_ushort(src[k * hw])) & 0x7fffu);
-    const GroupScale g = group_scale<__half>(mag, 127.f);
-    const bool rare = __any_sync(0xffffffffu, g.rare);
-    if (!live) return;
-    for (int k = 0; k < K; k += 8) {
-        uint32_t w[4] = {0, 0, 0, 0};
+    const __half* src = x + img * K * hw + (live ? m - img * hw : 0);
+    auto load = [&](int k0, Q::Vec (&v)[4]) {
+        uint32_t w[16];
+        const __half* p = src + k0 * hw;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (k + i < K) w[i >> 1] |= static_cast<uint32_t>(__half_as_ushort(src[(k + i) * hw])) << ((i & 1) * 16);
-        *reinterpret_cast<uint2*>(codes + m * ldc + k) = codes8<__half>(Q::Vec{make_uint4(w[0], w[1], w[2], w[3])}, g, rare);
+        for (int i = 0; i < 32; ++i, p += hw) {
+            const uint32_t h = live && k0 + i < K ? __half_as_ushort(__ldg(p)) : 0u;
+            w[i >> 1] = i & 1 ? w[i >> 1] | (h << 16) : h;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i].v = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    };
+    uint32_t mag = 0;
+    for (int k0 = warp * 32; k0 < K; k0 += 256) {
+        Q::Vec v[4];
+        load(k0, v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mag = max(mag, Q::mag(v[i]));
     }
-    scales[m] = g.s;
+    atomicMax(&s_mag[lane], mag);
+    __syncthreads();
+    const GroupScale g = group_scale<__half>(s_mag[lane], 127.f);
+    const bool rare = __any_sync(0xffffffffu, g.rare);
+    for (int k0 = warp * 32; k0 < K; k0 += 256) {
+        Q::Vec v[4];
+        load(k0, v);
+        uint8_t* dst = codes + m * ldc + k0;
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            const uint2 lo = codes8<__half>(v[i], g, rare), hi = codes8<__half>(v[i + 1], g, rare);
+            if (live && k0 + i * 8 < ldc) *reinterpret_cast<uint4*>(dst + i * 8) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        }
+    }
+    if (warp == 0 && live) scales[m] = g.s;
 }
 
 // par of ProductArgs from the weight rows' scales and the bias (may be null).
@@ -345,7 +373,7 @@ int dn_linear8_forward_nchw(dn_linear8* L, const void* input, int N, int H, int 
     a.lda = round16(L->cin);
     auto* codes = static_cast<uint8_t*>(workspace);
     auto* scales = reinterpret_cast<float*>(codes + rows * a.lda);
-    const cudaError_t e = launch_pdl(quantise_planes_kernel, dim3(static_cast<unsigned>((rows + 255) / 256)), dim3(256), 0, s,
+    const cudaError_t e = launch_pdl(quantise_planes_kernel, dim3(static_cast<unsigned>((rows + 31) / 32)), dim3(256), 0, s,
                                      static_cast<const __half*>(input), rows, L->cin, hw, codes, a.lda, scales);
     if (e != cudaSuccess) return dn_cuda_fail(e, "dn_linear8_forward_nchw: quantise launch");
     a.a = reinterpret_cast<const int8_t*>(codes);

@@ -38,7 +38,9 @@ struct FusedArgs {
     int64_t ldx;     // row stride (token rows)
     int m_tiles;
     int vec_in;      // token rows: 16-byte loads of x are aligned
-    int tma_out, vec_out;
+    int flat;        // token rows one behind the other that are no multiple of 16 bytes: loaded as one run
+    int tma_out;
+    int pairs;       // direct stores: pairs of outputs are 4-byte aligned
     int unit;        // columns of a staging tile (tma_out)
 };
 
@@ -59,7 +61,12 @@ struct Shape {
     static constexpr int kSubs = kBytesK / kSpan;
     static constexpr int kA = kRows * kBytesK, kB = NT * kBytesK;
     static constexpr int kStg = kWarps * 32 * 128;
+    // The tile's tokens as they came, where they are loaded as one run, come
+    // behind that; up to kRunK channels, so that a CTA stays below 223 KB.
     static constexpr int kSmem = 1024 + kA + kB + kStg;
+    static constexpr int kRoomK = (228352 - kSmem) / (kRows * 2);
+    static constexpr int kRunK = PLANES ? 0 : kRoomK < 8 * SG ? kRoomK : 8 * SG;
+    static constexpr int smem(int run_k) { return kSmem + kRows * 2 * run_k; }
 };
 
 template <typename T, bool PLANES, int SG, int NT>
@@ -136,6 +143,18 @@ __global__ void __launch_bounds__(Shape<PLANES, SG, NT>::kThreads) product_fused
                 }
                 v[i].v = make_uint4(w[0], w[1], w[2], w[3]);
             }
+        } else if (g.flat) {
+            // This warp's rows are one run of kWarpRows K values from a 16-byte boundary on.
+            const int64_t first = (static_cast<int64_t>(tile) * kRows + warp * kWarpRows) * K;
+            const int64_t end = p.rows * K;
+#pragma unroll
+            for (int i = 0; i < S::kVecs; ++i) {
+                const int f = (lane + 32 * i) * 8;
+                const int64_t at = first + f;
+                v[i] = f >= kWarpRows * K || at >= end ? Q::zero()
+                       : at + 8 <= end                 ? Q::load(g.x + at)
+                                                       : Q::load_some(g.x + at, static_cast<int>(end - at));
+            }
         } else {
             const int64_t m0 = static_cast<int64_t>(tile) * kRows + warp * kWarpRows + sub;
             const bool in = l * 8 < K;
@@ -175,6 +194,19 @@ __global__ void __launch_bounds__(Shape<PLANES, SG, NT>::kThreads) product_fused
             }
             sx[r] = q.s;
         } else {
+            if (g.flat) {  // from the run to a lane's vectors of its rows
+                uint8_t* raw = smem + S::kA + S::kB + S::kStg + warp * kWarpRows * K * 2;
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < S::kVecs; ++i)
+                    if ((lane + 32 * i) * 8 < kWarpRows * K) *reinterpret_cast<uint4*>(raw + (lane + 32 * i) * 16) = v[i].v;
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < S::kVecs; ++i)
+                    v[i] = l * 8 < K ? Q::load_some(reinterpret_cast<const __half*>(raw) + (i * kPer + sub) * K + l * 8,
+                                                    min(8, K - l * 8))
+                                     : Q::zero();
+            }
             auto scale_of = [&](int i) {
                 uint32_t mag = Q::mag(v[i]);
 #pragma unroll
@@ -273,8 +305,8 @@ __global__ void __launch_bounds__(Shape<PLANES, SG, NT>::kThreads) product_fused
                     for (int i = 0; i < 32; i += kVec)
                         *reinterpret_cast<uint4*>(stg + sw_offset(lane, (c - c0 + i) / kVec, span)) =
                             pack16(y + i, static_cast<T*>(nullptr));
-                } else if (live) {
-                    store_row32(out + row * p.ldo + c, y, c, p.n_out, g.vec_out);
+                } else {
+                    store_block32(stg, y, out, p.ldo, m0, p.rows, c, p.n_out, g.pairs);
                 }
             }
             if (!PLANES && g.tma_out) {
@@ -300,7 +332,8 @@ int run(FusedArgs& g, int sms, cudaStream_t s) {
     const int out_cols = p.gate ? NT / 2 : NT;
     const bool al16 = !PLANES && reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo * sizeof(T) % 16 == 0 &&
                       p.ldo >= p.n_out;
-    g.tma_out = g.vec_out = al16;
+    g.tma_out = al16;
+    g.pairs = reinterpret_cast<uintptr_t>(p.out) % 4 == 0 && p.ldo % 2 == 0;
     // Staging rows of 128 bytes, or shorter ones so that every group of four
     // warps has columns to finish.
     g.unit = std::max(32, std::min<int>(128 / sizeof(T), out_cols / S::kGroups));
@@ -311,10 +344,13 @@ int run(FusedArgs& g, int sms, cudaStream_t s) {
     static int resident[64] = {};
     int per_sm = 0;
     auto kernel = product_fused_kernel<T, PLANES, SG, NT>;
-    cudaError_t e = tmem_kernel_ctas(kernel, S::kThreads, S::kSmem, S::kSmem, NT, resident, &per_sm);
+    g.flat = g.flat && p.seg_c <= S::kRunK;
+    const int smem = S::smem(g.flat ? p.seg_c : 0), most = S::smem(S::kRunK);
+    int fresh[64] = {};  // a run's buffer depends on Cin
+    cudaError_t e = tmem_kernel_ctas(kernel, S::kThreads, smem, most, NT, g.flat ? fresh : resident, &per_sm);
     if (e == cudaSuccess)
-        e = launch_pdl(kernel, dim3(static_cast<unsigned>(std::min(g.m_tiles, per_sm * sms))), dim3(S::kThreads), S::kSmem,
-                       s, g, map);
+        e = launch_pdl(kernel, dim3(static_cast<unsigned>(std::min(g.m_tiles, per_sm * sms))), dim3(S::kThreads), smem, s, g,
+                       map);
     return e == cudaSuccess ? DN_OK : dn_cuda_fail(e, "linear8: fused launch");
 }
 
@@ -350,6 +386,7 @@ int launch_product_fused(const ProductArgs& a, const void* x, int64_t ldx, int o
     g.x = static_cast<const __half*>(x);
     g.ldx = ldx;
     g.vec_in = a.seg_c % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0;
+    g.flat = !a.planes && !g.vec_in && ldx == a.seg_c && reinterpret_cast<uintptr_t>(x) % 16 == 0;
     g.m_tiles = static_cast<int>((a.rows + kRows - 1) / kRows);
     if (a.planes) return run_k<__half, true>(g, sms, s);
     return out_dtype == 1 ? run_k<__half, false>(g, sms, s) : run_k<float, false>(g, sms, s);

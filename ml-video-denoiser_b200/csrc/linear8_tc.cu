@@ -68,7 +68,7 @@ struct TcArgs {
     int stage, stages;   // bytes and number of the ring's stages
     int units;           // K chunks of a stage: 1, or (resident weight) all of a tile's
     int seg_full;        // accumulators are handed over one by one, not a tile's together
-    int vec_out;         // direct stores: 16-byte vectors of a row are aligned
+    int pairs;           // direct stores of FP16 rows: pairs are 4-byte aligned
 };
 
 // 32 columns from c on, (scale, bias) from par.
@@ -263,11 +263,10 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
                     pack16(y + i, static_cast<T*>(nullptr));
         };
         auto store32 = [&](const float (&y)[32], int c, int64_t row, int64_t img) {
-            if (row >= p.rows) return;
-            if (p.planes)
+            if (!p.planes)
+                store_block32(stg, y, out, p.ldo, row - lane, p.rows, c, p.n_out, g.pairs);
+            else if (row < p.rows)
                 store_planes32(out + (img * p.n_out + c) * p.ldo + (row - img * p.ldo), p.ldo, y, c, p.n_out);
-            else
-                store_row32(out + row * p.ldo + c, y, c, p.n_out, g.vec_out);
         };
         auto stage_free = [&]() {
             if (lane == 0) bulk_wait_read0();
@@ -416,7 +415,8 @@ int run(TcArgs& g, int sms, cudaStream_t s) {
     g.m_tiles = static_cast<int>((p.rows + kRows - 1) / kRows);
     g.n_tiles = (p.n_out + out_cols - 1) / out_cols;
     const bool al16 = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo * sizeof(T) % 16 == 0 && p.ldo >= p.n_out;
-    g.tma_out = g.vec_out = !p.planes && al16;
+    g.tma_out = !p.planes && al16;
+    g.pairs = reinterpret_cast<uintptr_t>(p.out) % 4 == 0 && p.ldo % 2 == 0;
     // A weight of one column tile that leaves room for four stages of codes
     // stays in shared memory.
     const int64_t b_bytes = static_cast<int64_t>(p.segs) * g.chunks * NT * g.kc;

@@ -73,6 +73,7 @@ struct QuantOf<__half> {
         const uint32_t a = umax16x2(umax16x2(x.v.x & m, x.v.y & m), umax16x2(x.v.z & m, x.v.w & m));
         return max(a >> 16, a & 0xffffu);
     }
+    __device__ static __forceinline__ uint32_t mag1(__half x) { return __half_as_ushort(x) & 0x7fffu; }
     __device__ static __forceinline__ float mag_value(uint32_t bits) {
         return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
     }
@@ -109,6 +110,7 @@ struct QuantOf<float> {
         for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
         return m;
     }
+    __device__ static __forceinline__ uint32_t mag1(float x) { return __float_as_uint(x) & 0x7fffffffu; }
     __device__ static __forceinline__ float mag_value(uint32_t bits) { return __uint_as_float(bits); }
 };
 
@@ -153,6 +155,27 @@ __device__ __forceinline__ uint2 codes8_fast(const QuantOf<__half>::Vec& x, floa
     return low_bytes(u);
 }
 
+// The code of one value of any group, in the low byte.
+template <typename T>
+__device__ __forceinline__ uint32_t code1f(float x, const GroupScale& g) {
+    const float v = g.s == g.s ? x : 0.f;  // a group that is not finite: codes 0
+    if (QuantOf<T>::kF32) {
+        const float q0 = __fsub_rn(__fmaf_rn(v, g.r, kRint), kRint);
+        const float rest = __fmaf_rn(-q0, g.s, v);
+        const float two = 2.f * fabsf(rest);
+        const int q = static_cast<int>(q0);
+        const bool over = two > g.s || (two == g.s && (q & 1));
+        return g.s == g.s ? static_cast<uint32_t>(over ? q + (rest > 0.f ? 1 : -1) : q) : 0u;
+    }
+    float t = __fmul_rn(v, g.r);
+    if (g.rare) t = fmaf(fmaf(-t, g.s, v), g.r, t);
+    return g.s == g.s ? __float_as_uint(__fadd_rn(t, kRint)) : 0u;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t code1(T x, const GroupScale& g) {
+    return code1f<T>(static_cast<float>(x), g);
+}
+
 // Codes of 8 values of any group.
 template <typename T>
 __device__ __forceinline__ uint2 codes8_rare(const typename QuantOf<T>::Vec& x, const GroupScale& g) {
@@ -160,21 +183,7 @@ __device__ __forceinline__ uint2 codes8_rare(const typename QuantOf<T>::Vec& x, 
     QuantOf<T>::unpack(x, f);
     uint32_t u[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float v = g.s == g.s ? f[i] : 0.f;  // a group that is not finite: codes 0
-        if (QuantOf<T>::kF32) {
-            const float q0 = __fsub_rn(__fmaf_rn(v, g.r, kRint), kRint);
-            const float rest = __fmaf_rn(-q0, g.s, v);
-            const float two = 2.f * fabsf(rest);
-            const int q = static_cast<int>(q0);
-            const bool over = two > g.s || (two == g.s && (q & 1));
-            u[i] = g.s == g.s ? static_cast<uint32_t>(over ? q + (rest > 0.f ? 1 : -1) : q) : 0u;
-        } else {
-            float t = __fmul_rn(v, g.r);
-            if (g.rare) t = fmaf(fmaf(-t, g.s, v), g.r, t);
-            u[i] = g.s == g.s ? __float_as_uint(__fadd_rn(t, kRint)) : 0u;
-        }
-    }
+    for (int i = 0; i < 8; ++i) u[i] = code1f<T>(f[i], g);
     return low_bytes(u);
 }
 

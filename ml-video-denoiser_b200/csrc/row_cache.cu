@@ -140,10 +140,13 @@ __global__ void __launch_bounds__(kThreads) write_vec_kernel(const WriteArgs a) 
     }
 }
 
-// Any size and alignment: a warp per group, two passes over it.
+// Any size and alignment: a warp per group, two passes over it, lanes along
+// the columns (a pair of them each, so that a byte of 4-bit codes is one
+// lane's). kKeep pairs a lane stay in registers between the passes.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) write_any_kernel(const WriteArgs a) {
     using Q = QuantOf<T>;
+    constexpr int kKeep = 8;
     pdl_trigger();
     pdl_wait();
     const int lane = threadIdx.x & 31;
@@ -154,28 +157,38 @@ __global__ void __launch_bounds__(kThreads) write_any_kernel(const WriteArgs a) 
     const int n = a.p.group;
     const T* src = static_cast<const T*>(a.p.x) + row * a.p.ldx + static_cast<int64_t>(grp) * n;
     const float qmax = a.p.bits == 8 ? 127.f : 7.f;
+    T keep[kKeep][2];
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i) {
+        const int c = lane * 2 + 64 * i;
+        keep[i][0] = c < n ? src[c] : T(0.f);
+        keep[i][1] = c + 1 < n ? src[c + 1] : T(0.f);
+    }
     uint32_t mag = 0;
-    for (int c = lane * 8; c < n; c += 256) mag = max(mag, Q::mag(Q::load_some(src + c, min(8, n - c))));
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i) mag = max(mag, max(Q::mag1(keep[i][0]), Q::mag1(keep[i][1])));
+    for (int c = lane * 2 + 64 * kKeep; c < n; c += 64) {
+        mag = max(mag, Q::mag1(src[c]));
+        if (c + 1 < n) mag = max(mag, Q::mag1(src[c + 1]));
+    }
     mag = __reduce_max_sync(0xffffffffu, mag);
     const GroupScale g = group_scale<T>(mag, qmax);
-    const bool rare = g.rare;  // the same on every lane
     const int64_t slot = slot_of(a, row);
     if (!wins<32>(a, row, grp, slot, true)) return;
     uint8_t* dst = a.p.codes + slot * a.p.ldc + static_cast<int64_t>(grp) * n * a.p.bits / 8;
-    for (int c = lane * 8; c < n; c += 256) {
-        const int m = min(8, n - c);
-        const uint2 w = codes8<T>(Q::load_some(src + c, m), g, rare);
-        if (a.p.bits == 8) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < m) dst[c + i] = static_cast<uint8_t>((i < 4 ? w.x : w.y) >> ((i & 3) * 8));
+    auto put = [&](int c, T x0, T x1) {
+        const uint32_t q0 = code1<T>(x0, g), q1 = code1<T>(x1, g);
+        if (a.p.bits == 4) {
+            dst[c / 2] = static_cast<uint8_t>((q0 & 15u) | (q1 << 4));
         } else {
-            const uint32_t b = pack_nibbles(w);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (2 * i < m) dst[c / 2 + i] = static_cast<uint8_t>(b >> (i * 8));
+            dst[c] = static_cast<uint8_t>(q0);
+            if (c + 1 < n) dst[c + 1] = static_cast<uint8_t>(q1);
         }
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i)
+        if (lane * 2 + 64 * i < n) put(lane * 2 + 64 * i, keep[i][0], keep[i][1]);
+    for (int c = lane * 2 + 64 * kKeep; c < n; c += 64) put(c, src[c], c + 1 < n ? src[c + 1] : T(0.f));
     if (lane == 0) a.p.scales[slot * a.ngroups + grp] = g.s;
 }
 
