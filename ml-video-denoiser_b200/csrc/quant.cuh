@@ -121,7 +121,7 @@ __device__ __forceinline__ GroupScale group_scale(uint32_t mag, float qmax) {
     g.s = fmaxf(__fmul_rn(a, qmax == 127.f ? 1.f / 127.f : 1.f / 7.f), kTinyScale);
     g.r = reciprocal(g.s);
     if (QuantOf<T>::kF32) {
-        g.rare = true;
+        g.rare = !(a <= 3.402823466e38f);
     } else {
         const float d = fmaf(g.s, qmax, -a);  // exact sign of s - a / qmax
         g.r *= d > 0.f ? 1.f - 4.76837158e-7f : 1.f + 4.76837158e-7f;
@@ -187,15 +187,38 @@ __device__ __forceinline__ uint2 codes8_rare(const typename QuantOf<T>::Vec& x, 
     return low_bytes(u);
 }
 
+// Codes of 8 FP32 values of a finite group: q0 of each, unless a value lies
+// within 2^-14 of a border between two codes (in units of s), where q0 may be
+// off by one.
+__device__ __forceinline__ uint2 codes8_fast(const QuantOf<float>::Vec& x, const GroupScale& g) {
+    float f[8];
+    QuantOf<float>::unpack(x, f);
+    const float2 r2 = make_float2(g.r, g.r), ns2 = make_float2(-g.s, -g.s), one2 = make_float2(1.f, 1.f);
+    const float2 magic2 = make_float2(kRint, kRint), nmagic2 = make_float2(-kRint, -kRint);
+    uint32_t u[8];
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 v = make_float2(f[2 * i], f[2 * i + 1]);
+        const float2 t = ffma2(v, r2, magic2);
+        const float2 rest = ffma2(ffma2(t, one2, nmagic2), ns2, v);
+        most = fmaxf(most, fmaxf(fabsf(rest.x), fabsf(rest.y)));
+        u[2 * i] = __float_as_uint(t.x);
+        u[2 * i + 1] = __float_as_uint(t.y);
+    }
+    if (most >= g.s * (0.5f - 6.10351562e-5f)) return codes8_rare<float>(x, g);
+    return low_bytes(u);
+}
+
 // Codes of 8 values; `rare`: whether a lane of the warp has a rare group
-// (warp-uniform; always for FP32).
+// (warp-uniform).
 template <typename T>
 __device__ __forceinline__ uint2 codes8(const typename QuantOf<T>::Vec& x, const GroupScale& g, bool rare) {
-    if constexpr (QuantOf<T>::kF32) {
-        return codes8_rare<T>(x, g);
-    } else {
-        return rare ? codes8_rare<T>(x, g) : codes8_fast(x, g.r);
-    }
+    if (rare) return codes8_rare<T>(x, g);
+    if constexpr (QuantOf<T>::kF32)
+        return codes8_fast(x, g);
+    else
+        return codes8_fast(x, g.r);
 }
 
 // 8 byte codes -> 8 nibbles (the even one in the low half of each byte).

@@ -44,25 +44,28 @@ struct WriteArgs {
     int order;
 };
 
-__device__ __forceinline__ int64_t slot_of(const WriteArgs& a, int64_t row) {
+// A launch has fewer than 2^30 groups, so rows and groups are counted in 32
+// bits; addresses in 64.
+__device__ __forceinline__ int64_t slot_of(const WriteArgs& a, int row) {
     return a.p.slots ? a.p.slots[row] : a.p.row0 + row;
 }
 
 // Whether group g of `row` is written; reports a slot behind the cache.
 // Warp-wide call; the SG lanes of a sub-warp pass the same row.
 template <int SG>
-__device__ __forceinline__ bool wins(const WriteArgs& a, int64_t row, int g, int64_t slot, bool live) {
+__device__ __forceinline__ bool wins(const WriteArgs& a, int row, int g, int64_t slot, bool live) {
+    if (!a.p.slots) return live;
     if (live && slot >= a.p.capacity) report_error(a.p.err, kSiteWrite, kErrBadShape);
     live = live && slot >= 0 && slot < a.p.capacity;
     if (a.order == kOrderScan) {
         const int lane = threadIdx.x & 31;
         bool later = false;
-        for (int64_t j = lane % SG; j < a.p.rows; j += SG) later = later || (j > row && a.p.slots[j] == slot);
+        for (int j = lane % SG; j < static_cast<int>(a.p.rows); j += SG) later = later || (j > row && a.p.slots[j] == slot);
         const uint32_t hit = __ballot_sync(0xffffffffu, later);
         const uint32_t mine = SG == 32 ? 0xffffffffu : ((1u << (SG & 31)) - 1u) << (lane / SG * SG);
         live = live && !(hit & mine);
     } else if (a.order == kOrderMark && live) {
-        live = __ldcg(reinterpret_cast<const int*>(a.p.scales + slot * a.ngroups + g)) == static_cast<int>(row);
+        live = __ldcg(reinterpret_cast<const int*>(a.p.scales + slot * a.ngroups + g)) == row;
     }
     __syncwarp();  // every lane has read the mark before one of them writes the scale over it
     return live;
@@ -83,29 +86,28 @@ __global__ void __launch_bounds__(kThreads) mark_kernel(const WriteArgs a, int p
         atomicMax(m, static_cast<int>(row));
 }
 
-template <typename T, int SG, int V, int U>
+template <typename T, int BITS, int SG, int V, int U>
 __global__ void __launch_bounds__(kThreads) write_vec_kernel(const WriteArgs a) {
     using Q = QuantOf<T>;
     pdl_trigger();
     pdl_wait();
     constexpr int kPer = 32 / SG;  // groups of a warp at a time
+    constexpr float qmax = BITS == 8 ? 127.f : 7.f;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int sub = lane / SG, l = lane % SG;
     const int nv = a.p.group / 8;
-    const int64_t units = a.p.rows * a.ngroups;
-    const int64_t u0 = (static_cast<int64_t>(blockIdx.x) * kWarps + warp) * (kPer * U);
+    const int units = static_cast<int>(a.p.rows) * a.ngroups;
+    const int u0 = (blockIdx.x * kWarps + warp) * (kPer * U);
     if (u0 >= units) return;
-    const float qmax = a.p.bits == 8 ? 127.f : 7.f;
     const T* x = static_cast<const T*>(a.p.x);
     typename Q::Vec v[U][V];
-    int64_t row[U];
-    int grp[U];
+    int row[U], grp[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-        const int64_t u = u0 + i * kPer + sub;
-        row[i] = a.ngroups == 1 ? u : u / a.ngroups;
-        grp[i] = a.ngroups == 1 ? 0 : static_cast<int>(u - row[i] * a.ngroups);
-        const T* src = x + row[i] * a.p.ldx + static_cast<int64_t>(grp[i]) * a.p.group;
+        const int u = u0 + i * kPer + sub;
+        row[i] = a.ngroups == 1 ? u : static_cast<int>(static_cast<uint32_t>(u) / static_cast<uint32_t>(a.ngroups));
+        grp[i] = a.ngroups == 1 ? 0 : u - row[i] * a.ngroups;
+        const T* src = x + row[i] * a.p.ldx + grp[i] * a.p.group;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             const int c = l + k * SG;
@@ -124,13 +126,13 @@ __global__ void __launch_bounds__(kThreads) write_vec_kernel(const WriteArgs a) 
         const bool rare = __any_sync(0xffffffffu, g.rare);
         const int64_t slot = there ? slot_of(a, row[i]) : -1;
         if (!wins<SG>(a, row[i], grp[i], slot, there)) continue;
-        uint8_t* dst = a.p.codes + slot * a.p.ldc + static_cast<int64_t>(grp[i]) * a.p.group * a.p.bits / 8;
+        uint8_t* dst = a.p.codes + slot * a.p.ldc + static_cast<int64_t>(grp[i]) * (a.p.group * BITS / 8);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             const int c = l + k * SG;
             if (c < nv) {
                 const uint2 w = codes8<T>(v[i][k], g, rare);
-                if (a.p.bits == 8)
+                if (BITS == 8)
                     *reinterpret_cast<uint2*>(dst + c * 8) = w;
                 else
                     *reinterpret_cast<uint32_t*>(dst + c * 4) = pack_nibbles(w);
@@ -140,56 +142,68 @@ __global__ void __launch_bounds__(kThreads) write_vec_kernel(const WriteArgs a) 
     }
 }
 
-// Any size and alignment: a warp per group, two passes over it, lanes along
-// the columns (a pair of them each, so that a byte of 4-bit codes is one
-// lane's). kKeep pairs a lane stay in registers between the passes.
-template <typename T>
+// Any size and alignment: a warp takes U groups, lanes along the columns (a
+// pair of them each, so that a byte of 4-bit codes is one lane's). KEEP pairs a
+// lane stay in registers; what a group has more is read twice.
+template <typename T, int KEEP, int U>
 __global__ void __launch_bounds__(kThreads) write_any_kernel(const WriteArgs a) {
     using Q = QuantOf<T>;
-    constexpr int kKeep = 8;
     pdl_trigger();
     pdl_wait();
     const int lane = threadIdx.x & 31;
-    const int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-    if (u >= a.p.rows * a.ngroups) return;
-    const int64_t row = u / a.ngroups;
-    const int grp = static_cast<int>(u - row * a.ngroups);
+    const int units = static_cast<int>(a.p.rows) * a.ngroups;
+    const int u0 = (blockIdx.x * kWarps + (threadIdx.x >> 5)) * U;
     const int n = a.p.group;
-    const T* src = static_cast<const T*>(a.p.x) + row * a.p.ldx + static_cast<int64_t>(grp) * n;
     const float qmax = a.p.bits == 8 ? 127.f : 7.f;
-    T keep[kKeep][2];
-#pragma unroll
-    for (int i = 0; i < kKeep; ++i) {
-        const int c = lane * 2 + 64 * i;
-        keep[i][0] = c < n ? src[c] : T(0.f);
-        keep[i][1] = c + 1 < n ? src[c + 1] : T(0.f);
-    }
-    uint32_t mag = 0;
-#pragma unroll
-    for (int i = 0; i < kKeep; ++i) mag = max(mag, max(Q::mag1(keep[i][0]), Q::mag1(keep[i][1])));
-    for (int c = lane * 2 + 64 * kKeep; c < n; c += 64) {
-        mag = max(mag, Q::mag1(src[c]));
-        if (c + 1 < n) mag = max(mag, Q::mag1(src[c + 1]));
-    }
-    mag = __reduce_max_sync(0xffffffffu, mag);
-    const GroupScale g = group_scale<T>(mag, qmax);
-    const int64_t slot = slot_of(a, row);
-    if (!wins<32>(a, row, grp, slot, true)) return;
-    uint8_t* dst = a.p.codes + slot * a.p.ldc + static_cast<int64_t>(grp) * n * a.p.bits / 8;
-    auto put = [&](int c, T x0, T x1) {
-        const uint32_t q0 = code1<T>(x0, g), q1 = code1<T>(x1, g);
-        if (a.p.bits == 4) {
-            dst[c / 2] = static_cast<uint8_t>((q0 & 15u) | (q1 << 4));
-        } else {
-            dst[c] = static_cast<uint8_t>(q0);
-            if (c + 1 < n) dst[c + 1] = static_cast<uint8_t>(q1);
-        }
+    T keep[U][KEEP][2];
+    auto place = [&](int u, int& row, int& grp) {
+        row = static_cast<int>(static_cast<uint32_t>(u) / static_cast<uint32_t>(a.ngroups));
+        grp = u - row * a.ngroups;
+        return static_cast<const T*>(a.p.x) + row * a.p.ldx + static_cast<int64_t>(grp) * n;
     };
 #pragma unroll
-    for (int i = 0; i < kKeep; ++i)
-        if (lane * 2 + 64 * i < n) put(lane * 2 + 64 * i, keep[i][0], keep[i][1]);
-    for (int c = lane * 2 + 64 * kKeep; c < n; c += 64) put(c, src[c], c + 1 < n ? src[c + 1] : T(0.f));
-    if (lane == 0) a.p.scales[slot * a.ngroups + grp] = g.s;
+    for (int j = 0; j < U; ++j) {
+        int row, grp;
+        const T* src = place(min(u0 + j, units - 1), row, grp);
+#pragma unroll
+        for (int i = 0; i < KEEP; ++i) {
+            const int c = lane * 2 + 64 * i;
+            keep[j][i][0] = c < n ? src[c] : T(0.f);
+            keep[j][i][1] = c + 1 < n ? src[c + 1] : T(0.f);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+        if (u0 + j >= units) break;
+        int row, grp;
+        const T* src = place(u0 + j, row, grp);
+        uint32_t mag = 0;
+#pragma unroll
+        for (int i = 0; i < KEEP; ++i) mag = max(mag, max(Q::mag1(keep[j][i][0]), Q::mag1(keep[j][i][1])));
+        for (int c = lane * 2 + 64 * KEEP; c < n; c += 64) {
+            mag = max(mag, Q::mag1(src[c]));
+            if (c + 1 < n) mag = max(mag, Q::mag1(src[c + 1]));
+        }
+        mag = __reduce_max_sync(0xffffffffu, mag);
+        const GroupScale g = group_scale<T>(mag, qmax);
+        const int64_t slot = slot_of(a, row);
+        if (!wins<32>(a, row, grp, slot, true)) continue;
+        uint8_t* dst = a.p.codes + slot * a.p.ldc + static_cast<int64_t>(grp) * n * a.p.bits / 8;
+        auto put = [&](int c, T x0, T x1) {
+            const uint32_t q0 = code1<T>(x0, g), q1 = code1<T>(x1, g);
+            if (a.p.bits == 4) {
+                dst[c / 2] = static_cast<uint8_t>((q0 & 15u) | (q1 << 4));
+            } else {
+                dst[c] = static_cast<uint8_t>(q0);
+                if (c + 1 < n) dst[c + 1] = static_cast<uint8_t>(q1);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < KEEP; ++i)
+            if (lane * 2 + 64 * i < n) put(lane * 2 + 64 * i, keep[j][i][0], keep[j][i][1]);
+        for (int c = lane * 2 + 64 * KEEP; c < n; c += 64) put(c, src[c], c + 1 < n ? src[c + 1] : T(0.f));
+        if (lane == 0) a.p.scales[slot * a.ngroups + grp] = g.s;
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -300,26 +314,37 @@ __global__ void __launch_bounds__(kThreads) read_vec_kernel(const ReadArgs a) {
     }
 }
 
-// Any size and alignment: a warp per row.
-template <typename T>
+// Any size and alignment: a warp takes U rows, lanes along the columns.
+template <typename T, int BITS, int U>
 __global__ void __launch_bounds__(kThreads) read_any_kernel(const ReadArgs a) {
     pdl_trigger();
     pdl_wait();
     const int lane = threadIdx.x & 31;
     const int b = blockIdx.y;
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-    const int64_t src = source_row(a, b, i, sequence_rows(a, b));
-    if (src < 0) return;
-    const uint8_t* p = a.codes + src * a.ldc;
-    const float* sc = a.scales + src * a.ngroups;
-    T* out = static_cast<T*>(a.out) + b * a.out_batch + i * a.ldo;
+    const int64_t n = sequence_rows(a, b);
+    const int64_t i0 = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * U;
+    if (i0 >= n) return;
+    int64_t src[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) src[k] = source_row(a, b, i0 + k, n);
+    T* out = static_cast<T*>(a.out) + b * a.out_batch + i0 * a.ldo;
     for (int c = lane; c < a.cols; c += 32) {
-        int q;
-        if (a.bits == 8)
-            q = static_cast<int8_t>(p[c]);
-        else
-            q = static_cast<int>((p[c >> 1] >> ((c & 1) * 4)) & 15u) - ((p[c >> 1] >> ((c & 1) * 4)) & 8u ? 16 : 0);
-        store1(out + c, static_cast<float>(q) * sc[a.ngroups == 1 ? 0 : c / a.group]);
+        const int g = a.ngroups == 1 ? 0 : c / a.group;
+        int q[U];
+        float s[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            if (src[k] < 0) continue;
+            const uint8_t* p = a.codes + src[k] * a.ldc;
+            q[k] = BITS == 8 ? static_cast<int>(static_cast<int8_t>(p[c])) : static_cast<int>(p[c >> 1]);
+            s[k] = a.scales[src[k] * a.ngroups + g];
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            if (src[k] < 0) continue;
+            if (BITS == 4) q[k] = static_cast<int>(static_cast<uint32_t>(q[k]) << (c & 1 ? 24 : 28)) >> 28;  // the signed nibble
+            store1(out + k * a.ldo + c, static_cast<float>(q[k]) * s[k]);
+        }
     }
 }
 
@@ -331,38 +356,49 @@ int pow2_lanes(int nv) {
     return s;
 }
 
-template <typename T, int SG, int V, int U>
+template <typename T, int BITS, int SG, int V, int U>
 cudaError_t write_run(const WriteArgs& a, cudaStream_t s) {
     const int64_t per = static_cast<int64_t>(kWarps) * (32 / SG) * U;
     const int64_t units = a.p.rows * a.ngroups;
-    return launch_pdl(write_vec_kernel<T, SG, V, U>, dim3(static_cast<unsigned>((units + per - 1) / per)), dim3(kThreads),
-                      0, s, a);
+    return launch_pdl(write_vec_kernel<T, BITS, SG, V, U>, dim3(static_cast<unsigned>((units + per - 1) / per)),
+                      dim3(kThreads), 0, s, a);
+}
+
+template <typename T, int KEEP, int U>
+cudaError_t write_any(const WriteArgs& a, cudaStream_t s) {
+    const int64_t units = a.p.rows * a.ngroups, per = static_cast<int64_t>(kWarps) * U;
+    return launch_pdl(write_any_kernel<T, KEEP, U>, dim3(static_cast<unsigned>((units + per - 1) / per)), dim3(kThreads), 0,
+                      s, a);
+}
+
+template <typename T, int BITS>
+cudaError_t write_bits(const WriteArgs& a, cudaStream_t s) {
+    const int nv = a.p.group / 8;
+    switch (pow2_lanes(nv)) {
+        case 1: return write_run<T, BITS, 1, 1, 4>(a, s);
+        case 2: return write_run<T, BITS, 2, 1, 4>(a, s);
+        case 4: return write_run<T, BITS, 4, 1, 4>(a, s);
+        case 8: return write_run<T, BITS, 8, 1, 4>(a, s);
+        case 16: return write_run<T, BITS, 16, 1, 4>(a, s);
+        default: break;
+    }
+    if (nv <= 32) return write_run<T, BITS, 32, 1, 4>(a, s);
+    if (nv <= 64) return write_run<T, BITS, 32, 2, 2>(a, s);
+    if (nv <= 128) return write_run<T, BITS, 32, 4, 1>(a, s);
+    return write_run<T, BITS, 32, 8, 1>(a, s);
 }
 
 template <typename T>
 cudaError_t write_type(const WriteArgs& a, cudaStream_t s) {
     const CacheWrite& p = a.p;
-    const int nv = p.group / 8;
     // A vector of 8 codes has `bits` bytes.
-    const bool vec = p.group % 8 == 0 && nv <= 256 && aligned(p.x, 16) && p.ldx * sizeof(T) % 16 == 0 &&
+    const bool vec = p.group % 8 == 0 && p.group <= 2048 && aligned(p.x, 16) && p.ldx * sizeof(T) % 16 == 0 &&
                      aligned(p.codes, p.bits) && p.ldc % p.bits == 0;
-    if (!vec) {
-        const int64_t units = p.rows * a.ngroups;
-        return launch_pdl(write_any_kernel<T>, dim3(static_cast<unsigned>((units + kWarps - 1) / kWarps)),
-                          dim3(kThreads), 0, s, a);
-    }
-    switch (pow2_lanes(nv)) {
-        case 1: return write_run<T, 1, 1, 4>(a, s);
-        case 2: return write_run<T, 2, 1, 4>(a, s);
-        case 4: return write_run<T, 4, 1, 4>(a, s);
-        case 8: return write_run<T, 8, 1, 4>(a, s);
-        case 16: return write_run<T, 16, 1, 4>(a, s);
-        default: break;
-    }
-    if (nv <= 32) return write_run<T, 32, 1, 4>(a, s);
-    if (nv <= 64) return write_run<T, 32, 2, 2>(a, s);
-    if (nv <= 128) return write_run<T, 32, 4, 1>(a, s);
-    return write_run<T, 32, 8, 1>(a, s);
+    if (vec) return p.bits == 8 ? write_bits<T, 8>(a, s) : write_bits<T, 4>(a, s);
+    // 8 pairs a lane in registers: groups of one row, or pieces of several.
+    if (p.group <= 64) return write_any<T, 1, 8>(a, s);
+    if (p.group <= 256) return write_any<T, 4, 2>(a, s);
+    return write_any<T, 8, 1>(a, s);
 }
 
 template <typename T, int BITS, int SG, int U>
@@ -388,9 +424,12 @@ template <typename T>
 cudaError_t read_type(const ReadArgs& a, int batch, cudaStream_t s) {
     const bool vec = a.cols % 8 == 0 && a.group % 8 == 0 && aligned(a.codes, a.bits) && a.ldc % a.bits == 0 &&
                      aligned(a.out, 16) && a.ldo * sizeof(T) % 16 == 0 && a.out_batch * sizeof(T) % 16 == 0;
-    if (!vec)
-        return launch_pdl(read_any_kernel<T>, dim3(static_cast<unsigned>((a.rows + kWarps - 1) / kWarps), batch),
-                          dim3(kThreads), 0, s, a);
+    if (!vec) {
+        constexpr int kU = 8;
+        const dim3 grid(static_cast<unsigned>((a.rows + kWarps * kU - 1) / (kWarps * kU)), batch);
+        return a.bits == 8 ? launch_pdl(read_any_kernel<T, 8, kU>, grid, dim3(kThreads), 0, s, a)
+                           : launch_pdl(read_any_kernel<T, 4, kU>, grid, dim3(kThreads), 0, s, a);
+    }
     return a.bits == 8 ? read_bits<T, 8>(a, batch, s) : read_bits<T, 4>(a, batch, s);
 }
 
