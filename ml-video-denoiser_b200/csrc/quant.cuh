@@ -227,23 +227,27 @@ __device__ __forceinline__ uint32_t pack_nibbles(uint2 w) {
     return __byte_perm(a | (a >> 4), b | (b >> 4), 0x6420);
 }
 
-// Four signed byte codes as floats: the byte, biased to unsigned, becomes the
-// low mantissa byte of 2^23 + (q + 128).
-__device__ __forceinline__ void bytes_to_f(uint32_t w, float (&f)[4]) {
+// Signed byte codes as floats, four at a time: the byte, biased to unsigned,
+// becomes the low mantissa byte of 2^23 + (q + 128).
+__device__ __forceinline__ void bytes_to_f(uint32_t w, float2 (&f)[2]) {
     const uint32_t b = w ^ 0x80808080u;
+    const float2 one2 = make_float2(1.f, 1.f), bias2 = make_float2(-8388736.f, -8388736.f);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        f[i] = __uint_as_float(__byte_perm(b, 0x4b000000u, 0x7440 | i)) - 8388736.f;
+    for (int i = 0; i < 2; ++i)
+        f[i] = ffma2(make_float2(__uint_as_float(__byte_perm(b, 0x4b000000u, 0x7440 | (2 * i))),
+                                 __uint_as_float(__byte_perm(b, 0x4b000000u, 0x7440 | (2 * i + 1)))),
+                     one2, bias2);
 }
 
 // Eight nibble codes as floats, in order.
-__device__ __forceinline__ void nibbles_to_f(uint32_t w, float (&f)[8]) {
+__device__ __forceinline__ void nibbles_to_f(uint32_t w, float2 (&f)[4]) {
     const uint32_t lo = (w & 0x0f0f0f0fu) ^ 0x08080808u, hi = ((w >> 4) & 0x0f0f0f0fu) ^ 0x08080808u;
+    const float2 one2 = make_float2(1.f, 1.f), bias2 = make_float2(-8388616.f, -8388616.f);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        f[2 * i] = __uint_as_float(__byte_perm(lo, 0x4b000000u, 0x7440 | i)) - 8388616.f;
-        f[2 * i + 1] = __uint_as_float(__byte_perm(hi, 0x4b000000u, 0x7440 | i)) - 8388616.f;
-    }
+    for (int i = 0; i < 4; ++i)
+        f[i] = ffma2(make_float2(__uint_as_float(__byte_perm(lo, 0x4b000000u, 0x7440 | i)),
+                                 __uint_as_float(__byte_perm(hi, 0x4b000000u, 0x7440 | i))),
+                     one2, bias2);
 }
 
 }  // namespace dnb

@@ -220,7 +220,7 @@ struct ReadArgs {
     int64_t row0;
     const int32_t* table;  // read_pages (else null)
     int64_t table_ld;
-    uint32_t page_rows;
+    uint32_t page_rows, page_mul, page_shift;  // i / page_rows = (umulhi(i, page_mul) + i) >> page_shift for i < 2^31
     const int32_t* lengths;
     int64_t rows;          // rows of out a sequence may fill
     void* out;
@@ -229,14 +229,15 @@ struct ReadArgs {
 };
 
 // Cache row of out row i of sequence b, or -1. i < 2^31.
-__device__ __forceinline__ int64_t source_row(const ReadArgs& a, int b, int64_t i, int64_t n) {
-    if (i >= n) return -1;
+__device__ __forceinline__ int64_t source_row(const ReadArgs& a, int b, int64_t i64, int64_t n) {
+    if (i64 >= n) return -1;
+    const uint32_t i = static_cast<uint32_t>(i64);
     int64_t r;
     if (a.table) {
-        const uint32_t q = static_cast<uint32_t>(i) / a.page_rows;
-        const int32_t page = a.table[b * a.table_ld + q];
+        const uint32_t q = (__umulhi(i, a.page_mul) + i) >> a.page_shift;
+        const int32_t page = __ldg(a.table + b * a.table_ld + q);
         if (page < 0) return -1;
-        r = static_cast<int64_t>(page) * a.page_rows + (static_cast<uint32_t>(i) - q * a.page_rows);
+        r = static_cast<int64_t>(page) * a.page_rows + (i - q * a.page_rows);
     } else {
         r = a.slots ? a.slots[i] : a.row0 + i;
         if (r < 0) return -1;
@@ -254,62 +255,76 @@ __device__ __forceinline__ int64_t sequence_rows(const ReadArgs& a, int b) {
     return n < 0 ? 0 : (n < a.rows ? n : a.rows);
 }
 
-__device__ __forceinline__ void store8(__half* p, const float (&f)[8]) { *reinterpret_cast<uint4*>(p) = f_to_h8(f); }
-__device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+__device__ __forceinline__ void store8(__half* p, const float2 (&f)[4]) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack_half2(f[0].x, f[0].y), pack_half2(f[1].x, f[1].y),
+                                              pack_half2(f[2].x, f[2].y), pack_half2(f[3].x, f[3].y));
+}
+__device__ __forceinline__ void store8(float* p, const float2 (&f)[4]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
+    reinterpret_cast<float4*>(p)[1] = make_float4(f[2].x, f[2].y, f[3].x, f[3].y);
 }
 __device__ __forceinline__ void store1(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 
-// SG lanes per row (a lane 8 columns at a time), U rows of each sub-warp in
-// flight.
-template <typename T, int BITS, int SG, int U>
+// SG lanes per row, a lane W = 8 or 16 columns at a time (of one group), U rows
+// of each sub-warp in flight. 16 columns halve the work per row, which bounds
+// narrow rows: READ16.
+template <typename T, int BITS, int SG, int U, int W>
 __global__ void __launch_bounds__(kThreads) read_vec_kernel(const ReadArgs a) {
     pdl_trigger();
     pdl_wait();
     constexpr int kPer = 32 / SG;
+    constexpr int kWords = W * BITS / 32;
     const int lane = threadIdx.x & 31;
     const int sub = lane / SG, l = lane % SG;
     const int b = blockIdx.y;
     const int64_t n = sequence_rows(a, b);
     const int64_t i0 = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * (kPer * U) + sub;
     if (i0 - sub >= n) return;
-    const int nv = a.cols / 8;
+    const int nv = a.cols / W;
     int64_t src[U];
 #pragma unroll
     for (int k = 0; k < U; ++k) src[k] = source_row(a, b, i0 + k * kPer, n);
-    T* out = static_cast<T*>(a.out) + b * a.out_batch;
+    T* out = static_cast<T*>(a.out) + b * a.out_batch + i0 * a.ldo;
     for (int c = l; c < nv; c += SG) {
-        uint2 w[U];
+        uint32_t w[U][kWords];
         float s[U];
-        const int g = a.ngroups == 1 ? 0 : c * 8 / a.group;
+        const int g = a.ngroups == 1 ? 0 : c * W / a.group;
 #pragma unroll
         for (int k = 0; k < U; ++k) {
             if (src[k] < 0) continue;
-            const uint8_t* p = a.codes + src[k] * a.ldc;
-            if (BITS == 8)
-                w[k] = *reinterpret_cast<const uint2*>(p + c * 8);
-            else
-                w[k].x = *reinterpret_cast<const uint32_t*>(p + c * 4);
+            const uint8_t* p = a.codes + src[k] * a.ldc + c * (W * BITS / 8);
+            if constexpr (kWords == 4) {
+                const uint4 v = *reinterpret_cast<const uint4*>(p);
+                w[k][0] = v.x, w[k][1] = v.y, w[k][2] = v.z, w[k][3] = v.w;
+            } else if constexpr (kWords == 2) {
+                const uint2 v = *reinterpret_cast<const uint2*>(p);
+                w[k][0] = v.x, w[k][1] = v.y;
+            } else {
+                w[k][0] = *reinterpret_cast<const uint32_t*>(p);
+            }
             s[k] = a.scales[src[k] * a.ngroups + g];
         }
 #pragma unroll
         for (int k = 0; k < U; ++k) {
             if (src[k] < 0) continue;
-            float f[8];
-            if (BITS == 8) {
-                float lo[4], hi[4];
-                bytes_to_f(w[k].x, lo);
-                bytes_to_f(w[k].y, hi);
+            const float2 s2 = make_float2(s[k], s[k]), zero2 = make_float2(0.f, 0.f);
+            T* o = out + k * kPer * a.ldo + c * W;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) f[i] = lo[i], f[i + 4] = hi[i];
-            } else {
-                nibbles_to_f(w[k].x, f);
+            for (int h = 0; h < W / 8; ++h) {
+                float2 f[4];
+                if constexpr (BITS == 8) {
+                    float2 lo[2], hi[2];
+                    bytes_to_f(w[k][2 * h], lo);
+                    bytes_to_f(w[k][2 * h + 1], hi);
+                    f[0] = lo[0], f[1] = lo[1], f[2] = hi[0], f[3] = hi[1];
+                } else {
+                    nibbles_to_f(w[k][h], f);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[i] = ffma2(f[i], s2, zero2);
+                store8(o + h * 8, f);
             }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] *= s[k];
-            store8(out + (i0 + k * kPer) * a.ldo + c * 8, f);
         }
     }
 }
@@ -401,23 +416,29 @@ cudaError_t write_type(const WriteArgs& a, cudaStream_t s) {
     return write_any<T, 8, 1>(a, s);
 }
 
-template <typename T, int BITS, int SG, int U>
+template <typename T, int BITS, int SG, int U, int W>
 cudaError_t read_run(const ReadArgs& a, int batch, cudaStream_t s) {
     const int64_t per = static_cast<int64_t>(kWarps) * (32 / SG) * U;
-    return launch_pdl(read_vec_kernel<T, BITS, SG, U>, dim3(static_cast<unsigned>((a.rows + per - 1) / per), batch),
+    return launch_pdl(read_vec_kernel<T, BITS, SG, U, W>, dim3(static_cast<unsigned>((a.rows + per - 1) / per), batch),
                       dim3(kThreads), 0, s, a);
+}
+
+template <typename T, int BITS, int W>
+cudaError_t read_width(const ReadArgs& a, int batch, cudaStream_t s) {
+    switch (pow2_lanes(a.cols / W)) {
+        case 1: return read_run<T, BITS, 1, 4, W>(a, batch, s);
+        case 2: return read_run<T, BITS, 2, 4, W>(a, batch, s);
+        case 4: return read_run<T, BITS, 4, 4, W>(a, batch, s);
+        case 8: return read_run<T, BITS, 8, 4, W>(a, batch, s);
+        case 16: return read_run<T, BITS, 16, 4, W>(a, batch, s);
+        default: return read_run<T, BITS, 32, 4, W>(a, batch, s);
+    }
 }
 
 template <typename T, int BITS>
 cudaError_t read_bits(const ReadArgs& a, int batch, cudaStream_t s) {
-    switch (pow2_lanes(a.cols / 8)) {
-        case 1: return read_run<T, BITS, 1, 4>(a, batch, s);
-        case 2: return read_run<T, BITS, 2, 4>(a, batch, s);
-        case 4: return read_run<T, BITS, 4, 4>(a, batch, s);
-        case 8: return read_run<T, BITS, 8, 4>(a, batch, s);
-        case 16: return read_run<T, BITS, 16, 4>(a, batch, s);
-        default: return read_run<T, BITS, 32, 4>(a, batch, s);
-    }
+    const bool wide = a.cols % 16 == 0 && a.group % 16 == 0 && aligned(a.codes, 2 * BITS) && a.ldc % (2 * BITS) == 0;
+    return wide ? read_width<T, BITS, 16>(a, batch, s) : read_width<T, BITS, 8>(a, batch, s);
 }
 
 template <typename T>
@@ -571,6 +592,9 @@ int dn_launch_cache_read_pages(const void* codes, int64_t ld_codes, const float*
     a.table = table;
     a.table_ld = table_ld;
     a.page_rows = static_cast<uint32_t>(page_rows);
+    while ((1LL << a.page_shift) < page_rows) ++a.page_shift;
+    a.page_mul = static_cast<uint32_t>((((1ULL << a.page_shift) - static_cast<uint64_t>(page_rows)) << 32) /
+                                           static_cast<uint64_t>(page_rows) + 1);
     a.lengths = lengths;
     a.rows = rows;
     a.out = out;
