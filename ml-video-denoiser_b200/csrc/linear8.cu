@@ -23,57 +23,101 @@ namespace {
 constexpr int kMaxK = 131072;  // 127 * 127 * 131072 < 2^31
 
 // Codes and scales of the pixels of NCHW planes (layers too wide for one pass):
-// a CTA of eight warps takes 32 pixels, a lane one of them and a warp 32
-// channels at a time, so that the loads of 32 channels are in flight and a
-// lane's codes are a whole 32-byte sector. Two passes over the planes; the
-// second finds them in L1 or L2.
+// a CTA of eight warps takes 32 PX pixels, a lane PX adjacent ones of them
+// (two where pairs are 4-byte aligned) and a warp 32 channels at a time, so
+// that the loads of 32 channels are in flight and a lane's codes are a whole
+// 32-byte sector. A warp's first run of channels stays in registers between the
+// two passes, the others are read again out of L1 or L2 (four runs in registers
+// cost more in occupancy than they save).
+template <int PX>
 __global__ void __launch_bounds__(256) quantise_planes_kernel(const __half* __restrict__ x, int64_t rows, int K, int64_t hw,
                                                               uint8_t* __restrict__ codes, int64_t ldc,
                                                               float* __restrict__ scales) {
     using Q = QuantOf<__half>;
-    __shared__ uint32_t s_mag[32];
+    __shared__ uint32_t s_mag[32 * PX];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (threadIdx.x < 32) s_mag[threadIdx.x] = 0;
+    if (threadIdx.x < 32 * PX) s_mag[threadIdx.x] = 0;
     __syncthreads();
     pdl_trigger();
     pdl_wait();
-    const int64_t m = static_cast<int64_t>(blockIdx.x) * 32 + lane;
-    const bool live = m < rows;
+    const int64_t m = (static_cast<int64_t>(blockIdx.x) * 32 + lane) * PX;
+    const bool live = m < rows;  // PX == 2: the planes' pixels are even in number
     const int64_t img = live ? m / hw : 0;
     const __half* src = x + img * K * hw + (live ? m - img * hw : 0);
-    auto load = [&](int k0, Q::Vec (&v)[4]) {
-        uint32_t w[16];
+    auto load = [&](int k0, Q::Vec (&v)[PX][4]) {
+        uint32_t w[PX][16];
         const __half* p = src + k0 * hw;
 #pragma unroll
-        for (int i = 0; i < 32; ++i, p += hw) {
-            const uint32_t h = live && k0 + i < K ? __half_as_ushort(__ldg(p)) : 0u;
-            w[i >> 1] = i & 1 ? w[i >> 1] | (h << 16) : h;
+        for (int i = 0; i < 32; i += 2, p += 2 * hw) {
+            if constexpr (PX == 2) {
+                const uint32_t a = live && k0 + i < K ? __ldg(reinterpret_cast<const uint32_t*>(p)) : 0u;
+                const uint32_t b = live && k0 + i + 1 < K ? __ldg(reinterpret_cast<const uint32_t*>(p + hw)) : 0u;
+                w[0][i >> 1] = __byte_perm(a, b, 0x5410);
+                w[1][i >> 1] = __byte_perm(a, b, 0x7632);
+            } else {
+                const uint32_t a = live && k0 + i < K ? __half_as_ushort(__ldg(p)) : 0u;
+                const uint32_t b = live && k0 + i + 1 < K ? __half_as_ushort(__ldg(p + hw)) : 0u;
+                w[0][i >> 1] = a | (b << 16);
+            }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i].v = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        for (int q = 0; q < PX; ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[q][i].v = make_uint4(w[q][4 * i], w[q][4 * i + 1], w[q][4 * i + 2], w[q][4 * i + 3]);
     };
-    uint32_t mag = 0;
-    for (int k0 = warp * 32; k0 < K; k0 += 256) {
-        Q::Vec v[4];
-        load(k0, v);
+    uint32_t mag[PX] = {};
+    auto largest = [&](const Q::Vec (&v)[PX][4]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mag = max(mag, Q::mag(v[i]));
+        for (int q = 0; q < PX; ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mag[q] = max(mag[q], Q::mag(v[q][i]));
+    };
+    Q::Vec keep[PX][4];
+    load(warp * 32, keep);
+    largest(keep);
+    for (int k0 = warp * 32 + 256; k0 < K; k0 += 256) {
+        Q::Vec v[PX][4];
+        load(k0, v);
+        largest(v);
     }
-    atomicMax(&s_mag[lane], mag);
+#pragma unroll
+    for (int q = 0; q < PX; ++q) atomicMax(&s_mag[lane * PX + q], mag[q]);
     __syncthreads();
-    const GroupScale g = group_scale<__half>(s_mag[lane], 127.f);
-    const bool rare = __any_sync(0xffffffffu, g.rare);
-    for (int k0 = warp * 32; k0 < K; k0 += 256) {
-        Q::Vec v[4];
-        load(k0, v);
-        uint8_t* dst = codes + m * ldc + k0;
+    GroupScale g[PX];
+    bool rare = false;
 #pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-            const uint2 lo = codes8<__half>(v[i], g, rare), hi = codes8<__half>(v[i + 1], g, rare);
-            if (live && k0 + i * 8 < ldc) *reinterpret_cast<uint4*>(dst + i * 8) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-        }
+    for (int q = 0; q < PX; ++q) {
+        g[q] = group_scale<__half>(s_mag[lane * PX + q], 127.f);
+        rare = rare || g[q].rare;
     }
-    if (warp == 0 && live) scales[m] = g.s;
+    rare = __any_sync(0xffffffffu, rare);
+    auto store = [&](int k0, const Q::Vec (&v)[PX][4]) {
+#pragma unroll
+        for (int q = 0; q < PX; ++q) {
+            uint8_t* dst = codes + (m + q) * ldc + k0;
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                const uint2 lo = codes8<__half>(v[q][i], g[q], rare), hi = codes8<__half>(v[q][i + 1], g[q], rare);
+                if (live && k0 + i * 8 < ldc) *reinterpret_cast<uint4*>(dst + i * 8) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            }
+        }
+    };
+    store(warp * 32, keep);
+    for (int k0 = warp * 32 + 256; k0 < K; k0 += 256) {
+        Q::Vec v[PX][4];
+        load(k0, v);
+        store(k0, v);
+    }
+    if (warp == 0 && live)
+#pragma unroll
+        for (int q = 0; q < PX; ++q) scales[m + q] = g[q].s;
+}
+
+template <int PX>
+cudaError_t quantise_planes(const void* x, int64_t rows, int K, int64_t hw, uint8_t* codes, int64_t ldc, float* scales,
+                            cudaStream_t s) {
+    return launch_pdl(quantise_planes_kernel<PX>, dim3(static_cast<unsigned>((rows + 32 * PX - 1) / (32 * PX))),
+                      dim3(256), 0, s, static_cast<const __half*>(x), rows, K, hw, codes, ldc, scales);
 }
 
 // par of ProductArgs from the weight rows' scales and the bias (may be null).
@@ -373,8 +417,9 @@ int dn_linear8_forward_nchw(dn_linear8* L, const void* input, int N, int H, int 
     a.lda = round16(L->cin);
     auto* codes = static_cast<uint8_t*>(workspace);
     auto* scales = reinterpret_cast<float*>(codes + rows * a.lda);
-    const cudaError_t e = launch_pdl(quantise_planes_kernel, dim3(static_cast<unsigned>((rows + 31) / 32)), dim3(256), 0, s,
-                                     static_cast<const __half*>(input), rows, L->cin, hw, codes, a.lda, scales);
+    const bool pairs = hw % 2 == 0 && aligned_to(input, 4);
+    const cudaError_t e = pairs ? quantise_planes<2>(input, rows, L->cin, hw, codes, a.lda, scales, s)
+                                : quantise_planes<1>(input, rows, L->cin, hw, codes, a.lda, scales, s);
     if (e != cudaSuccess) return dn_cuda_fail(e, "dn_linear8_forward_nchw: quantise launch");
     a.a = reinterpret_cast<const int8_t*>(codes);
     a.as = scales;

@@ -25,7 +25,10 @@ namespace {
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTokens = 8;
-constexpr int kMaxBytes = 64 * 1024;  // codes of all tokens in shared memory
+// Codes of all tokens in shared memory. Every CTA makes them all, which costs
+// more than the tensor-core path from there on (8 x 8000 -> 4096: 59 us against
+// 40; 8 x 4096: 19 against 24).
+constexpr int kMaxBytes = 40 * 1024;
 
 struct FewArgs {
     ProductArgs p;
@@ -59,8 +62,10 @@ __global__ void __launch_bounds__(kThreads) product_few_kernel(const __grid_cons
 #pragma unroll
     for (int j = 0; j < CPW; ++j)
         wv[j] = lane < vecs ? __ldg(reinterpret_cast<const uint4*>(w[j]) + lane) : make_uint4(0, 0, 0, 0);
-    if (tid < R) s_mag[tid] = 0;
-    __syncthreads();
+    if (R < kWarps) {
+        if (tid < R) s_mag[tid] = 0;
+        __syncthreads();
+    }
     pdl_trigger();
     pdl_wait();
 
@@ -71,20 +76,36 @@ __global__ void __launch_bounds__(kThreads) product_few_kernel(const __grid_cons
         const T* src = x + r * g.ldx + k * 8;
         return g.vec_in ? Q::load(src) : Q::load_some(src, min(8, K - k * 8));
     };
-    for (int r = 0; r < rows; ++r) {
-        uint32_t mag = 0;
-        for (int k = tid; k < groups; k += kThreads) mag = max(mag, Q::mag(load(r, k)));
-        mag = __reduce_max_sync(0xffffffffu, mag);
-        if (lane == 0) atomicMax(&s_mag[r], mag);
-    }
-    __syncthreads();
-    for (int r = 0; r < R; ++r) {
-        const GroupScale q = group_scale<T>(r < rows ? s_mag[r] : 0u, 127.f);
-        if (tid == 0) s_scale[r] = q.s;
-        const bool rare = q.rare;  // the same on every thread
-        for (int k = tid; k < vecs * 2; k += kThreads)
-            *reinterpret_cast<uint2*>(s_codes + r * p.ldw + k * 8) =
-                codes8<T>(r < rows && k < groups ? load(r, k) : Q::zero(), q, rare);
+    auto code_at = [&](int r, int k) { return reinterpret_cast<uint2*>(s_codes + r * p.ldw + k * 8); };
+    if constexpr (R >= kWarps) {
+        // A warp per token.
+        for (int r = tid >> 5; r < R; r += kWarps) {
+            uint32_t mag = 0;
+            if (r < rows)
+#pragma unroll 4
+                for (int k = lane; k < groups; k += 32) mag = max(mag, Q::mag(load(r, k)));
+            mag = __reduce_max_sync(0xffffffffu, mag);
+            const GroupScale q = group_scale<T>(mag, 127.f);
+            if (lane == 0) s_scale[r] = q.s;
+#pragma unroll 4
+            for (int k = lane; k < vecs * 2; k += 32)
+                *code_at(r, k) = codes8<T>(r < rows && k < groups ? load(r, k) : Q::zero(), q, q.rare);
+        }
+    } else {
+        // All warps on one or two tokens.
+        for (int r = 0; r < rows; ++r) {
+            uint32_t mag = 0;
+            for (int k = tid; k < groups; k += kThreads) mag = max(mag, Q::mag(load(r, k)));
+            mag = __reduce_max_sync(0xffffffffu, mag);
+            if (lane == 0) atomicMax(&s_mag[r], mag);
+        }
+        __syncthreads();
+        for (int r = 0; r < R; ++r) {
+            const GroupScale q = group_scale<T>(r < rows ? s_mag[r] : 0u, 127.f);
+            if (tid == 0) s_scale[r] = q.s;
+            for (int k = tid; k < vecs * 2; k += kThreads)
+                *code_at(r, k) = codes8<T>(r < rows && k < groups ? load(r, k) : Q::zero(), q, q.rare);
+        }
     }
     __syncthreads();
 
@@ -142,16 +163,6 @@ template <typename T, int R, int CPW>
 cudaError_t run(const FewArgs& g, cudaStream_t s) {
     const int per = kWarps * (g.p.gate ? CPW / 2 : CPW);
     const size_t smem = static_cast<size_t>(R) * g.p.ldw;
-    if (smem > 32 * 1024) {
-        static bool configured[64] = {};
-        int device = 0;
-        cudaError_t e = cudaGetDevice(&device);
-        if (e == cudaSuccess && (device >= 64 || !configured[device])) {
-            e = cudaFuncSetAttribute(product_few_kernel<T, R, CPW>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxBytes);
-            if (e == cudaSuccess && device < 64) configured[device] = true;
-        }
-        if (e != cudaSuccess) return e;
-    }
     return launch_pdl(product_few_kernel<T, R, CPW>, dim3((g.p.n_out + per - 1) / per), dim3(kThreads), smem, s, g);
 }
 

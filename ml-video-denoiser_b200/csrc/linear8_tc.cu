@@ -62,6 +62,7 @@ struct TcArgs {
     ProductArgs p;
     int kc, chunks;      // bytes of a K chunk, chunks of a segment
     int m_tiles, n_tiles;
+    int box_rows;        // token rows of a load: 128, or fewer of a single tile
     int tma_out;         // 1: staged TMA stores
     int unit;            // columns of a staging tile
     int resident;        // the whole weight stays in shared memory (one column tile)
@@ -148,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
             wait_or_abort(&bar_b, 0, &s_abort, p.err, 0x77);
         }
     } else if (warp == 8) {
-        const uint32_t bytes = static_cast<uint32_t>(kRows * kc * units);
+        const uint32_t bytes = static_cast<uint32_t>(g.box_rows * kc * units);
         int filled = 0, left = 0, s = 0;  // stages begun, chunks that the current one still takes
         uint32_t ph = 1;
         bool ok = true;
@@ -435,7 +436,11 @@ int run(TcArgs& g, int sms, cudaStream_t s) {
     // blocks), and for direct stores.
     g.unit = SEG || !g.tma_out ? 32 : std::min<int>(128 / sizeof(T), out_cols);
     Maps maps{};
-    DN_TRY(linear8_map(&maps.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.a, p.seg_c, p.a_rows, p.lda, g.kc, kRows));
+    // TMA takes about as long for a row that does not exist as for one that does;
+    // of a single short tile only the rows that it has are loaded. The operand's
+    // other rows hold what was there, and their sums are not stored.
+    g.box_rows = p.rows < kRows ? static_cast<int>((p.rows + 7) / 8 * 8) : kRows;
+    DN_TRY(linear8_map(&maps.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.a, p.seg_c, p.a_rows, p.lda, g.kc, g.box_rows));
     DN_TRY(linear8_map(&maps.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.w, p.ldw, p.cout, p.ldw, g.kc, p.gate ? NT / 2 : NT));
     if (g.tma_out)
         DN_TRY(linear8_map(&maps.out, sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
