@@ -26,9 +26,9 @@ constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTokens = 8;
 // Codes of all tokens in shared memory. Every CTA makes them all, which costs
-// more than the tensor-core path from there on (8 x 8000 -> 4096: 59 us against
-// 40; 8 x 4096: 19 against 24).
-constexpr int kMaxBytes = 40 * 1024;
+// more than the tensor-core path from there on (8 x 4096 -> 4096: 19 us against
+// 12, -> 512: 15 against 11; 4 x 4096 -> 4096: 12 and 12, -> 512: 7 against 11).
+constexpr int kMaxBytes = 16 * 1024;
 
 struct FewArgs {
     ProductArgs p;

@@ -142,6 +142,54 @@ __global__ void __launch_bounds__(kThreads) write_vec_kernel(const WriteArgs a) 
     }
 }
 
+// Groups of more than 2048 columns: a CTA per group, V vectors a thread in
+// registers; what a group has beyond them is read twice.
+template <typename T, int BITS, int V>
+__global__ void __launch_bounds__(kThreads) write_wide_kernel(const WriteArgs a) {
+    using Q = QuantOf<T>;
+    __shared__ uint32_t s_mag;
+    pdl_trigger();
+    if (threadIdx.x == 0) s_mag = 0;
+    __syncthreads();
+    pdl_wait();
+    constexpr float qmax = BITS == 8 ? 127.f : 7.f;
+    const int u = blockIdx.x;
+    const int row = static_cast<int>(static_cast<uint32_t>(u) / static_cast<uint32_t>(a.ngroups)), grp = u - row * a.ngroups;
+    const int nv = a.p.group / 8;
+    const T* src = static_cast<const T*>(a.p.x) + row * a.p.ldx + static_cast<int64_t>(grp) * a.p.group;
+    typename Q::Vec v[V];
+    uint32_t mag = 0;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const int c = threadIdx.x + k * kThreads;
+        v[k] = c < nv ? Q::load(src + c * 8) : Q::zero();
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) mag = max(mag, Q::mag(v[k]));
+    for (int c = threadIdx.x + V * kThreads; c < nv; c += kThreads) mag = max(mag, Q::mag(Q::load(src + c * 8)));
+    mag = __reduce_max_sync(0xffffffffu, mag);
+    if ((threadIdx.x & 31) == 0) atomicMax(&s_mag, mag);
+    __syncthreads();
+    const GroupScale g = group_scale<T>(s_mag, qmax);
+    const int64_t slot = slot_of(a, row);
+    const bool won = wins<32>(a, row, grp, slot, true);
+    __syncthreads();  // every warp has read the mark before one thread writes the scale over it
+    if (!won) return;
+    uint8_t* dst = a.p.codes + slot * a.p.ldc + static_cast<int64_t>(grp) * a.p.group * BITS / 8;
+    auto put = [&](int c, const typename Q::Vec& x) {
+        const uint2 w = codes8<T>(x, g, g.rare);
+        if (BITS == 8)
+            *reinterpret_cast<uint2*>(dst + static_cast<int64_t>(c) * 8) = w;
+        else
+            *reinterpret_cast<uint32_t*>(dst + static_cast<int64_t>(c) * 4) = pack_nibbles(w);
+    };
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+        if (static_cast<int>(threadIdx.x) + k * kThreads < nv) put(threadIdx.x + k * kThreads, v[k]);
+    for (int c = threadIdx.x + V * kThreads; c < nv; c += kThreads) put(c, Q::load(src + c * 8));
+    if (threadIdx.x == 0) a.p.scales[slot * a.ngroups + grp] = g.s;
+}
+
 // Any size and alignment: a warp takes U groups, lanes along the columns (a
 // pair of them each, so that a byte of 4-bit codes is one lane's). KEEP pairs a
 // lane stay in registers; what a group has more is read twice.
@@ -400,14 +448,17 @@ cudaError_t write_bits(const WriteArgs& a, cudaStream_t s) {
     if (nv <= 32) return write_run<T, BITS, 32, 1, 4>(a, s);
     if (nv <= 64) return write_run<T, BITS, 32, 2, 2>(a, s);
     if (nv <= 128) return write_run<T, BITS, 32, 4, 1>(a, s);
-    return write_run<T, BITS, 32, 8, 1>(a, s);
+    if (nv <= 256) return write_run<T, BITS, 32, 8, 1>(a, s);
+    const dim3 grid(static_cast<unsigned>(a.p.rows * a.ngroups));
+    if (nv <= 2 * kThreads) return launch_pdl(write_wide_kernel<T, BITS, 2>, grid, dim3(kThreads), 0, s, a);
+    return launch_pdl(write_wide_kernel<T, BITS, 4>, grid, dim3(kThreads), 0, s, a);
 }
 
 template <typename T>
 cudaError_t write_type(const WriteArgs& a, cudaStream_t s) {
     const CacheWrite& p = a.p;
     // A vector of 8 codes has `bits` bytes.
-    const bool vec = p.group % 8 == 0 && p.group <= 2048 && aligned(p.x, 16) && p.ldx * sizeof(T) % 16 == 0 &&
+    const bool vec = p.group % 8 == 0 && aligned(p.x, 16) && p.ldx * sizeof(T) % 16 == 0 &&
                      aligned(p.codes, p.bits) && p.ldc % p.bits == 0;
     if (vec) return p.bits == 8 ? write_bits<T, 8>(a, s) : write_bits<T, 4>(a, s);
     // 8 pairs a lane in registers: groups of one row, or pieces of several.

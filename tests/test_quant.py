@@ -172,7 +172,8 @@ def test_layer_create_from_a_store_refuses(pkg, tmp_path):
 @pytest.mark.parametrize("dtype", [np.float16, np.float32])
 @pytest.mark.parametrize("rows,cols,group", [(1, 1, 0), (1, 8, 0), (3, 7, 0), (5, 24, 0), (70, 32, 0), (33, 32, 8),
                                              (9, 64, 16), (6, 96, 0), (13, 192, 64), (7, 520, 0), (40, 512, 32),
-                                             (5, 1000, 0), (4, 2048, 0), (3, 2064, 0), (2, 5001, 0), (2, 4608, 2304)])
+                                             (5, 1000, 0), (4, 2048, 0), (3, 2064, 0), (2, 5001, 0), (2, 4608, 2304),
+                                             (2, 4096, 0), (3, 9000, 0), (2, 20008, 0)])
 def test_codes_and_scales(Q, bits, dtype, rows, cols, group):
     rng = np.random.default_rng(rows * 1000 + cols + bits)
     x = rows_of(rng, rows, cols, dtype)
@@ -269,7 +270,7 @@ def test_strides_and_alignment(Q):
 
 @gpu
 @pytest.mark.parametrize("rows,cols,group", [(1, 32, 0), (40, 32, 0), (256, 24, 0), (300, 32, 0), (2000, 64, 16),
-                                             (300, 33, 0), (90, 512, 32)])
+                                             (300, 33, 0), (90, 512, 32), (260, 2304, 0), (30, 2304, 0)])
 @pytest.mark.parametrize("bits", [8, 4])
 def test_scattered_rows_the_last_of_a_slot_counts(Q, rows, cols, group, bits):
     rng = np.random.default_rng(rows + cols)
