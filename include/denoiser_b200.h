@@ -160,6 +160,18 @@ int dn_model_encode_frame(dn_model* model, const void* frame, int C, int H, int 
 int dn_model_decode_window(dn_model* model, const int* slots, int T, const void* beauty, int C, int H, int W,
                            void* y, void* stream);
 
+/* Where the model keeps the features of the frame in `slot`: `level` 0 ..
+ * num_levels - 1 the encoder's skips, num_levels the deep features; FP16
+ * [rows][channels], a row per pixel of the padded frame at that level. For
+ * holding frames elsewhere (dn_launch_cache_write / dn_launch_cache_read_rows
+ * of denoiser_b200_quant.h, straight into and out of a slot) and decoding
+ * several sequences in turn with one model. Plans the buffers for H x W frames
+ * like dn_model_encode_frame, and the address holds as long as they do: while
+ * the frame size does not change. DN_ERR_INVALID_ARG as there, and for a level
+ * outside [0, num_levels]. */
+int dn_model_frame_features(dn_model* model, int H, int W, int slot, int level, void** features, int64_t* rows,
+                            int* channels);
+
 /* Synchronise `stream`; DN_ERR_DEVICE if a kernel reported a device-side
  * error (e.g. a bounded wait that expired) since the last check. */
 int dn_model_sync(dn_model* model, void* stream);

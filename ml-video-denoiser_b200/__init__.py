@@ -88,6 +88,7 @@ SIGNATURES = {
     "dn_model_forward_host": (_I, [_P, _P, _I64P, _I, _P, _P]),
     "dn_model_encode_frame": (_I, [_P, _P, _I, _I, _I, _I, _P]),
     "dn_model_decode_window": (_I, [_P, _IP, _I, _P, _I, _I, _I, _P, _P]),
+    "dn_model_frame_features": (_I, [_P, _I, _I, _I, _I, _PP, _I64P, _IP]),
     "dn_model_sync": (_I, [_P, _P]),
     "dn_model_stats": (_I, [_P, _SZP, _SZP, _IP]),
     "dn_model_set_fused": (_I, [_P, _I]),
@@ -258,6 +259,13 @@ class Weights:
                 "in_channels": v[2].value, "num_frames": v[3].value, "use_warp": bool(v[4].value)}
 
 
+class _DeviceMemory:
+    """Device memory of the engine, as torch.as_tensor takes it."""
+
+    def __init__(self, ptr: int, shape, typestr: str):
+        self.__cuda_array_interface__ = {"shape": shape, "typestr": typestr, "data": (ptr, False), "version": 2}
+
+
 class Model:
     """NAFNet / NAFNetTemporal engine instance on one CUDA device.
 
@@ -360,6 +368,20 @@ class Model:
         check(lib().dn_model_decode_window(self._h, arr, len(slots), ctypes.c_void_p(beauty.data_ptr()), c, h, w,
                                            ctypes.c_void_p(out.data_ptr()), stream_handle(stream)))
         return out
+
+    def frame_features(self, h: int, w: int, slot: int, level: int):
+        """Temporal models: the features of the h x w frame in cache slot `slot`
+        as the engine holds them, an FP16 CUDA tensor (rows, channels) on its
+        own memory: `level` 0 .. num_levels - 1 the skips, num_levels the deep
+        features, a row per pixel of the padded frame. Valid while the frame
+        size does not change and the model lives."""
+        import torch
+
+        p, rows, ch = ctypes.c_void_p(), ctypes.c_int64(), ctypes.c_int()
+        check(lib().dn_model_frame_features(self._h, h, w, slot, level, ctypes.byref(p), ctypes.byref(rows),
+                                            ctypes.byref(ch)))
+        return torch.as_tensor(_DeviceMemory(p.value, (rows.value, ch.value), "<f2"),
+                               device=torch.device("cuda", self.device))
 
     def sync(self, stream=None) -> None:
         """Synchronise the stream and raise if a kernel flagged a device error."""

@@ -1222,6 +1222,22 @@ int Engine::decode_window(const int* slots, const __half* beauty, int C, int H, 
     return temporal_tail(slots, beauty, C * H * W, y, s);
 }
 
+int Engine::frame_features(int H, int W, int slot, int level, __half** features, int64_t* rows, int* channels) {
+    const int L = info_.num_levels;
+    if (info_.kind == 0) return dn_fail(DN_ERR_INVALID_ARG, "frame_features: spatial models have no frame cache");
+    if (slot < 0 || slot >= info_.num_frames) return dn_fail(DN_ERR_INVALID_ARG, "frame_features: slot outside [0, T)");
+    if (level < 0 || level > L) return dn_fail(DN_ERR_INVALID_ARG, "frame_features: level outside [0, num_levels]");
+    DeviceGuard dg(device_);
+    Shape sh;
+    DN_TRY(make_shape(1, info_.num_frames, info_.in_channels, H, W, sh));
+    const int64_t n = static_cast<int64_t>(shape_.Hp >> level) * (shape_.Wp >> level);
+    const int c = level < L ? levels_[level].C : levels_[L - 1].C * 2;
+    if (features) *features = (level < L ? enc_x_[level] : mid_x_) + slot * n * c;
+    if (rows) *rows = n;
+    if (channels) *channels = c;
+    return DN_OK;
+}
+
 int Engine::check_device(cudaStream_t s) {
     DeviceGuard dg(device_);
     cudaError_t e = cudaStreamSynchronize(s);

@@ -82,6 +82,10 @@ public:
     int encode_frame(const __half* frame, int C, int H, int W, int slot, cudaStream_t s);
     int decode_window(const int* slots, const __half* beauty, int C, int H, int W, __half* y, cudaStream_t s);
 
+    // The features of cache slot `slot` at `level` (num_levels = deep features)
+    // of H x W frames: FP16 [rows][channels].
+    int frame_features(int H, int W, int slot, int level, __half** features, int64_t* rows, int* channels);
+
     // Waits for `s` and returns DN_ERR_DEVICE if a kernel flagged an error
     // since the last check (the word is cleared).
     int check_device(cudaStream_t s);

@@ -38,7 +38,6 @@ struct FusedArgs {
     int64_t ldx;     // row stride (token rows)
     int m_tiles;
     int vec_in;      // token rows: 16-byte loads of x are aligned
-    int flat;        // token rows one behind the other that are no multiple of 16 bytes: loaded as one run
     int tma_out;
     int pairs;       // direct stores: pairs of outputs are 4-byte aligned
     int unit;        // columns of a staging tile (tma_out)
@@ -69,7 +68,9 @@ struct Shape {
     static constexpr int smem(int run_k) { return kSmem + kRows * 2 * run_k; }
 };
 
-template <typename T, bool PLANES, int SG, int NT>
+// RUN: token rows one behind the other that are no multiple of 16 bytes, loaded
+// as one run.
+template <typename T, bool PLANES, int SG, int NT, bool RUN>
 __global__ void __launch_bounds__(Shape<PLANES, SG, NT>::kThreads) product_fused_kernel(
     const __grid_constant__ FusedArgs g, const __grid_constant__ CUtensorMap out_map) {
     using S = Shape<PLANES, SG, NT>;
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(Shape<PLANES, SG, NT>::kThreads) product_fused
                 }
                 v[i].v = make_uint4(w[0], w[1], w[2], w[3]);
             }
-        } else if (g.flat) {
+        } else if (RUN) {
             // This warp's rows are one run of kWarpRows K values from a 16-byte boundary on.
             const int64_t first = (static_cast<int64_t>(tile) * kRows + warp * kWarpRows) * K;
             const int64_t end = p.rows * K;
@@ -194,7 +195,7 @@ __global__ void __launch_bounds__(Shape<PLANES, SG, NT>::kThreads) product_fused
             }
             sx[r] = q.s;
         } else {
-            if (g.flat) {  // from the run to a lane's vectors of its rows
+            if (RUN) {  // from the run to a lane's vectors of its rows
                 uint8_t* raw = smem + S::kA + S::kB + S::kStg + warp * kWarpRows * K * 2;
                 __syncwarp();
 #pragma unroll
@@ -325,7 +326,7 @@ __global__ void __launch_bounds__(Shape<PLANES, SG, NT>::kThreads) product_fused
     if (warp == 0) tmem_dealloc(tmem, kCols);
 }
 
-template <typename T, bool PLANES, int SG, int NT>
+template <typename T, bool PLANES, int SG, int NT, bool RUN>
 int run(FusedArgs& g, int sms, cudaStream_t s) {
     using S = Shape<PLANES, SG, NT>;
     const ProductArgs& p = g.p;
@@ -343,35 +344,42 @@ int run(FusedArgs& g, int sms, cudaStream_t s) {
                            sizeof(T), p.out, p.n_out, p.rows, p.ldo, g.unit, 32));
     static int resident[64] = {};
     int per_sm = 0;
-    auto kernel = product_fused_kernel<T, PLANES, SG, NT>;
-    g.flat = g.flat && p.seg_c <= S::kRunK;
-    const int smem = S::smem(g.flat ? p.seg_c : 0), most = S::smem(S::kRunK);
+    auto kernel = product_fused_kernel<T, PLANES, SG, NT, RUN>;
+    const int smem = S::smem(RUN ? p.seg_c : 0);
     int fresh[64] = {};  // a run's buffer depends on Cin
-    cudaError_t e = tmem_kernel_ctas(kernel, S::kThreads, smem, most, NT, g.flat ? fresh : resident, &per_sm);
+    cudaError_t e = tmem_kernel_ctas(kernel, S::kThreads, smem, S::smem(RUN ? S::kRunK : 0), NT, RUN ? fresh : resident, &per_sm);
     if (e == cudaSuccess)
         e = launch_pdl(kernel, dim3(static_cast<unsigned>(std::min(g.m_tiles, per_sm * sms))), dim3(S::kThreads), smem, s, g,
                        map);
     return e == cudaSuccess ? DN_OK : dn_cuda_fail(e, "linear8: fused launch");
 }
 
+template <typename T, bool PLANES, int SG, int NT>
+int run_kind(FusedArgs& g, const void* x, int sms, cudaStream_t s) {
+    const bool contiguous = !g.vec_in && g.ldx == g.p.seg_c && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+    if constexpr (!PLANES)
+        if (contiguous && g.p.seg_c <= Shape<PLANES, SG, NT>::kRunK) return run<T, PLANES, SG, NT, true>(g, sms, s);
+    return run<T, PLANES, SG, NT, false>(g, sms, s);
+}
+
 template <typename T, bool PLANES, int SG>
-int run_nt(FusedArgs& g, int sms, cudaStream_t s) {
+int run_nt(FusedArgs& g, const void* x, int sms, cudaStream_t s) {
     const int need = fused_width(g.p);
-    if (need <= 32) return run<T, PLANES, SG, 32>(g, sms, s);
-    if (need <= 64) return run<T, PLANES, SG, 64>(g, sms, s);
-    if (need <= 128) return run<T, PLANES, SG, 128>(g, sms, s);
-    return run<T, PLANES, SG, 256>(g, sms, s);
+    if (need <= 32) return run_kind<T, PLANES, SG, 32>(g, x, sms, s);
+    if (need <= 64) return run_kind<T, PLANES, SG, 64>(g, x, sms, s);
+    if (need <= 128) return run_kind<T, PLANES, SG, 128>(g, x, sms, s);
+    return run_kind<T, PLANES, SG, 256>(g, x, sms, s);
 }
 
 template <typename T, bool PLANES>
-int run_k(FusedArgs& g, int sms, cudaStream_t s) {
+int run_k(FusedArgs& g, const void* x, int sms, cudaStream_t s) {
     const int K = g.p.seg_c;
-    if (K <= 16) return run_nt<T, PLANES, 2>(g, sms, s);
-    if (K <= 32) return run_nt<T, PLANES, 4>(g, sms, s);
-    if (K <= 64) return run_nt<T, PLANES, 8>(g, sms, s);
+    if (K <= 16) return run_nt<T, PLANES, 2>(g, x, sms, s);
+    if (K <= 32) return run_nt<T, PLANES, 4>(g, x, sms, s);
+    if (K <= 64) return run_nt<T, PLANES, 8>(g, x, sms, s);
     if constexpr (!PLANES)
-        if (K > 128) return run_nt<T, PLANES, 32>(g, sms, s);
-    return run_nt<T, PLANES, 16>(g, sms, s);
+        if (K > 128) return run_nt<T, PLANES, 32>(g, x, sms, s);
+    return run_nt<T, PLANES, 16>(g, x, sms, s);
 }
 
 }  // namespace
@@ -386,10 +394,9 @@ int launch_product_fused(const ProductArgs& a, const void* x, int64_t ldx, int o
     g.x = static_cast<const __half*>(x);
     g.ldx = ldx;
     g.vec_in = a.seg_c % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % 8 == 0;
-    g.flat = !a.planes && !g.vec_in && ldx == a.seg_c && reinterpret_cast<uintptr_t>(x) % 16 == 0;
     g.m_tiles = static_cast<int>((a.rows + kRows - 1) / kRows);
-    if (a.planes) return run_k<__half, true>(g, sms, s);
-    return out_dtype == 1 ? run_k<__half, false>(g, sms, s) : run_k<float, false>(g, sms, s);
+    if (a.planes) return run_k<__half, true>(g, x, sms, s);
+    return out_dtype == 1 ? run_k<__half, false>(g, x, sms, s) : run_k<float, false>(g, x, sms, s);
 }
 
 }  // namespace dnb

@@ -4,6 +4,9 @@ include/denoiser_b200_quant.h (which has the exact definitions):
 ``RowCache``  rows quantised to 8 or 4 bits as they are written (a scale for
               each row or group of columns) and read back through row numbers
               or page tables;
+``FrameStore`` encoded frames of a temporal model in RowCaches, so that one
+              model decodes several sequences in turn (``sharding.
+              denoise_streams``);
 ``Linear8``   the product of tokens with a weight matrix in 8-bit integers,
               a scale for each token and each output channel: over token rows,
               over the pixels of NCHW planes (a 1x1 convolution), or straight
@@ -205,6 +208,44 @@ class RowCache:
                 self._err.zero_()
         if word:
             raise DenoiserError(DN_ERR_DEVICE, f"RowCache: a slot or page lies behind the cache (error word {word:#x})")
+
+
+class FrameStore:
+    """``frames`` encoded h x w frames of a temporal Model in 8 (or 4) bits, a
+    RowCache per level: ``park`` quantises a frame's features out of the model's
+    cache slot, ``restore`` puts them back into a slot (any one, any number of
+    times). A slot holds them in FP16; the store takes half of that (or a
+    quarter), and the model's T slots can serve many sequences."""
+
+    def __init__(self, model, h: int, w: int, frames: int, bits: int = 8, group: int = 0):
+        self.model, self.h, self.w, self.frames = model, h, w, frames
+        self.caches = []
+        for level in range(model.num_levels + 1):
+            rows, cols = model.frame_features(h, w, 0, level).shape
+            self.caches.append(RowCache(frames, rows, cols, bits=bits, group=group, device=model.device))
+
+    def _entry(self, entry: int) -> int:
+        if not 0 <= entry < self.frames:
+            _bad(f"FrameStore: entry {entry} outside [0, {self.frames})")
+        return entry
+
+    def park(self, slot: int, entry: int, stream=None) -> None:
+        """The frame in the model's cache slot `slot` into `entry`."""
+        self._entry(entry)
+        for level, c in enumerate(self.caches):
+            c.write(self.model.frame_features(self.h, self.w, slot, level), row0=entry * c.page_rows, stream=stream)
+
+    def restore(self, entry: int, slot: int, stream=None) -> None:
+        """The frame of `entry` into the model's cache slot `slot`."""
+        self._entry(entry)
+        for level, c in enumerate(self.caches):
+            c.read_rows(row0=entry * c.page_rows, rows=c.page_rows,
+                        out=self.model.frame_features(self.h, self.w, slot, level), stream=stream)
+
+    @property
+    def bytes(self) -> int:
+        """Device bytes of the held codes and scales."""
+        return sum(c.codes.numel() + 4 * c.scales.numel() for c in self.caches)
 
 
 class Linear8:

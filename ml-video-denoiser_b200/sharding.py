@@ -115,6 +115,52 @@ def denoise_range(model, frames, n_frames: int, start: int, end: int, num_frames
     return results
 
 
+def denoise_streams(model, clips, num_frames: int, bits: int = 8, store=None, stream=None, on_frame=None):
+    """Denoise several clips of one frame size in turn with one temporal model:
+    output 0 of every clip, then output 1, and so on (streams that are served
+    together). `clips` is a list of (frames, n_frames) as ``denoise_range``
+    takes them.
+
+    The model's T cache slots hold one window; the encoded frames of all clips'
+    windows wait in a ``quant.FrameStore`` in 8 (or 4) bits (`store`: one with
+    T entries per clip, or made here), so that every frame is encoded once and
+    not T times per output. Every frame goes through the store, one clip's too:
+    what a clip's outputs are does not depend on the others.
+
+    Returns [(clip, frame index, output)]; ``on_frame(clip, i, y)``, when given,
+    is called after each output."""
+    T = num_frames
+    if T <= 1 or T % 2 == 0:
+        raise ValueError("num_frames must be an odd number above 1")
+    results = []
+    in_slot = [None] * T                  # (clip, frame) that each model slot holds, as restored from the store
+    held = [[-1] * T for _ in clips]      # frame in each of a clip's store entries
+    for i in range(max((n for _, n in clips), default=0)):
+        for k, (frames, n) in enumerate(clips):
+            if i >= n:
+                continue
+            win = window(i, T, n)
+            for f in dict.fromkeys(win):
+                s, entry = f % T, k * T + f % T
+                if held[k][s] != f:
+                    x = frames(f).unsqueeze(0).contiguous()
+                    if store is None:
+                        from .quant import FrameStore
+
+                        store = FrameStore(model, x.shape[2], x.shape[3], len(clips) * T, bits=bits)
+                    model.encode_frame(x, s, stream=stream)
+                    store.park(s, entry, stream=stream)
+                    held[k][s], in_slot[s] = f, None
+                if in_slot[s] != (k, f):
+                    store.restore(entry, s, stream=stream)
+                    in_slot[s] = (k, f)
+            y = model.decode_window([f % T for f in win], frames(i).unsqueeze(0).contiguous(), stream=stream)[0]
+            results.append((k, i, y))
+            if on_frame is not None:
+                on_frame(k, i, y)
+    return results
+
+
 # ---------------------------------------------------------------------------
 # Clip coordinator with segment re-queue
 # ---------------------------------------------------------------------------

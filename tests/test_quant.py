@@ -562,6 +562,112 @@ def test_calls_refuse(pkg, Q):
 
 
 # ---------------------------------------------------------------------------------------------------------------------
+# Frames of a temporal model in the cache
+# ---------------------------------------------------------------------------------------------------------------------
+
+class FakeModel:
+    """encode: 10 times the frame, in the slot; decode: the window's slots."""
+
+    def __init__(self, T):
+        self.slots, self.encoded, self.num_frames = [None] * T, 0, T
+
+    def encode_frame(self, x, slot, stream=None):
+        self.slots[slot] = float(x.ravel()[0]) * 10
+        self.encoded += 1
+
+    def decode_window(self, slots, beauty, stream=None):
+        return [(tuple(self.slots[s] for s in slots), float(beauty.ravel()[0]))]
+
+
+class FakeStore:
+    """Adds a quarter to what it holds, so that a frame past it shows."""
+
+    def __init__(self, model):
+        self.model, self.held = model, {}
+
+    def park(self, slot, entry, stream=None):
+        self.held[entry] = self.model.slots[slot] + 0.25
+
+    def restore(self, entry, slot, stream=None):
+        self.model.slots[slot] = self.held[entry]
+
+
+@pytest.mark.parametrize("T", [3, 5])
+def test_streams_served_in_turn(pkg, T):
+    """Every frame is encoded once, and every window is its clip's, each frame
+    as it comes out of the store."""
+    S = importlib.import_module(pkg.__name__ + ".sharding")
+    lengths = [6, 1, 4]
+    clips = [(lambda f, k=k: torch.full((3, 2, 2), 100.0 * k + f), n) for k, n in enumerate(lengths)]
+    m = FakeModel(T)
+    got = S.denoise_streams(m, clips, T, store=FakeStore(m))
+    assert [(k, i) for k, i, _ in got] == [(k, i) for i in range(6) for k in range(3) if i < lengths[k]]
+    for k, i, y in got:
+        want = tuple((100.0 * k + f) * 10 + 0.25 for f in S.window(i, T, lengths[k]))
+        assert y == (want, 100.0 * k + i)
+    assert m.encoded == sum(lengths)
+    with pytest.raises(ValueError):
+        S.denoise_streams(m, clips, 4)
+    assert S.denoise_streams(m, [], T) == []
+
+
+def small_temporal(pkg, tmp_path, kind, T):
+    synth = importlib.import_module(pkg.__name__ + ".synth")
+    cfg = synth.NAFConfig(base_channels=8, enc_blocks=(1, 1), middle_blocks=1, dec_blocks=(1, 1))
+    return pkg.Model(synth.make_model_dir(str(tmp_path), cfg, 4, kind, T, True)[0])
+
+
+@gpu
+@pytest.mark.parametrize("kind,T", [("legacy", 3), ("py", 5)])
+@pytest.mark.parametrize("bits", [8, 4])
+def test_streams_through_the_frame_store(pkg, Q, tmp_path, kind, T, bits):
+    """A parked frame is its features' codes; outputs of clips in turn are those
+    of a decode whose slots hold the values that the codes stand for, and do not
+    depend on the other clips."""
+    S = importlib.import_module(pkg.__name__ + ".sharding")
+    m = small_temporal(pkg, tmp_path, kind, T)
+    H, W = 30, 42
+    rng = np.random.default_rng(6)
+    clips = [[dev(rng.uniform(0, 1, (3, H, W)).astype(np.float16)) for _ in range(n)] for n in (5, 3)]
+    store = Q.FrameStore(m, H, W, 2, bits=bits)
+    m.encode_frame(clips[0][1].unsqueeze(0), 1)
+    raw = [host(m.frame_features(H, W, 1, l)).copy() for l in range(m.num_levels + 1)]
+    assert [r.shape[1] for r in raw] == m.enc_channels + [2 * m.enc_channels[-1]]
+    store.park(1, 1)
+    store.restore(1, 0)
+    for l, (r, c) in enumerate(zip(raw, store.caches)):
+        q, s = qo.quantise(r, bits)
+        assert_held(c, slice(c.page_rows, 2 * c.page_rows), q, s, bits)
+        assert_read(host(m.frame_features(H, W, 0, l)), q, s)
+        np.testing.assert_array_equal(host(m.frame_features(H, W, 1, l)), r)
+        c.sync()
+    take = [(lambda f, c=c: c[f], len(c)) for c in clips]
+    both = {(k, i): y.clone() for k, i, y in S.denoise_streams(m, take, T, bits=bits)}
+    m.sync()
+    assert sorted(both) == [(k, i) for k, c in enumerate(clips) for i in range(len(c))]
+    for k, c in enumerate(clips):
+        alone = {i: y.clone() for _, i, y in S.denoise_streams(m, [take[k]], T, bits=bits)}
+        for i in range(len(c)):
+            assert torch.equal(alone[i], both[k, i]), (k, i)
+    for i in (0, 3):
+        win = S.window(i, T, 5)
+        for f in dict.fromkeys(win):
+            m.encode_frame(clips[0][f].unsqueeze(0), f % T)
+            for l in range(m.num_levels + 1):
+                v = m.frame_features(H, W, f % T, l)
+                q, s = qo.quantise(host(v), bits)
+                # the FP32 product of code and scale, rounded to FP16, as the cache reads it
+                v.copy_(dev((q.astype(np.float32) * s).astype(np.float16)))
+        want = m.decode_window([f % T for f in win], clips[0][i].unsqueeze(0))[0]
+        assert torch.equal(both[0, i], want), i
+    for bad in (lambda: store.park(1, 2), lambda: store.restore(-1, 0), lambda: store.park(T, 0),
+                lambda: m.frame_features(H, W, 0, m.num_levels + 1), lambda: m.frame_features(H, W, 0, -1)):
+        with pytest.raises(pkg.InvalidArgumentError):
+            bad()
+    assert store.bytes < sum(r.nbytes for r in raw) * 2
+
+
+# ---------------------------------------------------------------------------------------------------------------------
 # Together
 # ---------------------------------------------------------------------------------------------------------------------
 
