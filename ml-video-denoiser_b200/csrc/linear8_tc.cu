@@ -183,6 +183,9 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
             const int n0 = (tile % g.n_tiles) * out_cols;
             for (int t = 0; ok && t < segs; ++t)
                 for (int j = 0; j < chunks; ++j) {
+                    // The ring filled up once ahead of the earlier kernels; what
+                    // empties it waits for them, however long they take.
+                    if (filled == kSt) pdl_wait();
                     ok = wait_or_abort(&bar_empty[s], ph, &s_abort, p.err, 0x70);
                     if (!ok) break;
                     uint8_t* sb = smem + s * stage + kStageA;

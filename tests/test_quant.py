@@ -495,6 +495,33 @@ def test_rows_that_are_not_finite_stay_by_themselves(Q, rows, k):
 
 
 @gpu
+def test_the_longest_sum(Q):
+    """131072 channels, every product of codes 127 * 127: the int32 sum's limit."""
+    k = 131072
+    x = torch.ones(20, k, dtype=torch.float16, device="cuda")
+    x[1::2] = -1
+    layer = Q.Linear8.from_tensors(torch.full((40, k), 0.5, dtype=torch.float16, device="cuda"))
+    for rows in (1, 20):
+        y, e = qo.product(*qo.quantise(host(x[:rows])), *qo.quantise(np.full((40, k), 0.5, np.float16)))
+        assert_product(host(layer(x[:rows], out_dtype=torch.float32)), y, e)
+    layer.sync()
+
+
+@gpu
+def test_behind_a_long_kernel(Q):
+    """The product's weight loads run ahead of the earlier work on the stream;
+    its bounded waits do not begin before that is done."""
+    rng = np.random.default_rng(9)
+    layer, (qw, sw, b) = make(Q, rng, 2048, 600, False, True)
+    x = rows_of(rng, 200, 2048)
+    dx = dev(x)
+    torch.cuda._sleep(int(2.6 * 1.965e9))
+    got = layer(dx)
+    layer.sync()
+    assert_product(host(got), *qo.product(*qo.quantise(x), qw, sw, b))
+
+
+@gpu
 def test_no_rows_is_no_work(Q):
     layer = Q.Linear8.from_tensors(torch.ones(6, 32, dtype=torch.float16, device="cuda"))
     assert layer(torch.zeros(0, 32, dtype=torch.float16, device="cuda")).shape == (0, 6)
