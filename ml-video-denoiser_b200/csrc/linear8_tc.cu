@@ -77,8 +77,8 @@ __device__ __forceinline__ void finish32(const float2* par, float (&y)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
         const float4 w = __ldg(reinterpret_cast<const float4*>(par + i));
-        y[i] = fmaf(y[i], w.x, w.y);
-        y[i + 1] = fmaf(y[i + 1], w.z, w.w);
+        const float2 z = ffma2(make_float2(y[i], y[i + 1]), make_float2(w.x, w.z), make_float2(w.y, w.w));
+        y[i] = z.x, y[i + 1] = z.y;
     }
 }
 
@@ -341,8 +341,13 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
                         int a[32];
                         tmem_ld32(lane_base + (q % kAcc) * NT + col[k], a);
                         tmem_ld_wait();
+                        const float2 st2 = make_float2(st, st);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) y[k][i] = fmaf(static_cast<float>(a[i]), st, y[k][i]);
+                        for (int i = 0; i < 32; i += 2) {
+                            const float2 z = ffma2(make_float2(static_cast<float>(a[i]), static_cast<float>(a[i + 1])), st2,
+                                                   make_float2(y[k][i], y[k][i + 1]));
+                            y[k][i] = z.x, y[k][i + 1] = z.y;
+                        }
                     }
                     acc_done(q);
                     ++q;
