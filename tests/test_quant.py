@@ -413,6 +413,20 @@ def test_token_rows(Q, rows, k, n, gate, x_type, y_type):
 
 
 @gpu
+@pytest.mark.parametrize("rows,k,n", [(19000, 300, 256), (5000, 272, 1030), (4999, 520, 1024), (9473, 261, 512)])
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("y_type", [torch.float16, torch.float32])
+def test_many_tiles(Q, rows, k, n, gate, y_type):
+    """More tiles than SMs, in the widest form."""
+    rng = np.random.default_rng(rows)
+    layer, (qw, sw, b) = make(Q, rng, k, n, gate, bias=True)
+    x = rows_of(rng, rows, k)
+    got = host(layer(dev(x), out_dtype=y_type))
+    layer.sync()
+    assert_product(got, *qo.product(*qo.quantise(x), qw, sw, b, gate))
+
+
+@gpu
 @pytest.mark.parametrize("n_img,k,h,w,n", [(1, 3, 1, 1, 5), (1, 32, 33, 47, 64), (2, 64, 16, 20, 128), (3, 17, 9, 7, 34),
                                            (1, 256, 24, 32, 256), (2, 300, 13, 11, 520), (1, 128, 64, 64, 32),
                                            (2, 16, 1, 129, 8), (1, 512, 8, 16, 64), (5, 48, 3, 5, 96),
