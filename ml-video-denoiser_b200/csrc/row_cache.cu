@@ -316,7 +316,8 @@ __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 
 // SG lanes per row, a lane W = 8 or 16 columns at a time (of one group), U rows
 // of each sub-warp in flight. 16 columns halve the work per row, which bounds
-// narrow rows: READ16.
+// narrow rows (five frames of 522240 x 64: 105 us on the device, 107 with 8
+// columns; a kernel that only writes its 334 MB takes 88).
 template <typename T, int BITS, int SG, int U, int W>
 __global__ void __launch_bounds__(kThreads) read_vec_kernel(const ReadArgs a) {
     pdl_trigger();
@@ -474,15 +475,23 @@ cudaError_t read_run(const ReadArgs& a, int batch, cudaStream_t s) {
                       dim3(kThreads), 0, s, a);
 }
 
+template <typename T, int BITS, int SG, int W>
+cudaError_t read_rows(const ReadArgs& a, int batch, cudaStream_t s) {
+    // Four rows in flight per sub-warp where that still gives every SM four
+    // CTAs; short reads spread over more warps instead.
+    const int64_t ctas = a.rows * batch / (kWarps * (32 / SG) * 4);
+    return ctas >= 4 * 148 ? read_run<T, BITS, SG, 4, W>(a, batch, s) : read_run<T, BITS, SG, 1, W>(a, batch, s);
+}
+
 template <typename T, int BITS, int W>
 cudaError_t read_width(const ReadArgs& a, int batch, cudaStream_t s) {
     switch (pow2_lanes(a.cols / W)) {
-        case 1: return read_run<T, BITS, 1, 4, W>(a, batch, s);
-        case 2: return read_run<T, BITS, 2, 4, W>(a, batch, s);
-        case 4: return read_run<T, BITS, 4, 4, W>(a, batch, s);
-        case 8: return read_run<T, BITS, 8, 4, W>(a, batch, s);
-        case 16: return read_run<T, BITS, 16, 4, W>(a, batch, s);
-        default: return read_run<T, BITS, 32, 4, W>(a, batch, s);
+        case 1: return read_rows<T, BITS, 1, W>(a, batch, s);
+        case 2: return read_rows<T, BITS, 2, W>(a, batch, s);
+        case 4: return read_rows<T, BITS, 4, W>(a, batch, s);
+        case 8: return read_rows<T, BITS, 8, W>(a, batch, s);
+        case 16: return read_rows<T, BITS, 16, W>(a, batch, s);
+        default: return read_rows<T, BITS, 32, W>(a, batch, s);
     }
 }
 
