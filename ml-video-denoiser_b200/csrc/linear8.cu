@@ -26,14 +26,18 @@ constexpr int kMaxK = 131072;  // 127 * 127 * 131072 < 2^31
 // a CTA of eight warps takes 32 PX pixels, a lane PX adjacent ones of them
 // (two where pairs are 4-byte aligned) and a warp 32 channels at a time, so
 // that the loads of 32 channels are in flight and a lane's codes are a whole
-// 32-byte sector. A warp's first run of channels stays in registers between the
-// two passes, the others are read again out of L1 or L2 (four runs in registers
-// cost more in occupancy than they save).
+// 32-byte sector. Between the two passes a warp's first run of channels stays in
+// registers; with pixel pairs the next `kept` ones stay in shared memory (each
+// lane its own vectors), what a very wide layer has beyond them is read again.
+// Single pixels read all of them again: there the occupancy is worth more (2
+// images of 36867 pixels, 1296 -> 26 gated: 152 us, 274 with 96 KB kept; pairs of
+// 36868: 112 us, 120 without).
 template <int PX>
 __global__ void __launch_bounds__(256) quantise_planes_kernel(const __half* __restrict__ x, int64_t rows, int K, int64_t hw,
                                                               uint8_t* __restrict__ codes, int64_t ldc,
-                                                              float* __restrict__ scales) {
+                                                              float* __restrict__ scales, int kept) {
     using Q = QuantOf<__half>;
+    extern __shared__ __align__(16) uint4 s_keep[];  // [run][warp][pixel][4][lane]
     __shared__ uint32_t s_mag[32 * PX];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x < 32 * PX) s_mag[threadIdx.x] = 0;
@@ -75,10 +79,17 @@ __global__ void __launch_bounds__(256) quantise_planes_kernel(const __half* __re
     Q::Vec keep[PX][4];
     load(warp * 32, keep);
     largest(keep);
-    for (int k0 = warp * 32 + 256; k0 < K; k0 += 256) {
+    auto kept_at = [&](int j, int q, int i) { return &s_keep[(((j * 8 + warp) * PX + q) * 4 + i) * 32 + lane]; };
+    for (int k0 = warp * 32 + 256, j = 0; k0 < K; k0 += 256, ++j) {
         Q::Vec v[PX][4];
         load(k0, v);
         largest(v);
+        if constexpr (PX == 2)
+            if (j < kept)
+#pragma unroll
+                for (int q = 0; q < PX; ++q)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) *kept_at(j, q, i) = v[q][i].v;
     }
 #pragma unroll
     for (int q = 0; q < PX; ++q) atomicMax(&s_mag[lane * PX + q], mag[q]);
@@ -103,9 +114,16 @@ __global__ void __launch_bounds__(256) quantise_planes_kernel(const __half* __re
         }
     };
     store(warp * 32, keep);
-    for (int k0 = warp * 32 + 256; k0 < K; k0 += 256) {
+    for (int k0 = warp * 32 + 256, j = 0; k0 < K; k0 += 256, ++j) {
         Q::Vec v[PX][4];
-        load(k0, v);
+        if (PX == 2 && j < kept) {
+#pragma unroll
+            for (int q = 0; q < PX; ++q)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[q][i].v = *kept_at(j, q, i);
+        } else {
+            load(k0, v);
+        }
         store(k0, v);
     }
     if (warp == 0 && live)
@@ -116,8 +134,20 @@ __global__ void __launch_bounds__(256) quantise_planes_kernel(const __half* __re
 template <int PX>
 cudaError_t quantise_planes(const void* x, int64_t rows, int K, int64_t hw, uint8_t* codes, int64_t ldc, float* scales,
                             cudaStream_t s) {
+    constexpr int kRun = 8 * PX * 4 * 32 * 16;  // one run of all warps
+    constexpr int kMost = PX == 2 ? 96 * 1024 / kRun : 0;  // two CTAs per SM
+    const int kept = std::min((K - 1) / 256, kMost);
+    static bool configured[64] = {};
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess && (device >= 64 || !configured[device])) {
+        e = cudaFuncSetAttribute(quantise_planes_kernel<PX>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost * kRun);
+        if (e == cudaSuccess && device < 64) configured[device] = true;
+    }
+    if (e != cudaSuccess) return e;
     return launch_pdl(quantise_planes_kernel<PX>, dim3(static_cast<unsigned>((rows + 32 * PX - 1) / (32 * PX))),
-                      dim3(256), 0, s, static_cast<const __half*>(x), rows, K, hw, codes, ldc, scales);
+                      dim3(256), static_cast<size_t>(kept) * kRun, s, static_cast<const __half*>(x), rows, K, hw, codes, ldc,
+                      scales, kept);
 }
 
 // par of ProductArgs from the weight rows' scales and the bias (may be null).

@@ -19,7 +19,10 @@ namespace dnb {
 int linear8_map(CUtensorMap* m, CUtensorMapDataType type, int esz, const void* base, int64_t cols, int64_t rows,
                 int64_t ld, int box_cols, int box_rows);
 
-PFN_cuTensorMapEncodeTiled_v12000 linear8_encoder();
+// The same over FP16 planes [images][channels][pixels], boxes of box_ch x
+// box_px pixels of one image (64 or 32, swizzled by their 128 or 64 bytes).
+int linear8_planes_map(CUtensorMap* m, const void* base, int64_t pixels, int64_t channels, int64_t images, int box_px,
+                       int box_ch);
 
 // CTAs per SM of a kernel that allocates tmem_cols TMEM columns: by registers
 // (allocated in eights a thread), shared memory (228 KB, 1 KB a CTA reserved)
@@ -69,6 +72,26 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, int (&r)[32]) {
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
           "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void stmatrix4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
+                 "r"(d)
+                 : "memory");
+}
+// 16 lanes x 32 columns: r[4 k + i] is (lane t / 4 + 8 (i / 2), column 8 k + 2 (t % 4) + i % 2).
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, int (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
 }
 

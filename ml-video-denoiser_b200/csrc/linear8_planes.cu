@@ -50,26 +50,6 @@ struct Shape {
     static int smem(bool gate) { return 1024 + 2 * kIn + kA + kB + (gate ? NT / 2 : NT) * 256; }
 };
 
-__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
-}
-__device__ __forceinline__ void stmatrix4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
-                 "r"(d)
-                 : "memory");
-}
-// 16 lanes x 32 columns: r[4 k + i] is (lane t / 4 + 8 (i / 2), column 8 k + 2 (t % 4) + i % 2).
-__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, int (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
-}
-
 template <int KP, int NT>
 __global__ void __launch_bounds__(kThreads) product_planes_kernel(const __grid_constant__ PlanesArgs g,
                                                                   const __grid_constant__ CUtensorMap in_map,
@@ -273,35 +253,18 @@ __global__ void __launch_bounds__(kThreads) product_planes_kernel(const __grid_c
     if (warp == 0) tmem_dealloc(tmem, kCols);
 }
 
-// Planes [images][channels][pixels] with boxes of 64 pixels x box_ch. (Output
-// boxes of 32 pixels, one per warp, cost 157 us instead of 93 at 32 -> 64
-// channels, 1088x1920: half lines, and twice the address translations where
-// the planes are megabytes apart. 16 images of 272x480, the same bytes in
-// nearer planes, take 78 us.)
-int planes_map(CUtensorMap* m, const void* base, int64_t pixels, int64_t channels, int64_t images, int box_ch) {
-    auto fn = linear8_encoder();
-    if (!fn) return dn_fail(DN_ERR_CUDA, "linear8: cuTensorMapEncodeTiled unavailable");
-    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(pixels), static_cast<cuuint64_t>(channels),
-                                static_cast<cuuint64_t>(images)};
-    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(pixels) * 2, static_cast<cuuint64_t>(pixels * channels) * 2};
-    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_ch), 1};
-    const cuuint32_t estr[3] = {1, 1, 1};
-    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS)
-        return dn_fail_str(DN_ERR_CUDA, "linear8: cuTensorMapEncodeTiled failed (" + std::to_string(r) + ")");
-    return DN_OK;
-}
-
 template <int KP, int NT>
 int run(PlanesArgs& g, const void* x, int sms, cudaStream_t s) {
     using S = Shape<KP, NT>;
     const ProductArgs& p = g.p;
     const int64_t images = p.rows / p.ldo;
     CUtensorMap in{}, out{};
-    DN_TRY(planes_map(&in, x, p.ldo, p.seg_c, images, KP));
-    DN_TRY(planes_map(&out, p.out, p.ldo, p.n_out, images, p.gate ? NT / 2 : NT));
+    DN_TRY(linear8_planes_map(&in, x, p.ldo, p.seg_c, images, 64, KP));
+    // (Output boxes of 32 pixels, one per warp, cost 157 us instead of 93 at 32 ->
+    // 64 channels, 1088x1920: half lines, and twice the address translations
+    // where the planes are megabytes apart. 16 images of 272x480, the same bytes
+    // in nearer planes, take 78 us.)
+    DN_TRY(linear8_planes_map(&out, p.out, p.ldo, p.n_out, images, 64, p.gate ? NT / 2 : NT));
     static int resident[2][64] = {};
     const int smem = S::smem(p.gate);
     int per_sm = 0;

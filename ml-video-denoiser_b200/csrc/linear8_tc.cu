@@ -70,6 +70,7 @@ struct TcArgs {
     int units;           // K chunks of a stage: 1, or (resident weight) all of a tile's
     int seg_full;        // accumulators are handed over one by one, not a tile's together
     int pairs;           // direct stores of FP16 rows: pairs are 4-byte aligned
+    int tma_planes;      // planes by TMA: boxes of 32 channels x 32 pixels of one image
 };
 
 // 32 columns from c on, (scale, bias) from par.
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
         fence_mbar_init();
         prefetch_tmap(&maps.a);
         prefetch_tmap(&maps.b);
-        if (g.tma_out) prefetch_tmap(&maps.out);
+        if (g.tma_out || g.tma_planes) prefetch_tmap(&maps.out);
     }
     tc_fence_before();
     __syncthreads();
@@ -306,6 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
                 next[t] = t < p.segs && tile < tiles && row < p.rows ? __ldg(p.as + p.arow[t] + row) : 0.f;
         };
         int q = 0, n = 0;
+        uint32_t boxes = 0;
         load_scales(blockIdx.x);
         for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
             const float s = next[0];
@@ -383,6 +385,67 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
                     for (int i = 0; i < 32; ++i) y[i] = static_cast<float>(a[i]) * s;
                     finish32(par, y);
                 };
+                if constexpr (sizeof(T) == 2) {
+                    if (g.tma_planes) {
+                        // As in linear8_planes.cu: lane t has, of pixels 8 i + t / 4,
+                        // channels 8 k + 2 (t % 4) and the next.
+                        const int j4 = lane & 3, px = lane >> 2;
+                        float sp[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sp[i] = __shfl_sync(0xffffffffu, s, 8 * i + px);
+                        auto block = [&](int c, const float2* par, float2 (&y)[4][4]) {
+                            int a[2][16];
+                            tmem_ld_16x32(acc + c, a[0]);
+                            tmem_ld_16x32(acc + (16u << 16) + c, a[1]);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const float4 w = __ldg(reinterpret_cast<const float4*>(par + 8 * k + 2 * j4));
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const int* v = &a[i >> 1][4 * k + 2 * (i & 1)];
+                                    const float2 t = ffma2(make_float2(static_cast<float>(v[0]), static_cast<float>(v[1])),
+                                                           make_float2(sp[i], sp[i]), make_float2(0.f, 0.f));
+                                    y[k][i] = ffma2(t, make_float2(w.x, w.z), make_float2(w.y, w.w));
+                                }
+                            }
+                        };
+                        const int64_t image = m0 / p.ldo;
+                        for (int c = 0, u = n & 1; c < out_cols; c += 32, ++u) {
+                            if ((u & 1) != group || n0 + c >= p.n_out) continue;
+                            float2 y[4][4];
+                            block(c, p.par + n0 + c, y);
+                            if (p.gate) {
+                                float2 z[4][4];
+                                block(half + c, p.par + p.npad + n0 + c, z);
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) y[k][i].x *= z[k][i].x, y[k][i].y *= z[k][i].y;
+                            }
+                            // Two boxes take turns in the staging tile.
+                            uint8_t* box = stg + (boxes++ & 1) * (32 * 64);
+                            if (lane == 0) bulk_wait_read1();
+                            __syncwarp();
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                stmatrix4_trans(smem_u32(box) + sw_offset(8 * k + (lane & 7), lane >> 3, 64),
+                                                pack_half2(y[k][0].x, y[k][0].y), pack_half2(y[k][1].x, y[k][1].y),
+                                                pack_half2(y[k][2].x, y[k][2].y), pack_half2(y[k][3].x, y[k][3].y));
+                            fence_async_smem();
+                            __syncwarp();
+                            if (lane == 0) {
+                                if (m0 < p.rows)
+                                    tma_store_3d(&maps.out, static_cast<int>(m0 - image * p.ldo), n0 + c,
+                                                 static_cast<int>(image), box);
+                                bulk_commit();
+                            }
+                        }
+                        acc_done(q);
+                        ++q;
+                        continue;
+                    }
+                }
                 // The two groups of four warps take the tile's runs of `unit`
                 // columns in turn.
                 for (int c0 = 0, u = n & 1; c0 < out_cols; c0 += g.unit, ++u) {
@@ -408,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
                 ++q;
             }
         }
-        if (g.tma_out && lane == 0) bulk_wait_read0();
+        if ((g.tma_out || g.tma_planes) && lane == 0) bulk_wait_read0();
     }
     tc_fence_before();
     __syncthreads();
@@ -453,6 +516,10 @@ int run(TcArgs& g, int sms, cudaStream_t s) {
     if (g.tma_out)
         DN_TRY(linear8_map(&maps.out, sizeof(T) == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
                            sizeof(T), p.out, p.n_out, p.rows, p.ldo, g.unit, 32));
+    // A warp's 32 pixels are of one image, and the planes are what TMA can address.
+    g.tma_planes = p.planes && sizeof(T) == 2 && !SEG && reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo % 8 == 0 &&
+                   (p.ldo % 32 == 0 || p.rows == p.ldo);
+    if (g.tma_planes) DN_TRY(linear8_planes_map(&maps.out, p.out, p.ldo, p.n_out, p.rows / p.ldo, 32, 32));
     const int64_t tiles = static_cast<int64_t>(g.m_tiles) * g.n_tiles;
     if (tiles >= (1LL << 30)) return dn_fail(DN_ERR_UNSUPPORTED, "linear8: the product has 2^30 tiles or more");
     static bool configured[64] = {};  // per device
@@ -501,8 +568,6 @@ int run_type(TcArgs& g, int sms, cudaStream_t s) {
 
 }  // namespace
 
-PFN_cuTensorMapEncodeTiled_v12000 linear8_encoder() { return tensor_map_encoder(); }
-
 int linear8_map(CUtensorMap* m, CUtensorMapDataType type, int esz, const void* base, int64_t cols, int64_t rows,
                 int64_t ld, int box_cols, int box_rows) {
     auto fn = tensor_map_encoder();
@@ -517,6 +582,24 @@ int linear8_map(CUtensorMap* m, CUtensorMapDataType type, int esz, const void* b
                                                 : CU_TENSOR_MAP_SWIZZLE_32B;
     const CUresult r = fn(m, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           swz, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return dn_fail_str(DN_ERR_CUDA, "linear8: cuTensorMapEncodeTiled failed (" + std::to_string(r) + ")");
+    return DN_OK;
+}
+
+int linear8_planes_map(CUtensorMap* m, const void* base, int64_t pixels, int64_t channels, int64_t images, int box_px,
+                       int box_ch) {
+    auto fn = tensor_map_encoder();
+    if (!fn) return dn_fail(DN_ERR_CUDA, "linear8: cuTensorMapEncodeTiled unavailable");
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(pixels), static_cast<cuuint64_t>(channels),
+                                static_cast<cuuint64_t>(images)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(pixels) * 2, static_cast<cuuint64_t>(pixels * channels) * 2};
+    const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_px), static_cast<cuuint32_t>(box_ch), 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          box_px == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
         return dn_fail_str(DN_ERR_CUDA, "linear8: cuTensorMapEncodeTiled failed (" + std::to_string(r) + ")");
     return DN_OK;

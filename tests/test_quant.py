@@ -431,7 +431,9 @@ def test_many_tiles(Q, rows, k, n, gate, y_type):
                                            (1, 256, 24, 32, 256), (2, 300, 13, 11, 520), (1, 128, 64, 64, 32),
                                            (2, 16, 1, 129, 8), (1, 512, 8, 16, 64), (5, 48, 3, 5, 96),
                                            (3, 17, 8, 9, 34), (2, 3, 2, 4, 7), (1, 100, 24, 40, 250), (4, 65, 1, 136, 130),
-                                           (1, 32, 40, 200, 64), (2, 128, 30, 44, 256), (1, 96, 16, 21, 20), (700, 8, 1, 8, 12)])
+                                           (1, 32, 40, 200, 64), (2, 128, 30, 44, 256), (1, 96, 16, 21, 20), (700, 8, 1, 8, 12),
+                                           (1, 700, 20, 30, 300), (3, 260, 8, 12, 290), (2, 1300, 4, 24, 40), (2, 264, 3, 24, 520),
+                                           (1, 2000, 1, 77, 33), (1, 130, 48, 100, 258), (2, 4200, 2, 16, 12)])
 @pytest.mark.parametrize("gate", [False, True])
 def test_planes(Q, n_img, k, h, w, n, gate):
     if gate and n % 2:
