@@ -82,8 +82,8 @@ typedef struct dn_linear8 dn_linear8;
 /* Weight (Cout, Cin) or (Cout, Cin, 1, 1) and optional bias (Cout) from the
  * store, quantised onto `device`. DN_ERR_NOT_FOUND for a missing key,
  * DN_ERR_FORMAT for another shape, DN_ERR_INVALID_ARG for an odd Cout with
- * gate or a Cin that segments does not divide, DN_ERR_UNSUPPORTED for
- * Cin > 131072 (the int32 sum) or segments > 8. */
+ * gate, a Cin that segments does not divide or a device that is not there,
+ * DN_ERR_UNSUPPORTED for Cin > 131072 (the int32 sum) or segments > 8. */
 int dn_linear8_create(const dn_weights* store, const char* weight_name, const char* bias_name, int gate, int segments,
                       int device, dn_linear8** out);
 /* The same from device memory of `device`: weight [cout][cin] with row stride

@@ -204,6 +204,16 @@ int check_shape(int64_t cout, int64_t cin, int gate, int segments) {
     return DN_OK;
 }
 
+int check_device(int device) {
+    int count = 0;
+    const cudaError_t e = cudaGetDeviceCount(&count);
+    if (e != cudaSuccess) return dn_cuda_fail(e, "dn_linear8_create: cudaGetDeviceCount");
+    if (device < 0 || device >= count)
+        return dn_fail_str(DN_ERR_INVALID_ARG, "dn_linear8_create: CUDA device " + std::to_string(device) +
+                                                   " not available (" + std::to_string(count) + " devices found)");
+    return DN_OK;
+}
+
 // The layer's own copy of the weight, quantised; the current device is the layer's.
 cudaError_t lay_out(dn_linear8* L, const void* weight, int dtype, int64_t ldw, const void* bias, cudaStream_t s, int& rc) {
     const int64_t codes = round16(L->cout * L->ldw);
@@ -329,6 +339,7 @@ int dn_linear8_create(const dn_weights* store, const char* weight_name, const ch
         if (!(sh.size() == 2 || (sh.size() == 4 && sh[2] == 1 && sh[3] == 1)))
             return dn_fail(DN_ERR_FORMAT, "dn_linear8_create: weight must be (Cout, Cin) or (Cout, Cin, 1, 1)");
         DN_TRY(check_shape(sh[0], sh[1], gate, segments));
+        DN_TRY(check_device(device));
         const int cout = static_cast<int>(sh[0]), cin = static_cast<int>(sh[1]);
         const std::vector<float> w = hw.to_f32(weight_name);
         std::vector<float> b;
@@ -360,6 +371,7 @@ int dn_linear8_create_device(const void* weight, int dtype, int64_t ldw, const v
     DN_TRY(check_matrix(weight, dtype, cout, ldw, cin, "dn_linear8_create_device"));
     if (!aligned_to(bias, dtype == 1 ? 2 : 4))
         return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_create_device: misaligned bias");
+    DN_TRY(check_device(device));
     DeviceScope scope(device);
     return create(weight, dtype, ldw, bias, cout, cin, gate, segments, device, static_cast<cudaStream_t>(stream), out);
 }

@@ -564,6 +564,17 @@ def test_layers_from_a_store_and_from_tensors_are_the_same(pkg, Q, tmp_path):
 
 
 @gpu
+def test_layers_of_a_device_that_is_not_there_are_refused(pkg, tmp_path):
+    store = store_of(pkg, tmp_path, {"b.weight": np.ones((4, 16), np.float16)})
+    w, lib, h = torch.ones(4, 16, dtype=torch.float16, device="cuda"), pkg.lib(), ctypes.c_void_p()
+    for device in (-1, torch.cuda.device_count()):
+        assert lib.dn_linear8_create(store._h, b"b.weight", None, 0, 1, device, ctypes.byref(h)) == pkg.DN_ERR_INVALID_ARG
+        assert lib.dn_linear8_create_device(w.data_ptr(), 1, 16, None, 4, 16, 0, 1, device, None,
+                                            ctypes.byref(h)) == pkg.DN_ERR_INVALID_ARG
+    assert h.value is None and torch.cuda.current_device() == 0
+
+
+@gpu
 def test_calls_refuse(pkg, Q):
     h = torch.float16
     layer = Q.Linear8.from_tensors(torch.ones(6, 32, dtype=h, device="cuda"))
