@@ -339,7 +339,6 @@ int dn_linear8_create(const dn_weights* store, const char* weight_name, const ch
         if (!(sh.size() == 2 || (sh.size() == 4 && sh[2] == 1 && sh[3] == 1)))
             return dn_fail(DN_ERR_FORMAT, "dn_linear8_create: weight must be (Cout, Cin) or (Cout, Cin, 1, 1)");
         DN_TRY(check_shape(sh[0], sh[1], gate, segments));
-        DN_TRY(check_device(device));
         const int cout = static_cast<int>(sh[0]), cin = static_cast<int>(sh[1]);
         const std::vector<float> w = hw.to_f32(weight_name);
         std::vector<float> b;
@@ -347,6 +346,7 @@ int dn_linear8_create(const dn_weights* store, const char* weight_name, const ch
             b = hw.to_f32(bias_name);
             if (static_cast<int64_t>(b.size()) != cout) return dn_fail(DN_ERR_FORMAT, "dn_linear8_create: bias size");
         }
+        DN_TRY(check_device(device));
         DeviceScope scope(device);
         float* dev = nullptr;
         const size_t nw = w.size() * 4, nb = b.size() * 4;
