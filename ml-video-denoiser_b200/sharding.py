@@ -122,10 +122,11 @@ def denoise_streams(model, clips, num_frames: int, bits: int = 8, store=None, st
     takes them.
 
     The model's T cache slots hold one window; the encoded frames of all clips'
-    windows wait in a ``quant.FrameStore`` in 8 (or 4) bits (`store`: one with
-    T entries per clip, or made here), so that every frame is encoded once and
-    not T times per output. Every frame goes through the store, one clip's too:
-    what a clip's outputs are does not depend on the others.
+    windows wait in a ``quant.FrameStore`` in 8 (or 4) bits (`store`: one of
+    this model and frame size with T entries per clip, or made here), so that
+    every frame is encoded once and not T times per output. Every frame goes
+    through the store, one clip's too: what a clip's outputs are does not depend
+    on the others.
 
     Returns [(clip, frame index, output)]; ``on_frame(clip, i, y)``, when given,
     is called after each output."""
@@ -145,9 +146,15 @@ def denoise_streams(model, clips, num_frames: int, bits: int = 8, store=None, st
                 if held[k][s] != f:
                     x = frames(f).unsqueeze(0).contiguous()
                     if store is None:
+                        import torch
+
                         from .quant import FrameStore
 
-                        store = FrameStore(model, x.shape[2], x.shape[3], len(clips) * T, bits=bits)
+                        with torch.cuda.stream(stream):  # its zeros are written before a frame is parked
+                            store = FrameStore(model, x.shape[2], x.shape[3], len(clips) * T, bits=bits)
+                    if store.model is not model or (store.h, store.w) != tuple(x.shape[2:]):
+                        raise ValueError(f"the store holds {store.h}x{store.w} frames of its model, clip {k} has "
+                                         f"{x.shape[2]}x{x.shape[3]}")
                     model.encode_frame(x, s, stream=stream)
                     store.park(s, entry, stream=stream)
                     held[k][s], in_slot[s] = f, None

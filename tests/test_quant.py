@@ -636,8 +636,8 @@ class FakeModel:
 class FakeStore:
     """Adds a quarter to what it holds, so that a frame past it shows."""
 
-    def __init__(self, model):
-        self.model, self.held = model, {}
+    def __init__(self, model, h=2, w=2):
+        self.model, self.held, self.h, self.w = model, {}, h, w
 
     def park(self, slot, entry, stream=None):
         self.held[entry] = self.model.slots[slot] + 0.25
@@ -663,6 +663,11 @@ def test_streams_served_in_turn(pkg, T):
     with pytest.raises(ValueError):
         S.denoise_streams(m, clips, 4)
     assert S.denoise_streams(m, [], T) == []
+    for store in (FakeStore(m, 2, 4), FakeStore(FakeModel(T))):
+        with pytest.raises(ValueError):
+            S.denoise_streams(m, clips, T, store=store)
+    with pytest.raises(ValueError):
+        S.denoise_streams(m, clips + [(lambda f: torch.zeros(3, 2, 4), 2)], T, store=FakeStore(m))
 
 
 def small_temporal(pkg, tmp_path, kind, T):
@@ -719,6 +724,25 @@ def test_streams_through_the_frame_store(pkg, Q, tmp_path, kind, T, bits):
         with pytest.raises(pkg.InvalidArgumentError):
             bad()
     assert store.bytes < sum(r.nbytes for r in raw) * 2
+
+
+@gpu
+def test_streams_on_a_stream_of_their_own(pkg, Q, tmp_path):
+    """The store is made on the stream it is used on: what the current stream
+    does later does not reach it."""
+    S = importlib.import_module(pkg.__name__ + ".sharding")
+    m = small_temporal(pkg, tmp_path, "py", 3)
+    rng = np.random.default_rng(7)
+    clips = [[dev(rng.uniform(0, 1, (3, 30, 42)).astype(np.float16)) for _ in range(4)] for _ in range(2)]
+    take = [(lambda f, c=c: c[f], 4) for c in clips]
+    want = [y.clone() for _, _, y in S.denoise_streams(m, take, 3)]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    torch.cuda._sleep(20_000_000)
+    got = S.denoise_streams(m, take, 3, stream=side)
+    torch.cuda.synchronize()
+    for (k, i, y), w in zip(got, want):
+        assert torch.equal(y, w), (k, i)
 
 
 # ---------------------------------------------------------------------------------------------------------------------
