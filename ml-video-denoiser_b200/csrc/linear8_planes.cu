@@ -1,5 +1,5 @@
 // The 8-bit product over NCHW planes of narrow layers (Cin <= 128, Cout <= 256)
-// whose planes TMA can address (H * W a multiple of 8, 16-byte aligned): one
+// whose planes TMA can address (H * W a multiple of 8, 32 or more; 16-byte aligned): one
 // pass, bound by HBM (2 Cin + 2 Cout bytes a pixel).
 //
 // Planes are channel-major and the operand of the MMA is pixel-major. The
@@ -123,6 +123,7 @@ __global__ void __launch_bounds__(kThreads) product_planes_kernel(const __grid_c
         if (static_cast<int>(blockIdx.x) < g.tiles) load(blockIdx.x, 0);
         if (static_cast<int>(blockIdx.x + gridDim.x) < g.tiles) load(blockIdx.x + gridDim.x, 1);
     }
+    int issued = static_cast<int>(blockIdx.x + gridDim.x) < g.tiles ? 2 : 1;  // loads, for the lane that issues them
     const uint64_t ad0 = sdesc_kmajor_sw(smem_u32(sa), KP), bd0 = sdesc_kmajor_sw(smem_u32(sb), KP);
     const int steps = (p.seg_c + 31) / 32;
     const int j4 = lane & 3, px = lane >> 2;  // a lane's channel pair and pixel of 8
@@ -185,7 +186,10 @@ __global__ void __launch_bounds__(kThreads) product_planes_kernel(const __grid_c
                     if (k < steps) mma_s8(tmem, ad0 + 2 * k, bd0 + 2 * k, idesc_s8(kRows, NT), k > 0 ? 1u : 0u);
                 mma_commit(&bar);
                 const int64_t next = static_cast<int64_t>(tile) + 2 * static_cast<int64_t>(gridDim.x);
-                if (next < g.tiles) load(static_cast<int>(next), b);
+                if (next < g.tiles && !s_abort) {
+                    load(static_cast<int>(next), b);
+                    ++issued;
+                }
             }
             __syncwarp();
         }
@@ -250,7 +254,13 @@ __global__ void __launch_bounds__(kThreads) product_planes_kernel(const __grid_c
     if (issues) bulk_wait_read0();
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) tmem_dealloc(tmem, kCols);
+    if (warp == 0) {
+        // After a wait that ran out: the loads in flight land before the CTA leaves.
+        if (elect_one() && s_abort)
+            for (int k = max(0, issued - 2); k < issued; ++k) mbar_wait(&bar_in[k & 1], (k >> 1) & 1, 100000000ull);
+        __syncwarp();
+        tmem_dealloc(tmem, kCols);
+    }
 }
 
 template <int KP, int NT>
@@ -288,7 +298,10 @@ int run_nt(PlanesArgs& g, const void* x, int sms, cudaStream_t s) {
 }  // namespace
 
 bool product_planes_takes(const ProductArgs& a, const void* x) {
-    return a.planes && fused_width(a) <= 256 && a.segs == 1 && a.seg_c <= 128 && a.ldo % 8 == 0 &&
+    // A tile is of one image, so planes of a few pixels fill it badly (522240
+    // pixels, 64 -> 64: 166 us in planes of 16 and 86 of 32; tiles across images
+    // take 112 us of any).
+    return a.planes && fused_width(a) <= 256 && a.segs == 1 && a.seg_c <= 128 && a.ldo % 8 == 0 && a.ldo >= 32 &&
            reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
 }
 
