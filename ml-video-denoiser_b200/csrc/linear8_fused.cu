@@ -57,7 +57,6 @@ struct Shape {
     static constexpr int kVecs = PLANES ? SG : (kRows / kWarps) * SG / 32;  // 8-value vectors of a lane
     static constexpr int kBytesK = SG <= 4 ? 32 : SG * 8;                   // bytes of an operand row
     static constexpr int kSpan = kBytesK < 128 ? kBytesK : 128;             // its swizzle span
-    static constexpr int kSubs = kBytesK / kSpan;
     static constexpr int kA = kRows * kBytesK, kB = NT * kBytesK;
     static constexpr int kStg = kWarps * 32 * 128;
     // The tile's tokens as they came, where they are loaded as one run, come
