@@ -34,7 +34,13 @@ extern "C" {
  * ld_codes bytes (8 bits: one code a byte; 4 bits: two, the even column in
  * the low half), and scales [capacity][cols / group]. `group` divides cols;
  * 0 = cols (one scale a row). Rows are counted in 64 bits, so a cache may
- * exceed 2^32 bytes; capacity < 2^31.
+ * exceed 2^32 bytes; capacity < 2^31. All `capacity` rows have their ld_codes
+ * bytes; those behind a row's codes are not written. Any alignment is right;
+ * `codes` and ld_codes multiples of 16 are fastest.
+ *
+ * The launchers run on the current device, which `stream` and the tensors
+ * belong to. Calls that may overlap must not write what another one reads or
+ * writes.
  *
  * A row number outside [0, capacity): negative ones are skipped in silence
  * (padding); others are skipped too and set *err_dev (a device word, may be
@@ -50,7 +56,8 @@ int dn_launch_cache_write(const void* x, int dtype, int64_t ldx, int64_t rows, i
                           int group, uint32_t* err_dev, void* stream);
 
 /* Read back rows: out row i (row stride ldo elements) = cache row slots[i],
- * or row0 + i where slots is NULL. Rows of skipped slots stay as they were. */
+ * or row0 + i where slots is NULL. Rows of skipped slots stay as they were, and
+ * so does what lies between rows. `out` must not overlap the cache. */
 int dn_launch_cache_read_rows(const void* codes, int64_t ld_codes, const float* scales, int64_t capacity, int cols,
                               int bits, int group, const int64_t* slots, int64_t row0, int64_t rows, void* out,
                               int dtype, int64_t ldo, uint32_t* err_dev, void* stream);

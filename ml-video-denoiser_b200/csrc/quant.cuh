@@ -68,6 +68,20 @@ struct QuantOf<__half> {
             if (i < n) w[i >> 1] |= static_cast<uint32_t>(__half_as_ushort(p[i])) << ((i & 1) * 16);
         return Vec{make_uint4(w[0], w[1], w[2], w[3])};
     }
+    __device__ static __forceinline__ Vec load_local(const __half (&h)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            w[i] = static_cast<uint32_t>(__half_as_ushort(h[2 * i])) | static_cast<uint32_t>(__half_as_ushort(h[2 * i + 1])) << 16;
+        return Vec{make_uint4(w[0], w[1], w[2], w[3])};
+    }
+    __device__ static __forceinline__ Vec only(Vec x, int lo, int hi) {  // elements outside [lo, hi) as zeros
+        uint32_t w[4] = {x.v.x, x.v.y, x.v.z, x.v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            w[i] &= (2 * i >= lo && 2 * i < hi ? 0xffffu : 0u) | (2 * i + 1 >= lo && 2 * i + 1 < hi ? 0xffff0000u : 0u);
+        return Vec{make_uint4(w[0], w[1], w[2], w[3])};
+    }
     __device__ static __forceinline__ uint32_t mag(const Vec& x) {
         const uint32_t m = 0x7fff7fffu;
         const uint32_t a = umax16x2(umax16x2(x.v.x & m, x.v.y & m), umax16x2(x.v.z & m, x.v.w & m));
@@ -91,6 +105,16 @@ struct QuantOf<float> {
     }
     __device__ static __forceinline__ Vec load(const float* p) {
         return Vec{__ldg(reinterpret_cast<const float4*>(p)), __ldg(reinterpret_cast<const float4*>(p) + 1)};
+    }
+    __device__ static __forceinline__ Vec load_local(const float (&f)[8]) {
+        return Vec{make_float4(f[0], f[1], f[2], f[3]), make_float4(f[4], f[5], f[6], f[7])};
+    }
+    __device__ static __forceinline__ Vec only(const Vec& x, int lo, int hi) {
+        float f[8];
+        unpack(x, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = i >= lo && i < hi ? f[i] : 0.f;
+        return Vec{make_float4(f[0], f[1], f[2], f[3]), make_float4(f[4], f[5], f[6], f[7])};
     }
     __device__ static __forceinline__ Vec load_some(const float* p, int n) {
         float f[8];

@@ -6,9 +6,13 @@
 // lanes takes one group of a row, a lane 8 columns (a 16-byte load of FP16),
 // so the group's maximum is log2(SG) shuffles and nothing passes through
 // shared memory; every lane has the loads of several groups in flight before
-// it uses the first. Groups that do not fit this (a column count or an address
-// that is no multiple of the vectors) take a warp per group with scalar
-// accesses.
+// it uses the first. Rows that begin anywhere (odd column counts, strides and
+// addresses) move between their own boundaries and the vectors' in registers.
+// What is left (cache rows without the vectors' alignment, groups that are wide
+// and odd) takes a warp per group with scalar accesses.
+//
+// Measured: 2088960 x 32 FP16 written in 41 us and read back in 35 (both 206 MB;
+// out of L2 in part); five frames of 522240 x 64 read in 93 (512 MB).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -29,7 +33,8 @@ constexpr int kWarps = kThreads / 32;
 constexpr uint32_t kSiteWrite = 0x60, kSiteRead = 0x61;
 
 // Rows of one scattered write may name the same slot; the last one counts.
-//   up to kScanRows rows: every group looks through the later slots;
+//   up to kScanRows rows: every group looks through the later slots (64 x 1024:
+//   2.5 us, 3.7 with marks; 1024 x 1024: 8.0 and 4.6);
 //   more: the slot's scale words, which are about to be overwritten, first
 //   hold the largest row index that names the slot (two small kernels). An
 //   index below 2^23 is never the bit pattern of a scale (scales are >= 2^-126,
@@ -86,7 +91,29 @@ __global__ void __launch_bounds__(kThreads) mark_kernel(const WriteArgs a, int p
         atomicMax(m, static_cast<int>(row));
 }
 
-template <typename T, int BITS, int SG, int V, int U>
+// 8 values from a 16-byte boundary `at` on, those outside [0, n) as zeros; the
+// first of the row is value `first` of the 8. What a row's neighbours lie in is
+// read with it, but nothing before the first row or behind the last one.
+template <typename T>
+__device__ __forceinline__ typename QuantOf<T>::Vec load_span(const T* at, int first, int n, const T* begin, const T* end) {
+    using Q = QuantOf<T>;
+    const int lo = max(first, 0), hi = min(first + n, 8);
+    if (lo >= hi) return Q::zero();
+    if (at >= begin && at + 8 <= end) {
+        const typename Q::Vec v = Q::load(at);
+        return lo > 0 || hi < 8 ? Q::only(v, lo, hi) : v;
+    }
+    T x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = i >= lo && i < hi ? at[i] : T(0.f);
+    return Q::load_local(x);
+}
+
+// SHIFT: rows that begin anywhere. A lane's 8 values begin at the 16-byte
+// boundary at or before its place in the row, so that they are one load; the
+// codes move to their own boundary in registers, with the next lane's (1000000
+// x 25: 182 us a value at a time, 36 this way).
+template <typename T, int BITS, int SG, int V, int U, bool SHIFT>
 __global__ void __launch_bounds__(kThreads) write_vec_kernel(const WriteArgs a) {
     using Q = QuantOf<T>;
     pdl_trigger();
@@ -100,18 +127,28 @@ __global__ void __launch_bounds__(kThreads) write_vec_kernel(const WriteArgs a) 
     const int u0 = (blockIdx.x * kWarps + warp) * (kPer * U);
     if (u0 >= units) return;
     const T* x = static_cast<const T*>(a.p.x);
+    const T* x_end = x + (a.p.rows - 1) * a.p.ldx + static_cast<int64_t>(a.ngroups) * a.p.group;
     typename Q::Vec v[U][V];
-    int row[U], grp[U];
+    int row[U], grp[U], off[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
         const int u = u0 + i * kPer + sub;
         row[i] = a.ngroups == 1 ? u : static_cast<int>(static_cast<uint32_t>(u) / static_cast<uint32_t>(a.ngroups));
         grp[i] = a.ngroups == 1 ? 0 : u - row[i] * a.ngroups;
         const T* src = x + row[i] * a.p.ldx + grp[i] * a.p.group;
+        if constexpr (SHIFT) {
+            off[i] = static_cast<int>(reinterpret_cast<uintptr_t>(src) / sizeof(T) % (16 / sizeof(T)));
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const int c = l + k * SG;
-            v[i][k] = (u < units && c < nv) ? Q::load(src + c * 8) : Q::zero();
+            for (int k = 0; k < V; ++k) {
+                const int c = l + k * SG;
+                v[i][k] = u < units ? load_span<T>(src - off[i] + c * 8, off[i] - c * 8, a.p.group, x, x_end) : Q::zero();
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const int c = l + k * SG;
+                v[i][k] = (u < units && c < nv) ? Q::load(src + c * 8) : Q::zero();
+            }
         }
     }
 #pragma unroll
@@ -125,12 +162,52 @@ __global__ void __launch_bounds__(kThreads) write_vec_kernel(const WriteArgs a) 
         const GroupScale g = group_scale<T>(mag, qmax);
         const bool rare = __any_sync(0xffffffffu, g.rare);
         const int64_t slot = there ? slot_of(a, row[i]) : -1;
+        uint2 q[V];
+        if constexpr (SHIFT) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                q[k] = codes8<T>(v[i][k], g, rare);
+                if (BITS == 4) q[k].x = pack_nibbles(q[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                // The next lane's, the last lane's next being the first one's next vector.
+                uint2 b = l == 0 ? (k + 1 < V ? q[k + 1 < V ? k + 1 : k] : make_uint2(0, 0)) : q[k];
+                if (SG == 1) {
+                    // (a lane's own next vector)
+                } else {
+                    const int from = (lane & ~(SG - 1)) | ((l + 1) & (SG - 1));
+                    b.x = __shfl_sync(0xffffffffu, b.x, from);
+                    if (BITS == 8) b.y = __shfl_sync(0xffffffffu, b.y, from);
+                }
+                if (BITS == 4) {
+                    q[k].x = __funnelshift_r(q[k].x, b.x, 4 * off[i]);
+                } else {
+                    const bool far = off[i] >= 4;
+                    const uint32_t w0 = far ? q[k].y : q[k].x, w1 = far ? b.x : q[k].y, w2 = far ? b.y : b.x;
+                    q[k] = make_uint2(__funnelshift_r(w0, w1, 8 * (off[i] & 3)), __funnelshift_r(w1, w2, 8 * (off[i] & 3)));
+                }
+            }
+        }
         if (!wins<SG>(a, row[i], grp[i], slot, there)) continue;
         uint8_t* dst = a.p.codes + slot * a.p.ldc + static_cast<int64_t>(grp[i]) * (a.p.group * BITS / 8);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             const int c = l + k * SG;
-            if (c < nv) {
+            if constexpr (SHIFT) {
+                const int left = a.p.group - c * 8;
+                if (left >= 8) {
+                    if (BITS == 8)
+                        *reinterpret_cast<uint2*>(dst + c * 8) = q[k];
+                    else
+                        *reinterpret_cast<uint32_t*>(dst + c * 4) = q[k].x;
+                } else {  // the row's last bytes
+#pragma unroll
+                    for (int b = 0; b < BITS; ++b)
+                        if (b * 8 < left * BITS)
+                            dst[c * BITS + b] = static_cast<uint8_t>((b < 4 ? q[k].x : q[k].y) >> (8 * (b & 3)));
+                }
+            } else if (c < nv) {
                 const uint2 w = codes8<T>(v[i][k], g, rare);
                 if (BITS == 8)
                     *reinterpret_cast<uint2*>(dst + c * 8) = w;
@@ -315,9 +392,7 @@ __device__ __forceinline__ void store1(__half* p, float v) { *p = __float2half_r
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 
 // SG lanes per row, a lane W = 8 or 16 columns at a time (of one group), U rows
-// of each sub-warp in flight. 16 columns halve the work per row, which bounds
-// narrow rows (five frames of 522240 x 64: 105 us on the device, 107 with 8
-// columns; a kernel that only writes its 334 MB takes 88).
+// of each sub-warp in flight.
 template <typename T, int BITS, int SG, int U, int W>
 __global__ void __launch_bounds__(kThreads) read_vec_kernel(const ReadArgs a) {
     pdl_trigger();
@@ -378,6 +453,55 @@ __global__ void __launch_bounds__(kThreads) read_vec_kernel(const ReadArgs a) {
     }
 }
 
+// Rows of out that begin anywhere: a lane's 8 columns begin at the 16-byte
+// boundary at or before its place in the row, so that all but a row's ends are
+// 16-byte stores; their codes are cut from the words they lie in (1000000 x 25:
+// 121 us a value at a time, 38 this way). One scale a row.
+template <typename T, int BITS, int SG>
+__global__ void __launch_bounds__(kThreads) read_shift_kernel(const ReadArgs a) {
+    pdl_trigger();
+    pdl_wait();
+    constexpr int kPer = 32 / SG;
+    const int lane = threadIdx.x & 31;
+    const int b = blockIdx.y;
+    const int64_t n = sequence_rows(a, b);
+    const int64_t i = (static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5)) * kPer + lane / SG;
+    const int64_t src = source_row(a, b, i, n);
+    if (src < 0) return;
+    T* out = static_cast<T*>(a.out) + b * a.out_batch + i * a.ldo;
+    const int off = static_cast<int>(reinterpret_cast<uintptr_t>(out) / sizeof(T) % (16 / sizeof(T)));
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(a.codes + src * a.ldc);
+    const int words = (a.cols * BITS + 31) / 32;
+    const float s = a.scales[src];
+    const float2 s2 = make_float2(s, s), zero2 = make_float2(0.f, 0.f);
+    for (int c = lane % SG * 8 - off; c < a.cols; c += SG * 8) {
+        constexpr int kIn = 32 / BITS;  // codes of a word
+        const int first = c >= 0 ? c / kIn : -((kIn - 1 - c) / kIn);
+        const int shift = (c - first * kIn) * BITS;
+        auto word = [&](int k) { return first + k >= 0 && first + k < words ? __ldg(w + first + k) : 0u; };
+        float2 f[4];
+        if constexpr (BITS == 8) {
+            const uint32_t w0 = word(0), w1 = word(1), w2 = shift ? word(2) : 0u;
+            float2 lo[2], hi[2];
+            bytes_to_f(__funnelshift_r(w0, w1, shift), lo);
+            bytes_to_f(__funnelshift_r(w1, w2, shift), hi);
+            f[0] = lo[0], f[1] = lo[1], f[2] = hi[0], f[3] = hi[1];
+        } else {
+            const uint32_t w0 = word(0), w1 = shift ? word(1) : 0u;
+            nibbles_to_f(__funnelshift_r(w0, w1, shift), f);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[k] = ffma2(f[k], s2, zero2);
+        if (c >= 0 && c + 8 <= a.cols) {
+            store8(out + c, f);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (c + k >= 0 && c + k < a.cols) store1(out + c + k, k & 1 ? f[k >> 1].y : f[k >> 1].x);
+        }
+    }
+}
+
 // Any size and alignment: a warp takes U rows, lanes along the columns.
 template <typename T, int BITS, int U>
 __global__ void __launch_bounds__(kThreads) read_any_kernel(const ReadArgs a) {
@@ -420,12 +544,22 @@ int pow2_lanes(int nv) {
     return s;
 }
 
-template <typename T, int BITS, int SG, int V, int U>
+template <typename T, int BITS, bool SHIFT, int SG, int V, int U>
 cudaError_t write_run(const WriteArgs& a, cudaStream_t s) {
     const int64_t per = static_cast<int64_t>(kWarps) * (32 / SG) * U;
     const int64_t units = a.p.rows * a.ngroups;
-    return launch_pdl(write_vec_kernel<T, BITS, SG, V, U>, dim3(static_cast<unsigned>((units + per - 1) / per)),
+    return launch_pdl(write_vec_kernel<T, BITS, SG, V, U, SHIFT>, dim3(static_cast<unsigned>((units + per - 1) / per)),
                       dim3(kThreads), 0, s, a);
+}
+
+// Two groups in flight per sub-warp for long FP16 writes, where that still gives
+// every SM four CTAs (522240 x 64: 21.6 us, 22.6 with one; 1000 x 256: 1.9 and
+// 1.5). FP32 values are twice the bytes a lane: one (522240 x 64: 29.5, 31.0
+// with two).
+template <typename T, int BITS, bool SHIFT, int SG>
+cudaError_t write_groups(const WriteArgs& a, cudaStream_t s) {
+    const bool two = sizeof(T) == 2 && a.p.rows * a.ngroups >= 4 * 148 * kWarps * (32 / SG) * 2;
+    return two ? write_run<T, BITS, SHIFT, SG, 1, 2>(a, s) : write_run<T, BITS, SHIFT, SG, 1, 1>(a, s);
 }
 
 template <typename T, int KEEP, int U>
@@ -435,21 +569,27 @@ cudaError_t write_any(const WriteArgs& a, cudaStream_t s) {
                       s, a);
 }
 
-template <typename T, int BITS>
+// Vectors that 8-value pieces of a group may touch: SHIFT begins up to a vector early.
+template <typename T, bool SHIFT>
+int group_vecs(const WriteArgs& a) {
+    return (a.p.group + 7 + (SHIFT ? static_cast<int>(16 / sizeof(T)) - 1 : 0)) / 8;
+}
+
+template <typename T, int BITS, bool SHIFT>
 cudaError_t write_bits(const WriteArgs& a, cudaStream_t s) {
-    const int nv = a.p.group / 8;
+    const int nv = group_vecs<T, SHIFT>(a);
     switch (pow2_lanes(nv)) {
-        case 1: return write_run<T, BITS, 1, 1, 4>(a, s);
-        case 2: return write_run<T, BITS, 2, 1, 4>(a, s);
-        case 4: return write_run<T, BITS, 4, 1, 4>(a, s);
-        case 8: return write_run<T, BITS, 8, 1, 4>(a, s);
-        case 16: return write_run<T, BITS, 16, 1, 4>(a, s);
+        case 1: return write_groups<T, BITS, SHIFT, 1>(a, s);
+        case 2: return write_groups<T, BITS, SHIFT, 2>(a, s);
+        case 4: return write_groups<T, BITS, SHIFT, 4>(a, s);
+        case 8: return write_groups<T, BITS, SHIFT, 8>(a, s);
+        case 16: return write_groups<T, BITS, SHIFT, 16>(a, s);
         default: break;
     }
-    if (nv <= 32) return write_run<T, BITS, 32, 1, 4>(a, s);
-    if (nv <= 64) return write_run<T, BITS, 32, 2, 2>(a, s);
-    if (nv <= 128) return write_run<T, BITS, 32, 4, 1>(a, s);
-    if (nv <= 256) return write_run<T, BITS, 32, 8, 1>(a, s);
+    if (nv <= 32) return write_groups<T, BITS, SHIFT, 32>(a, s);
+    if (nv <= 64) return write_run<T, BITS, SHIFT, 32, 2, 1>(a, s);
+    if (nv <= 128) return write_run<T, BITS, SHIFT, 32, 4, 1>(a, s);
+    if (SHIFT || nv <= 256) return write_run<T, BITS, SHIFT, 32, 8, 1>(a, s);
     const dim3 grid(static_cast<unsigned>(a.p.rows * a.ngroups));
     if (nv <= 2 * kThreads) return launch_pdl(write_wide_kernel<T, BITS, 2>, grid, dim3(kThreads), 0, s, a);
     return launch_pdl(write_wide_kernel<T, BITS, 4>, grid, dim3(kThreads), 0, s, a);
@@ -459,9 +599,10 @@ template <typename T>
 cudaError_t write_type(const WriteArgs& a, cudaStream_t s) {
     const CacheWrite& p = a.p;
     // A vector of 8 codes has `bits` bytes.
-    const bool vec = p.group % 8 == 0 && aligned(p.x, 16) && p.ldx * sizeof(T) % 16 == 0 &&
-                     aligned(p.codes, p.bits) && p.ldc % p.bits == 0;
-    if (vec) return p.bits == 8 ? write_bits<T, 8>(a, s) : write_bits<T, 4>(a, s);
+    const bool codes = aligned(p.codes, p.bits) && p.ldc % p.bits == 0;
+    const bool rows = p.group % 8 == 0 && aligned(p.x, 16) && p.ldx * sizeof(T) % 16 == 0;
+    if (codes && rows) return p.bits == 8 ? write_bits<T, 8, false>(a, s) : write_bits<T, 4, false>(a, s);
+    if (codes && group_vecs<T, true>(a) <= 256) return p.bits == 8 ? write_bits<T, 8, true>(a, s) : write_bits<T, 4, true>(a, s);
     // 8 pairs a lane in registers: groups of one row, or pieces of several.
     if (p.group <= 64) return write_any<T, 1, 8>(a, s);
     if (p.group <= 256) return write_any<T, 4, 2>(a, s);
@@ -477,10 +618,11 @@ cudaError_t read_run(const ReadArgs& a, int batch, cudaStream_t s) {
 
 template <typename T, int BITS, int SG, int W>
 cudaError_t read_rows(const ReadArgs& a, int batch, cudaStream_t s) {
-    // Four rows in flight per sub-warp where that still gives every SM four
-    // CTAs; short reads spread over more warps instead.
-    const int64_t ctas = a.rows * batch / (kWarps * (32 / SG) * 4);
-    return ctas >= 4 * 148 ? read_run<T, BITS, SG, 4, W>(a, batch, s) : read_run<T, BITS, SG, 1, W>(a, batch, s);
+    // One row in flight per sub-warp: more CTAs hide more than more loads of one
+    // (five frames of 522240 x 64 to FP16: 93 us, 102 with four rows). Lanes of 8
+    // FP16 columns take two in long reads (1000000 x 24: 16.4, 18.5 with one).
+    const bool two = W == 8 && sizeof(T) == 2 && a.rows * batch >= 4 * 148 * kWarps * (32 / SG) * 2;
+    return two ? read_run<T, BITS, SG, 2, W>(a, batch, s) : read_run<T, BITS, SG, 1, W>(a, batch, s);
 }
 
 template <typename T, int BITS, int W>
@@ -495,18 +637,40 @@ cudaError_t read_width(const ReadArgs& a, int batch, cudaStream_t s) {
     }
 }
 
+// 16 columns a lane halve the work per FP16 row (five frames of 522240 x 64: 93
+// us, 96 with 8). FP32 rows take 8, so that a lane's stores stay closer (522240 x
+// 64: 37 us, 41 with 16; 168000 x 512 from 4 bits: 76 and 91).
 template <typename T, int BITS>
 cudaError_t read_bits(const ReadArgs& a, int batch, cudaStream_t s) {
+    if constexpr (sizeof(T) == 4) return read_width<T, BITS, 8>(a, batch, s);
     const bool wide = a.cols % 16 == 0 && a.group % 16 == 0 && aligned(a.codes, 2 * BITS) && a.ldc % (2 * BITS) == 0;
     return wide ? read_width<T, BITS, 16>(a, batch, s) : read_width<T, BITS, 8>(a, batch, s);
+}
+
+template <typename T, int BITS>
+cudaError_t read_shift(const ReadArgs& a, int batch, cudaStream_t s) {
+    auto run = [&](auto kernel, int sg) {
+        const int64_t per = static_cast<int64_t>(kWarps) * (32 / sg);
+        return launch_pdl(kernel, dim3(static_cast<unsigned>((a.rows + per - 1) / per), batch), dim3(kThreads), 0, s, a);
+    };
+    switch (pow2_lanes((a.cols + 6 + static_cast<int>(16 / sizeof(T))) / 8)) {
+        case 1: return run(read_shift_kernel<T, BITS, 1>, 1);
+        case 2: return run(read_shift_kernel<T, BITS, 2>, 2);
+        case 4: return run(read_shift_kernel<T, BITS, 4>, 4);
+        case 8: return run(read_shift_kernel<T, BITS, 8>, 8);
+        case 16: return run(read_shift_kernel<T, BITS, 16>, 16);
+        default: return run(read_shift_kernel<T, BITS, 32>, 32);
+    }
 }
 
 template <typename T>
 cudaError_t read_type(const ReadArgs& a, int batch, cudaStream_t s) {
     const bool vec = a.cols % 8 == 0 && a.group % 8 == 0 && aligned(a.codes, a.bits) && a.ldc % a.bits == 0 &&
                      aligned(a.out, 16) && a.ldo * sizeof(T) % 16 == 0 && a.out_batch * sizeof(T) % 16 == 0;
+    if (!vec && a.ngroups == 1 && aligned(a.codes, 4) && a.ldc % 4 == 0)
+        return a.bits == 8 ? read_shift<T, 8>(a, batch, s) : read_shift<T, 4>(a, batch, s);
     if (!vec) {
-        constexpr int kU = 8;
+        constexpr int kU = 2;
         const dim3 grid(static_cast<unsigned>((a.rows + kWarps * kU - 1) / (kWarps * kU)), batch);
         return a.bits == 8 ? launch_pdl(read_any_kernel<T, 8, kU>, grid, dim3(kThreads), 0, s, a)
                            : launch_pdl(read_any_kernel<T, 4, kU>, grid, dim3(kThreads), 0, s, a);

@@ -124,8 +124,8 @@ class RowCache:
         return slots.data_ptr()
 
     def write(self, x, slots=None, row0: int = 0, stream=None) -> None:
-        """Rows x (rows, cols), FP16 or FP32, any row stride, into the cache
-        rows ``slots`` (int64 CUDA tensor), or ``row0``, ``row0 + 1``, ...
+        """Rows x (rows, cols), FP16 or FP32, any row stride that holds a row,
+        into the cache rows ``slots`` (int64 CUDA tensor), or ``row0``, ``row0 + 1``, ...
         Rows with a negative slot are skipped; a slot at or behind the capacity
         is skipped and reported by ``sync``. Of rows with the same slot the
         last one is held."""
@@ -325,8 +325,8 @@ class Linear8:
         return t.data_ptr(), need, t
 
     def forward(self, x, out=None, out_dtype=None, stream=None):
-        """Token rows x (rows, in_channels), FP16 or FP32, any row stride ->
-        (rows, out_channels) in ``out_dtype`` (default: x's) or into ``out``."""
+        """Token rows x (rows, in_channels), FP16 or FP32, any row stride that
+        holds a row -> (rows, out_channels) in ``out_dtype`` (default: x's) or into ``out``."""
         if _elsewhere(self.device, stream):
             with _on(self.device, stream):
                 return self.forward(x, out, out_dtype)

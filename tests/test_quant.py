@@ -245,6 +245,40 @@ def test_rows_of_zeros_extremes_and_values_that_are_not_finite(Q, dtype, cols):
 
 
 @gpu
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("rows,cols,gap", [(1, 1, 0), (5, 2, 0), (40, 7, 0), (33, 9, 1), (50, 17, 0), (20, 25, 3),
+                                           (300, 25, 0), (9, 63, 0), (9, 65, 7), (7, 250, 0), (5, 255, 1), (5, 257, 0),
+                                           (4, 333, 2), (3, 505, 0), (3, 1001, 0), (2, 2034, 1), (2, 2035, 0),
+                                           (2, 2041, 0), (2, 2047, 0), (20000, 11, 0), (12000, 40, 1)])
+def test_rows_that_begin_anywhere(Q, bits, dtype, rows, cols, gap):
+    """Rows at every place within 16 bytes: nothing of their neighbours (NaN) is
+    taken in, and no byte beside a row's own is written, in the cache or in out."""
+    rng = np.random.default_rng(rows + cols)
+    x = rows_of(rng, rows, cols, dtype)
+    q, s = qo.quantise(x, bits)
+    ld, pad = cols + gap, 16
+    t = torch.float16 if dtype == np.float16 else torch.float32
+    for first in (range(8) if rows < 100 else (0, 3)):
+        flat = torch.full((pad + rows * ld + 2 * pad,), float("nan"), dtype=t, device="cuda")
+        v = flat[pad + first:].as_strided((rows, cols), (ld, 1))
+        v.copy_(dev(x))
+        cache = Q.RowCache(1, rows + 2, cols, bits=bits)
+        cache.codes.fill_(0xa5)
+        cache.scales.fill_(-3.0)
+        cache.write(v, row0=1)
+        assert_held(cache, slice(1, rows + 1), q, s, bits)
+        codes = host(cache.codes)
+        assert (codes[:, bytes_of(cols, bits):] == 0xa5).all() and (codes[[0, -1]] == 0xa5).all()
+        flat.fill_(7.0)
+        cache.read_rows(row0=1, rows=rows, out=v)
+        assert_read(host(v.contiguous()), q, s)
+        v.fill_(7.0)
+        assert (host(flat) == 7.0).all()
+        cache.sync()
+
+
+@gpu
 def test_strides_and_alignment(Q):
     rng = np.random.default_rng(3)
     x = rows_of(rng, 9, 64)
@@ -433,7 +467,8 @@ def test_many_tiles(Q, rows, k, n, gate, y_type):
                                            (3, 17, 8, 9, 34), (2, 3, 2, 4, 7), (1, 100, 24, 40, 250), (4, 65, 1, 136, 130),
                                            (1, 32, 40, 200, 64), (2, 128, 30, 44, 256), (1, 96, 16, 21, 20), (700, 8, 1, 8, 12),
                                            (1, 700, 20, 30, 300), (3, 260, 8, 12, 290), (2, 1300, 4, 24, 40), (2, 264, 3, 24, 520),
-                                           (1, 2000, 1, 77, 33), (1, 130, 48, 100, 258), (2, 4200, 2, 16, 12)])
+                                           (1, 2000, 1, 77, 33), (1, 130, 48, 100, 258), (2, 4200, 2, 16, 12),
+                                           (700, 8, 1, 40, 12), (300, 40, 4, 8, 70)])
 @pytest.mark.parametrize("gate", [False, True])
 def test_planes(Q, n_img, k, h, w, n, gate):
     if gate and n % 2:
