@@ -301,7 +301,9 @@ int check_matrix(const void* p, int dtype, int64_t rows, int64_t ld, int64_t col
 
 // How the product of `rows` tokens runs. One pass where the tokens are few or
 // the layer is narrow; otherwise the tokens are quantised into the workspace
-// and the product reads their codes.
+// and the product reads their codes. (Narrow layers in one pass and in two:
+// 522240 x 64 -> 128 43 and 75 us, 130560 x 256 -> 256 33 and 53, 2000 x 64 ->
+// 128 5.2 and 6.2, planes 32 -> 64 of 1088x1920 92 and 456.)
 enum class Path { kFew, kFused, kTwoPass };
 
 Path path_of(const ProductArgs& a, int dtype) {

@@ -13,7 +13,8 @@
 //   4. epilogue: a lane is a token; scales, bias, SimpleGate in FP32, a staging
 //      tile per warp and a TMA store (or direct stores, see linear8_tc.cu).
 // Two to four CTAs per SM overlap each other's phases; there is one CTA-wide
-// barrier per tile.
+// barrier per tile. 522240 x 64 -> 128 takes 43 us on the device (4.7 TB/s; its
+// writes alone would take 35 at the rate of a plain fill).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 

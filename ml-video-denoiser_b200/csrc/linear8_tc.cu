@@ -14,11 +14,16 @@
 //               epilogues overlap the next products;
 //   warps 0-7   epilogue: a lane is a token; scales, bias, SimpleGate in FP32,
 //               then through a swizzled staging tile per warp and a TMA store
-//               (rows whose address or stride does not allow it, and planes,
-//               are stored directly).
+//               (rows and planes whose address or stride does not allow it
+//               are stored by the lanes).
 // A segment's int32 sum is exact; it is scaled once, in FP32: layers with
 // segments keep their columns' running sums in registers (NT <= 128: 64 a
 // lane). Every wait is bounded.
+//
+// Measured on the device: 8192 x 4096 -> 4096 113 us with its quantisation (2.43
+// POP/s; copies into shared memory, 48 KB a chunk, and the power limit bind),
+// the fusion of 5 cached frames of 522240 x 64 -> 64 62 us (3.9 TB/s; the
+// epilogue's instructions bind).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -490,13 +495,14 @@ int run(TcArgs& g, int sms, cudaStream_t s) {
     g.tma_out = !p.planes && al16;
     g.pairs = reinterpret_cast<uintptr_t>(p.out) % 4 == 0 && p.ldo % 2 == 0;
     // A weight of one column tile that leaves room for four stages of codes
-    // stays in shared memory.
+    // stays in shared memory (5 x 522240 x 64 -> 64: 63 us, 66.5 without; 5 x
+    // 2088960 x 32 -> 32: 216 and 237).
     const int64_t b_bytes = static_cast<int64_t>(p.segs) * g.chunks * NT * g.kc;
     g.resident = g.n_tiles == 1 && b_bytes <= Plan<NT>::kRing - 4 * kStageA;
     g.stage = g.resident ? kRows * g.kc : Plan<NT>::kStage;
     const int ring = Plan<NT>::kRing - static_cast<int>(g.resident ? b_bytes : 0);
     // With a resident weight all of a tile's chunks make one stage where three
-    // fit: fewer waits and commits.
+    // fit: fewer waits and commits (the same layers: 66 and 237 us without).
     const int tile_bytes = p.segs * g.chunks * g.stage;
     g.units = g.resident && 3 * tile_bytes <= ring ? p.segs * g.chunks : 1;
     g.stage *= g.units;
