@@ -140,7 +140,26 @@ __device__ __forceinline__ void store_block32(uint8_t* stg, const float (&y)[32]
     for (int i = 0; i < 16; ++i) w[lane * 16 + (i ^ (lane >> 1))] = pack_half2(y[2 * i], y[2 * i + 1]);
     __syncwarp();
     const int live = static_cast<int>(rows - row0 < 32 ? rows - row0 : 32);
-    if (pairs) {
+    // Whole blocks with all their loads before the first store: one by one, a
+    // block took 1450 cycles (pairs) or 1200.
+    if (live == 32 && c + 32 <= n_out) {
+        if (pairs) {
+            uint32_t v[16];
+            __half* o = out + (row0 + (lane >> 4)) * ldo + c + 2 * (lane & 15);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) v[k] = w[(2 * k + (lane >> 4)) * 16 + ((lane & 15) ^ k)];
+#pragma unroll
+            for (int k = 0; k < 16; ++k, o += 2 * ldo) *reinterpret_cast<uint32_t*>(o) = v[k];
+        } else {
+            uint32_t v[32];
+            __half* o = out + row0 * ldo + c + lane;
+#pragma unroll
+            for (int r = 0; r < 32; ++r) v[r] = w[r * 16 + ((lane >> 1) ^ (r >> 1))];
+#pragma unroll
+            for (int r = 0; r < 32; ++r, o += ldo)
+                *o = __ushort_as_half(static_cast<unsigned short>(lane & 1 ? v[r] >> 16 : v[r]));
+        }
+    } else if (pairs) {
         const int i = lane & 15, col = c + 2 * i;
         for (int r = lane >> 4; r < live; r += 2) {
             const uint32_t v = w[r * 16 + (i ^ (r >> 1))];
@@ -166,7 +185,14 @@ __device__ __forceinline__ void store_block32(uint8_t* stg, const float (&y)[32]
     for (int i = 0; i < 32; ++i) w[lane * 32 + (i ^ lane)] = y[i];
     __syncwarp();
     const int live = static_cast<int>(rows - row0 < 32 ? rows - row0 : 32);
-    if (c + lane < n_out)
+    if (live == 32 && c + 32 <= n_out) {
+        float v[32];
+        float* o = out + row0 * ldo + c + lane;
+#pragma unroll
+        for (int r = 0; r < 32; ++r) v[r] = w[r * 32 + (lane ^ r)];
+#pragma unroll
+        for (int r = 0; r < 32; ++r, o += ldo) *o = v[r];
+    } else if (c + lane < n_out)
         for (int r = 0; r < live; ++r) out[(row0 + r) * ldo + c + lane] = w[r * 32 + (lane ^ r)];
 }
 
