@@ -279,6 +279,26 @@ def test_rows_that_begin_anywhere(Q, bits, dtype, rows, cols, gap):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("cols,group", [(64, 8), (96, 32), (512, 256), (3 * 2040, 2040)])
+def test_groups_of_rows_that_begin_anywhere(Q, dtype, cols, group):
+    rng = np.random.default_rng(cols)
+    x = rows_of(rng, 21, cols, dtype)
+    t = torch.float16 if dtype == np.float16 else torch.float32
+    for bits in (8, 4):
+        q, s = qo.quantise(x, bits, group)
+        for first, ld in ((1, cols), (3, cols + 5), (6, cols + 2)):
+            v = torch.full((21 * ld + 16,), float("nan"), dtype=t, device="cuda")[first:].as_strided((21, cols), (ld, 1))
+            v.copy_(dev(x))
+            cache = Q.RowCache(21, 1, cols, bits=bits, group=group)
+            cache.write(v)
+            assert_held(cache, slice(None), q, s, bits)
+            v.fill_(7.0)
+            cache.read_rows(rows=21, out=v)
+            assert_read(host(v.contiguous()), q, s)
+
+
+@gpu
 def test_strides_and_alignment(Q):
     rng = np.random.default_rng(3)
     x = rows_of(rng, 9, 64)
@@ -304,7 +324,8 @@ def test_strides_and_alignment(Q):
 
 @gpu
 @pytest.mark.parametrize("rows,cols,group", [(1, 32, 0), (40, 32, 0), (256, 24, 0), (300, 32, 0), (2000, 64, 16),
-                                             (300, 33, 0), (90, 512, 32), (260, 2304, 0), (30, 2304, 0)])
+                                             (300, 33, 0), (90, 512, 32), (260, 2304, 0), (30, 2304, 0),
+                                             (90, 333, 0), (400, 1001, 0), (2, 5, 0)])
 @pytest.mark.parametrize("bits", [8, 4])
 def test_scattered_rows_the_last_of_a_slot_counts(Q, rows, cols, group, bits):
     rng = np.random.default_rng(rows + cols)
