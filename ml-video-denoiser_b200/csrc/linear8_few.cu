@@ -1,4 +1,4 @@
-// The 8-bit product of a few tokens (serving one token at a time): one launch
+// The 8-bit product of a few tokens (serving one or some tokens at a time): one launch
 // that quantises the tokens and streams the weight once. Bound by the weight's
 // bytes (Cout * Cin) where it is large, by latency where it is small.
 //
@@ -26,11 +26,16 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMaxTokens = 8;
+constexpr int kMaxTokens = 16;
 // Codes of all tokens in shared memory. Every CTA makes them all, which costs
 // more than the tensor-core path from there on (8 x 4096 -> 4096: 19 us against
-// 12, -> 512: 15 against 11; 4 x 4096 -> 4096: 12 and 12, -> 512: 7 against 11).
+// 12, -> 512: 15 against 11; 4 x 4096 -> 4096: 8.7 against 12).
 constexpr int kMaxBytes = 16 * 1024;
+// Nine to sixteen tokens: one launch and no workspace are worth five
+// microseconds of the host, where no SM has more than two CTAs (13 x 1000 ->
+// 520, FP32: 10.3 us a call, 14 by the tensor cores, replayed 8.0 and 6.9; 13 x
+// 1024 -> 16384: 22 and 13.8).
+constexpr int kManyTokens = 8, kManyChannels = 2 * 148 * 8;
 
 struct FewArgs {
     ProductArgs p;
@@ -80,17 +85,34 @@ __global__ void __launch_bounds__(kThreads) product_few_kernel(const __grid_cons
     };
     auto code_at = [&](int r, int k) { return reinterpret_cast<uint2*>(s_codes + r * p.ldw + k * 8); };
     if constexpr (R >= kWarps) {
-        // A warp per token.
-        for (int r = tid >> 5; r < R; r += kWarps) {
+        // A warp per token, the next one's first kKeep vectors a lane on their way;
+        // those stay in registers, what a token has more is read twice.
+        constexpr int kKeep = 4, kEach = R / kWarps;
+        typename Q::Vec v[kEach > 1 ? 2 : 1][kKeep];
+        auto fetch = [&](int r, typename Q::Vec (&t)[kKeep]) {
+#pragma unroll
+            for (int i = 0; i < kKeep; ++i) t[i] = r < rows && lane + 32 * i < groups ? load(r, lane + 32 * i) : Q::zero();
+        };
+        fetch(tid >> 5, v[0]);
+#pragma unroll
+        for (int t = 0; t < kEach; ++t) {
+            const int r = (tid >> 5) + t * kWarps;
+            if (t + 1 < kEach) fetch(r + kWarps, v[(t + 1) % 2]);
+            typename Q::Vec(&cur)[kKeep] = v[t % 2];
             uint32_t mag = 0;
+#pragma unroll
+            for (int i = 0; i < kKeep; ++i) mag = max(mag, Q::mag(cur[i]));
             if (r < rows)
 #pragma unroll 4
-                for (int k = lane; k < groups; k += 32) mag = max(mag, Q::mag(load(r, k)));
+                for (int k = lane + 32 * kKeep; k < groups; k += 32) mag = max(mag, Q::mag(load(r, k)));
             mag = __reduce_max_sync(0xffffffffu, mag);
             const GroupScale q = group_scale<T>(mag, 127.f);
             if (lane == 0) s_scale[r] = q.s;
+#pragma unroll
+            for (int i = 0; i < kKeep; ++i)
+                if (lane + 32 * i < vecs * 2) *code_at(r, lane + 32 * i) = codes8<T>(cur[i], q, q.rare);
 #pragma unroll 4
-            for (int k = lane; k < vecs * 2; k += 32)
+            for (int k = lane + 32 * kKeep; k < vecs * 2; k += 32)
                 *code_at(r, k) = codes8<T>(r < rows && k < groups ? load(r, k) : Q::zero(), q, q.rare);
         }
     } else {
@@ -170,8 +192,8 @@ cudaError_t run(const FewArgs& g, cudaStream_t s) {
 
 template <typename T, int R>
 cudaError_t run_cpw(const FewArgs& g, int sms, cudaStream_t s) {
-    // Four weight rows a warp where that still gives every SM a CTA (4 x 1024 ->
-    // 4096: 3.3 us, 4.3 with two rows; 8 x 512 -> 1024: 3.5 and 3.3).
+    // Four weight rows a warp where that still gives every SM a CTA (one token,
+    // 4096 -> 16384: 8.9 us, 10.5 with two rows; 8 x 512 -> 1024: 3.5 and 3.3).
     return g.p.cout >= sms * kWarps * 4 ? run<T, R, 4>(g, s) : run<T, R, 2>(g, s);
 }
 
@@ -180,14 +202,16 @@ cudaError_t run_rows(const FewArgs& g, int sms, cudaStream_t s) {
     if (g.p.rows == 1) return run_cpw<T, 1>(g, sms, s);
     if (g.p.rows == 2) return run_cpw<T, 2>(g, sms, s);
     if (g.p.rows <= 4) return run_cpw<T, 4>(g, sms, s);
-    return run_cpw<T, 8>(g, sms, s);
+    if (g.p.rows <= 8) return run_cpw<T, 8>(g, sms, s);
+    return run<T, 16, 2>(g, s);  // a lane for each of 32 sums
 }
 
 }  // namespace
 
 bool product_few_takes(const ProductArgs& a) {
-    const int64_t r = a.rows <= 2 ? a.rows : a.rows <= 4 ? 4 : 8;
-    return a.rows <= kMaxTokens && !a.planes && a.segs == 1 && r * a.ldw <= kMaxBytes;
+    const int64_t r = a.rows <= 2 ? a.rows : a.rows <= 4 ? 4 : a.rows <= 8 ? 8 : 16;
+    return a.rows <= kMaxTokens && !a.planes && a.segs == 1 && r * a.ldw <= kMaxBytes &&
+           (a.rows <= kManyTokens || a.cout <= kManyChannels);
 }
 
 int launch_product_few(const ProductArgs& a, const void* x, int dtype, int64_t ldx, int out_dtype, int sms,

@@ -452,7 +452,9 @@ def make(Q, rng, k, n, gate, bias, segments=1, dtype=np.float16):
     (1, 1, 1), (1, 512, 1024), (1, 4096, 40), (2, 16, 2), (3, 100, 6), (5, 1000, 520), (8, 64, 64), (16, 48, 130),
     (17, 31, 34), (32, 2048, 66), (33, 128, 256), (64, 4100, 12), (100, 256, 256), (127, 64, 128), (128, 256, 512),
     (129, 257, 514), (130, 32, 8), (200, 96, 200), (300, 64, 258), (257, 1024, 96), (384, 512, 300), (1000, 17, 18),
-    (4096, 64, 64), (2500, 640, 160), (700, 33, 1030), (1300, 384, 384)])
+    (4096, 64, 64), (2500, 640, 160), (700, 33, 1030), (1300, 384, 384), (3, 2047, 70), (4, 4096, 66),
+    (8, 2048, 300), (6, 1025, 34), (10, 3, 6), (9, 1024, 520), (13, 1000, 520), (12, 1001, 2368), (16, 777, 130),
+    (16, 1024, 2370), (13, 2150, 18), (12, 300, 2400)])
 @pytest.mark.parametrize("gate", [False, True])
 @pytest.mark.parametrize("x_type,y_type", [(np.float16, torch.float16), (np.float32, torch.float16),
                                            (np.float16, torch.float32)])
