@@ -11,6 +11,36 @@ run. There is no collective on the data path.
 """
 from __future__ import annotations
 
+import contextlib
+
+
+@contextlib.contextmanager
+def _on(stream):
+    """`stream` current (None: what is current stays so), behind the work that
+    the caller's stream has queued: what a loop's loader loads and copies and
+    what the model is given and returns then belong to the stream that the
+    model runs on. Yields the caller's stream, None if it is the same."""
+    if stream is None:
+        yield None
+        return
+    import torch
+
+    caller = torch.cuda.current_stream(stream.device)
+    if stream == caller:
+        caller = None
+    else:
+        stream.wait_stream(caller)
+    with torch.cuda.stream(stream):
+        yield caller
+
+
+def _used_on(t, stream):
+    """`t`, whatever stream it was made on: once it is let go, its memory waits
+    for the work that `stream` has queued by then (None: its own stream's)."""
+    if stream is not None and getattr(t, "is_cuda", False):
+        t.record_stream(stream)
+    return t
+
 
 def segment(n_frames: int, world: int, rank: int) -> tuple[int, int]:
     """[start, end) of the frames rank `rank` of `world` denoises: contiguous,
@@ -128,6 +158,10 @@ def denoise_streams(model, clips, num_frames: int, bits: int = 8, store=None, st
     through the store, one clip's too: what a clip's outputs are does not depend
     on the others.
 
+    Everything runs on `stream` (default: torch's current stream), the clips'
+    loaders and ``on_frame`` too: they are called with it current, and it begins
+    behind what the caller's current stream has queued.
+
     Returns [(clip, frame index, output)]; ``on_frame(clip, i, y)``, when given,
     is called after each output."""
     T = num_frames
@@ -136,35 +170,34 @@ def denoise_streams(model, clips, num_frames: int, bits: int = 8, store=None, st
     results = []
     in_slot = [None] * T                  # (clip, frame) that each model slot holds, as restored from the store
     held = [[-1] * T for _ in clips]      # frame in each of a clip's store entries
-    for i in range(max((n for _, n in clips), default=0)):
-        for k, (frames, n) in enumerate(clips):
-            if i >= n:
-                continue
-            win = window(i, T, n)
-            for f in dict.fromkeys(win):
-                s, entry = f % T, k * T + f % T
-                if held[k][s] != f:
-                    x = frames(f).unsqueeze(0).contiguous()
-                    if store is None:
-                        import torch
+    with _on(stream) as caller:
+        for i in range(max((n for _, n in clips), default=0)):
+            for k, (frames, n) in enumerate(clips):
+                if i >= n:
+                    continue
+                win = window(i, T, n)
+                for f in dict.fromkeys(win):
+                    s, entry = f % T, k * T + f % T
+                    if held[k][s] != f:
+                        x = _used_on(frames(f), stream).unsqueeze(0).contiguous()
+                        if store is None:
+                            from .quant import FrameStore
 
-                        from .quant import FrameStore
-
-                        with torch.cuda.stream(stream):  # its zeros are written before a frame is parked
                             store = FrameStore(model, x.shape[2], x.shape[3], len(clips) * T, bits=bits)
-                    if store.model is not model or (store.h, store.w) != tuple(x.shape[2:]):
-                        raise ValueError(f"the store holds {store.h}x{store.w} frames of its model, clip {k} has "
-                                         f"{x.shape[2]}x{x.shape[3]}")
-                    model.encode_frame(x, s, stream=stream)
-                    store.park(s, entry, stream=stream)
-                    held[k][s], in_slot[s] = f, None
-                if in_slot[s] != (k, f):
-                    store.restore(entry, s, stream=stream)
-                    in_slot[s] = (k, f)
-            y = model.decode_window([f % T for f in win], frames(i).unsqueeze(0).contiguous(), stream=stream)[0]
-            results.append((k, i, y))
-            if on_frame is not None:
-                on_frame(k, i, y)
+                        if store.model is not model or (store.h, store.w) != tuple(x.shape[2:]):
+                            raise ValueError(f"the store holds {store.h}x{store.w} frames of its model, clip {k} has "
+                                             f"{x.shape[2]}x{x.shape[3]}")
+                        model.encode_frame(x, s, stream=stream)
+                        store.park(s, entry, stream=stream)
+                        held[k][s], in_slot[s] = f, None
+                    if in_slot[s] != (k, f):
+                        store.restore(entry, s, stream=stream)
+                        in_slot[s] = (k, f)
+                beauty = _used_on(frames(i), stream).unsqueeze(0).contiguous()
+                y = _used_on(model.decode_window([f % T for f in win], beauty, stream=stream)[0], caller)
+                results.append((k, i, y))
+                if on_frame is not None:
+                    on_frame(k, i, y)
     return results
 
 

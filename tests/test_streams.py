@@ -1,0 +1,144 @@
+"""Sequences on a stream of their own: the loader's work, the copies, the model's
+calls and the outputs are ordered one behind the other, whatever stream the
+caller has current.
+
+On the CPU the streams are stand-ins that note who waited for whom and which one
+was current at each call; on the GPU a loader makes every frame anew (non-
+contiguous, out of pinned memory, dropped at once) while the caller's stream is
+busy, and the outputs equal those of one stream.
+"""
+import contextlib
+import importlib
+
+import numpy as np
+import pytest
+import torch
+
+gpu = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def S(pkg):
+    return importlib.import_module(pkg.__name__ + ".sharding")
+
+
+class FakeStream:
+    device = None
+
+    def __init__(self, name):
+        self.name, self.waited_for = name, []
+
+    def wait_stream(self, other):
+        self.waited_for.append(other.name)
+
+
+@pytest.fixture
+def streams(monkeypatch):
+    """A caller's stream, which is current, and a side stream."""
+    main, side = FakeStream("main"), FakeStream("side")
+    now = [main]
+
+    @contextlib.contextmanager
+    def use(s):
+        now.append(s if s is not None else now[-1])
+        yield
+        now.pop()
+
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: now[-1])
+    monkeypatch.setattr(torch.cuda, "stream", use)
+    return main, side, now
+
+
+class FakeModel:
+    """Notes the stream that is current at each call, and the one it is given."""
+
+    def __init__(self, T, now):
+        self.slots, self.now, self.calls = [None] * T, now, []
+
+    def note(self, stream):
+        self.calls.append((self.now[-1].name, None if stream is None else stream.name))
+
+    def encode_frame(self, x, slot, stream=None):
+        assert x.is_contiguous()
+        self.note(stream)
+        self.slots[slot] = float(x.ravel()[0])
+
+    def decode_window(self, slots, beauty, stream=None):
+        assert beauty.is_contiguous()
+        self.note(stream)
+        return beauty.new_tensor([[self.slots[s] for s in slots]])
+
+    def __call__(self, x, stream=None):
+        assert x.is_contiguous()
+        self.note(stream)
+        return x.flatten(1)[:, :1]
+
+
+class FakeStore:
+    def __init__(self, model, h, w):
+        self.model, self.held, self.h, self.w = model, {}, h, w
+
+    def park(self, slot, entry, stream=None):
+        self.model.note(stream)
+        self.held[entry] = self.model.slots[slot]
+
+    def restore(self, entry, slot, stream=None):
+        self.model.note(stream)
+        self.model.slots[slot] = self.held[entry]
+
+
+def loader(now, seen, base=0.0):
+    def frames(f):
+        seen.append(now[-1].name)
+        return torch.full((2, 4, 3), base + f).permute(2, 0, 1)  # a copy makes it contiguous
+    return frames
+
+
+def test_clips_in_turn_run_on_the_stream_that_they_are_given(S, streams):
+    main, side, now = streams
+    m, seen, done = FakeModel(3, now), [], []
+    clips = [(loader(now, seen, 100.0 * k), n) for k, n in enumerate((4, 2))]
+    got = S.denoise_streams(m, clips, 3, store=FakeStore(m, 2, 4), stream=side,
+                            on_frame=lambda k, i, y: done.append(now[-1].name))
+    assert set(seen) == {"side"} and set(done) == {"side"} and set(m.calls) == {("side", "side")}
+    assert side.waited_for == ["main"] and main.waited_for == [] and now == [main]
+    assert len(got) == 6
+    for k, i, y in got:
+        assert y.tolist() == [100.0 * k + f for f in S.window(i, 3, (4, 2)[k])]
+    m.calls.clear(), seen.clear()
+    S.denoise_streams(m, clips, 3, store=FakeStore(m, 2, 4))
+    assert set(seen) == {"main"} and set(m.calls) == {("main", None)} and main.waited_for == []
+
+
+def temporal(pkg, tmp_path, T=3):
+    synth = importlib.import_module(pkg.__name__ + ".synth")
+    cfg = synth.NAFConfig(base_channels=8, enc_blocks=(1, 1), middle_blocks=1, dec_blocks=(1, 1))
+    return pkg.Model(synth.make_model_dir(str(tmp_path), cfg, 4, "py", T, True)[0])
+
+
+def host_clip(seed, n, h=62, w=74):
+    """Frames (H, W, 3) in pinned memory, as a decoder leaves them."""
+    rng = np.random.default_rng(seed)
+    return [torch.from_numpy(rng.uniform(0, 1, (h, w, 3)).astype(np.float16)).pin_memory() for _ in range(n)]
+
+
+def fresh(clip):
+    """A loader whose frames nobody else holds."""
+    return lambda f: clip[f].to("cuda", non_blocking=True).permute(2, 0, 1)
+
+
+@gpu
+def test_clips_in_turn_with_frames_that_are_loaded_and_dropped(pkg, S, tmp_path):
+    m = temporal(pkg, tmp_path)
+    clips = [host_clip(s, 5) for s in (1, 2)]
+    take = [(fresh(c), 5) for c in clips]
+    want = [y.clone() for _, _, y in S.denoise_streams(m, take, 3)]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        torch.cuda._sleep(20_000_000)  # the caller's stream is busy when the loop begins
+        got = S.denoise_streams(m, take, 3, stream=side, on_frame=lambda k, i, y: torch.zeros(3, 62, 74, device="cuda"))
+        side.synchronize()
+        for (k, i, y), w in zip(got, want):
+            assert torch.equal(y, w), (k, i)
+    m.sync()
