@@ -111,37 +111,45 @@ def denoise_range(model, frames, n_frames: int, start: int, end: int, num_frames
     encoded once into slot f % T (distinct frames of one window never share a
     slot) and each output decodes its window from the slots, so the encoder
     runs once per loaded frame instead of T times per output. With
-    ``cache=False`` every window is assembled as a (1, T, C, H, W) clip."""
-    import torch
+    ``cache=False`` every window is assembled as a (1, T, C, H, W) clip.
 
+    Everything runs on `stream` (default: torch's current stream), `frames` and
+    ``on_frame`` too: they are called with it current, and it begins behind what
+    the caller's current stream has queued."""
     s, e = start, end
     results = []
 
+    def load(f):
+        return _used_on(frames(f), stream)
+
     def emit(i, y):
-        results.append((i, y))
+        results.append((i, _used_on(y, caller)))
         if on_frame is not None:
             on_frame(i, y)
 
-    if num_frames == 1:
+    with _on(stream) as caller:
+        if num_frames == 1:
+            for i in range(s, e):
+                emit(i, model(load(i).unsqueeze(0).contiguous(), stream=stream)[0])
+            return results
+        if not cache:
+            import torch
+
+            r = num_frames // 2
+            held = {f: load(f) for f in range(max(0, s - r), min(n_frames, e + r))}
+            for i in range(s, e):
+                x = torch.stack([held[f] for f in window(i, num_frames, n_frames)], dim=0).unsqueeze(0)
+                emit(i, model(x.contiguous(), stream=stream)[0])
+            return results
+        T = num_frames
+        in_slot = [-1] * T  # frame index held by each slot
         for i in range(s, e):
-            emit(i, model(frames(i).unsqueeze(0).contiguous(), stream=stream)[0])
-        return results
-    if not cache:
-        r = num_frames // 2
-        held = {f: frames(f) for f in range(max(0, s - r), min(n_frames, e + r))}
-        for i in range(s, e):
-            x = torch.stack([held[f] for f in window(i, num_frames, n_frames)], dim=0).unsqueeze(0)
-            emit(i, model(x.contiguous(), stream=stream)[0])
-        return results
-    T = num_frames
-    in_slot = [-1] * T  # frame index held by each slot
-    for i in range(s, e):
-        win = window(i, T, n_frames)
-        for f in win:
-            if in_slot[f % T] != f:
-                model.encode_frame(frames(f).unsqueeze(0).contiguous(), f % T, stream=stream)
-                in_slot[f % T] = f
-        emit(i, model.decode_window([f % T for f in win], frames(i).unsqueeze(0).contiguous(), stream=stream)[0])
+            win = window(i, T, n_frames)
+            for f in win:
+                if in_slot[f % T] != f:
+                    model.encode_frame(load(f).unsqueeze(0).contiguous(), f % T, stream=stream)
+                    in_slot[f % T] = f
+            emit(i, model.decode_window([f % T for f in win], load(i).unsqueeze(0).contiguous(), stream=stream)[0])
     return results
 
 

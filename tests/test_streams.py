@@ -110,6 +110,19 @@ def test_clips_in_turn_run_on_the_stream_that_they_are_given(S, streams):
     assert set(seen) == {"main"} and set(m.calls) == {("main", None)} and main.waited_for == []
 
 
+@pytest.mark.parametrize("T,cache", [(1, True), (3, True), (3, False)])
+def test_a_sequence_runs_on_the_stream_that_it_is_given(S, streams, T, cache):
+    main, side, now = streams
+    for stream, name in ((side, "side"), (None, "main"), (main, "main")):
+        m, seen, done = FakeModel(T, now), [], []
+        got = S.denoise_segment(m, loader(now, seen), 5, 1, 0, num_frames=T, stream=stream, cache=cache)
+        assert [i for i, _ in got] == list(range(5))
+        S.denoise_range(m, loader(now, seen), 5, 1, 3, T, stream, cache, on_frame=lambda i, y: done.append(now[-1].name))
+        assert set(seen) == {name} and done == [name] * 2 and {c for c, _ in m.calls} == {name}
+        assert now == [main] and main.waited_for == []
+    assert side.waited_for == ["main"] * 2
+
+
 def temporal(pkg, tmp_path, T=3):
     synth = importlib.import_module(pkg.__name__ + ".synth")
     cfg = synth.NAFConfig(base_channels=8, enc_blocks=(1, 1), middle_blocks=1, dec_blocks=(1, 1))
@@ -141,4 +154,21 @@ def test_clips_in_turn_with_frames_that_are_loaded_and_dropped(pkg, S, tmp_path)
         side.synchronize()
         for (k, i, y), w in zip(got, want):
             assert torch.equal(y, w), (k, i)
+    m.sync()
+
+
+@gpu
+@pytest.mark.parametrize("cache", [True, False])
+def test_a_sequence_with_frames_that_are_loaded_and_dropped(pkg, S, tmp_path, cache):
+    m = temporal(pkg, tmp_path)
+    clip = host_clip(3, 6)
+    want = [y.clone() for _, y in S.denoise_segment(m, fresh(clip), 6, 1, 0, num_frames=3, cache=cache)]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        torch.cuda._sleep(20_000_000)
+        got = S.denoise_segment(m, fresh(clip), 6, 1, 0, num_frames=3, stream=side, cache=cache)
+        side.synchronize()
+        for (i, y), w in zip(got, want):
+            assert torch.equal(y, w), i
     m.sync()
