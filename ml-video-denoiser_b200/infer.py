@@ -19,7 +19,7 @@ from __future__ import annotations
 
 import ctypes
 
-from . import check, lib, stream_handle
+from . import check, lib, sharding, stream_handle
 
 
 def _p(t) -> ctypes.c_void_p:
@@ -35,7 +35,6 @@ def tile_inference(model, x, tile_size: int, stream=None):
         raise ValueError("tile_inference: tile_size must be positive")
     s = stream if stream is not None else torch.cuda.current_stream(x.device)
     sh = stream_handle(s)
-    x = x.contiguous()
     h, w = x.shape[-2:]
     lead = tuple(x.shape[:-2])
     planes = 1
@@ -43,7 +42,8 @@ def tile_inference(model, x, tile_size: int, stream=None):
         planes *= d
     overlap = tile_size // 8
     stride = tile_size - overlap
-    with torch.cuda.stream(s):
+    with sharding._on(s) as caller:  # the copy that makes x contiguous too
+        x = sharding._used_on(x, s).contiguous()
         acc = torch.zeros(3, h, w, dtype=torch.float32, device=x.device)
         wsum = torch.zeros(h, w, dtype=torch.float32, device=x.device)
         for y1 in range(0, h, stride):
@@ -59,7 +59,7 @@ def tile_inference(model, x, tile_size: int, stream=None):
         check(lib().dn_tile_normalize(ctypes.cast(acc.data_ptr(), ctypes.POINTER(ctypes.c_float)),
                                       ctypes.cast(wsum.data_ptr(), ctypes.POINTER(ctypes.c_float)), _p(out), 3, h, w,
                                       sh))
-    return out
+    return sharding._used_on(out, caller)
 
 
 def _window(i: int, num_frames: int, n: int) -> list[int]:
@@ -77,8 +77,6 @@ def _sequence_pass(model, frames, num_frames: int, tile_size: int, stream):
             clip = torch.stack([frames[f] for f in _window(i, num_frames, n)], dim=0).unsqueeze(0)
             outs.append(tile_inference(model, clip, tile_size, stream)[0])
         return outs
-    from . import sharding
-
     return [y for _, y in sharding.denoise_segment(model, lambda i: frames[i], n, 1, 0, num_frames=num_frames,
                                                     stream=stream)]
 
@@ -95,14 +93,14 @@ def denoise_temporal_sequence(model, frames, num_frames: int, temporal_flip: boo
     if any(f.shape != frames[0].shape for f in frames):
         raise ValueError("Temporal inference requires all frames in a sequence to share shape")
     s = stream if stream is not None else torch.cuda.current_stream(frames[0].device)
-    forward = _sequence_pass(model, frames, num_frames, tile_size, s)
-    if not temporal_flip:
-        return forward
-    backward = _sequence_pass(model, frames[::-1], num_frames, tile_size, s)[::-1]
-    out = []
-    with torch.cuda.stream(s):
+    with sharding._on(s) as caller:  # the windows that the passes put together too
+        forward = _sequence_pass(model, [sharding._used_on(f, s) for f in frames], num_frames, tile_size, s)
+        if not temporal_flip:
+            return [sharding._used_on(y, caller) for y in forward]
+        backward = _sequence_pass(model, frames[::-1], num_frames, tile_size, s)[::-1]
+        out = []
         for f, b in zip(forward, backward):
             y = torch.empty_like(f)
             check(lib().dn_average_pair(_p(f), _p(b), _p(y), f.numel(), stream_handle(s)))
-            out.append(y)
+            out.append(sharding._used_on(y, caller))
     return out

@@ -23,7 +23,7 @@ def S(pkg):
 
 
 class FakeStream:
-    device = None
+    device, cuda_stream = None, 0
 
     def __init__(self, name):
         self.name, self.waited_for = name, []
@@ -121,6 +121,43 @@ def test_a_sequence_runs_on_the_stream_that_it_is_given(S, streams, T, cache):
         assert set(seen) == {name} and done == [name] * 2 and {c for c, _ in m.calls} == {name}
         assert now == [main] and main.waited_for == []
     assert side.waited_for == ["main"] * 2
+
+
+class NoKernels:
+    """The library's launchers, not called."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+class Noted(torch.Tensor):
+    """A tensor that notes the streams that are current when it is copied."""
+
+    def contiguous(self):
+        self.seen.append(self.now[-1].name)
+        return self.as_subclass(torch.Tensor).contiguous()
+
+
+@pytest.mark.parametrize("tile", [0, 8])
+@pytest.mark.parametrize("flip", [False, True])
+def test_whole_sequences_and_tiles_run_on_the_stream_that_they_are_given(pkg, streams, monkeypatch, tile, flip):
+    infer = importlib.import_module(pkg.__name__ + ".infer")
+    monkeypatch.setattr(infer, "lib", NoKernels)
+    monkeypatch.setattr(infer, "check", lambda rc: None)
+    main, side, now = streams
+    stacked, stack = [], torch.stack
+    monkeypatch.setattr(torch, "stack", lambda *a, **k: stacked.append(now[-1].name) or stack(*a, **k))
+    m = FakeModel(3, now)
+    m.decode_window = lambda slots, beauty, stream=None: m.note(stream) or beauty
+    m.__class__ = type("Whole", (FakeModel,), {"__call__": lambda s, x, stream=None: s.note(stream) or x[:, 0]})
+    frames = [torch.rand(2, 4, 12).permute(0, 2, 1) for _ in range(4)]
+    assert len(infer.denoise_temporal_sequence(m, frames, 3, flip, tile, stream=side)) == 4
+    assert set(m.calls) == {("side", "side")} and set(stacked) <= {"side"} and bool(stacked) == (tile > 0)
+    assert side.waited_for == ["main"] and now == [main]
+    x = torch.rand(1, 3, 16, 12).transpose(2, 3).as_subclass(Noted)
+    x.seen, x.now = [], now
+    infer.tile_inference(m, x, 8, stream=side)
+    assert x.seen == ["side"] and side.waited_for == ["main"] * 2 and main.waited_for == [] and now == [main]
 
 
 def temporal(pkg, tmp_path, T=3):
