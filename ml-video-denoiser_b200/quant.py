@@ -92,7 +92,10 @@ def _matrix(t, rows: int | None, cols: int, device: int, what: str) -> int:
 class RowCache:
     """``pages * page_rows`` rows of ``cols`` values held in ``bits`` bits (8
     or 4), with a scale for every ``group`` columns (0: one a row). ``codes``
-    and ``scales`` are the tensors it is held in; new rows read as zeros."""
+    and ``scales`` are the tensors it is held in; new rows read as zeros, on any
+    stream once the cache is made. Whoever uses one cache on several streams
+    orders writes and reads of the same rows, and keeps the cache until they are
+    done, as with any tensor."""
 
     def __init__(self, pages: int, page_rows: int, cols: int, bits: int = 8, group: int = 0, device=0):
         if pages < 0 or page_rows < 1 or cols < 1:
@@ -112,6 +115,11 @@ class RowCache:
         self.codes = torch.zeros(self.capacity, row, dtype=torch.uint8, device=d)
         self.scales = torch.zeros(self.capacity, cols // group, dtype=torch.float32, device=d)
         self._err = torch.zeros(1, dtype=torch.int32, device=d)
+        # The zeros are there before any call, whatever stream it is on. (In a
+        # capture they are part of the graph, in front of what uses them.)
+        with torch.cuda.device(d):
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream(d).synchronize()
         self._held = (self.codes.data_ptr(), row, self.scales.data_ptr(), self.capacity)
         self._err_ptr = self._err.data_ptr()
 

@@ -160,6 +160,30 @@ def test_whole_sequences_and_tiles_run_on_the_stream_that_they_are_given(pkg, st
     assert x.seen == ["side"] and side.waited_for == ["main"] * 2 and main.waited_for == [] and now == [main]
 
 
+def test_a_cache_is_made_when_its_constructor_returns(pkg, streams, monkeypatch):
+    """Its zeros, on the stream that is current, are waited for: later calls may
+    be on any stream."""
+    Q = importlib.import_module(pkg.__name__ + ".quant")
+    main, side, now = streams
+    order, zeros = [], torch.zeros
+
+    def filled(*size, device=None, **k):
+        order.append("zeros")
+        return zeros(*size, **k)
+
+    monkeypatch.setattr(torch, "zeros", filled)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing)
+    main.synchronize = lambda: order.append("synchronize")
+    capturing = False
+    Q.RowCache(2, 3, 8)
+    assert order == ["zeros"] * 3 + ["synchronize"]
+    order.clear()
+    capturing = True  # where it would end the capture
+    Q.RowCache(2, 3, 8)
+    assert order == ["zeros"] * 3
+
+
 def temporal(pkg, tmp_path, T=3):
     synth = importlib.import_module(pkg.__name__ + ".synth")
     cfg = synth.NAFConfig(base_channels=8, enc_blocks=(1, 1), middle_blocks=1, dec_blocks=(1, 1))
@@ -209,3 +233,41 @@ def test_a_sequence_with_frames_that_are_loaded_and_dropped(pkg, S, tmp_path, ca
         for (i, y), w in zip(got, want):
             assert torch.equal(y, w), i
     m.sync()
+
+
+@gpu
+def test_a_cache_used_on_another_stream_than_it_was_made_on(pkg):
+    Q = importlib.import_module(pkg.__name__ + ".quant")
+    side = torch.cuda.Stream()
+    x = torch.full((300, 64), 127.0, dtype=torch.float16, device="cuda")
+    slots = torch.tensor([300] * 300, device="cuda")  # behind the cache
+    for bits in (8, 4):
+        torch.cuda.synchronize()
+        torch.cuda._sleep(40_000_000)
+        cache = Q.RowCache(1, 300, 64, bits=bits)
+        cache.write(x, stream=side)
+        cache.write(x, slots=slots, stream=side)
+        with torch.cuda.stream(side):
+            back = cache.read_rows(rows=300)
+        with pytest.raises(pkg.DenoiserError):
+            cache.sync(stream=side)
+        torch.cuda.synchronize()
+        assert bool((back == 127).all()) and bool((cache.scales > 0).all())
+
+
+@gpu
+def test_a_cache_made_in_a_capture(pkg):
+    Q = importlib.import_module(pkg.__name__ + ".quant")
+    x = torch.ones(5, 32, dtype=torch.float16, device="cuda")
+    Q.RowCache(2, 5, 32).write(x)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        cache = Q.RowCache(2, 5, 32)
+        cache.write(x, row0=2)
+        out = cache.read_rows(rows=10)
+    for _ in range(2):
+        x += 1
+        g.replay()
+        torch.cuda.synchronize()
+        assert bool((out[2:7] == x).all()) and not bool(out[:2].any()) and not bool(out[7:].any())
