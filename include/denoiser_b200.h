@@ -167,10 +167,16 @@ int dn_model_decode_window(dn_model* model, const int* slots, int T, const void*
  * of denoiser_b200_quant.h, straight into and out of a slot) and decoding
  * several sequences in turn with one model. Plans the buffers for H x W frames
  * like dn_model_encode_frame, and the address holds as long as they do: while
- * the frame size does not change. DN_ERR_INVALID_ARG as there, and for a level
- * outside [0, num_levels]. */
+ * the frame size does not change (planning for another one drops what all
+ * slots hold). The caller may fill the slot through the addresses of its
+ * levels, so it counts as holding a frame from then on. `features` NULL: rows
+ * and channels alone; nothing is planned and no slot is dropped.
+ * DN_ERR_INVALID_ARG as there, and for a level outside [0, num_levels]. */
 int dn_model_frame_features(dn_model* model, int H, int W, int slot, int level, void** features, int64_t* rows,
                             int* channels);
+/* Size of the frame that `slot` holds; 0 x 0 for a slot that none was encoded or
+ * put into since the buffers were planned for the current frame size. */
+int dn_model_slot_frame(const dn_model* model, int slot, int* H, int* W);
 
 /* Synchronise `stream`; DN_ERR_DEVICE if a kernel reported a device-side
  * error (e.g. a bounded wait that expired) since the last check. */

@@ -89,6 +89,7 @@ SIGNATURES = {
     "dn_model_encode_frame": (_I, [_P, _P, _I, _I, _I, _I, _P]),
     "dn_model_decode_window": (_I, [_P, _IP, _I, _P, _I, _I, _I, _P, _P]),
     "dn_model_frame_features": (_I, [_P, _I, _I, _I, _I, _PP, _I64P, _IP]),
+    "dn_model_slot_frame": (_I, [_P, _I, _IP, _IP]),
     "dn_model_sync": (_I, [_P, _P]),
     "dn_model_stats": (_I, [_P, _SZP, _SZP, _IP]),
     "dn_model_set_fused": (_I, [_P, _I]),
@@ -374,7 +375,9 @@ class Model:
         as the engine holds them, an FP16 CUDA tensor (rows, channels) on its
         own memory: `level` 0 .. num_levels - 1 the skips, num_levels the deep
         features, a row per pixel of the padded frame. Valid while the frame
-        size does not change and the model lives."""
+        size does not change and the model lives; for a size that the model has
+        not been used with last, all slots are dropped, as by ``encode_frame``.
+        Whoever fills the levels puts a frame into the slot."""
         import torch
 
         p, rows, ch = ctypes.c_void_p(), ctypes.c_int64(), ctypes.c_int()
@@ -382,6 +385,18 @@ class Model:
                                             ctypes.byref(ch)))
         return torch.as_tensor(_DeviceMemory(p.value, (rows.value, ch.value), "<f2"),
                                device=torch.device("cuda", self.device))
+
+    def feature_shape(self, h: int, w: int, level: int) -> tuple[int, int]:
+        """(rows, channels) of ``frame_features``; the slots stay as they are."""
+        rows, ch = ctypes.c_int64(), ctypes.c_int()
+        check(lib().dn_model_frame_features(self._h, h, w, 0, level, None, ctypes.byref(rows), ctypes.byref(ch)))
+        return rows.value, ch.value
+
+    def slot_frame(self, slot: int) -> tuple[int, int]:
+        """Temporal models: (h, w) of the frame that cache slot `slot` holds; (0, 0): none."""
+        h, w = ctypes.c_int(), ctypes.c_int()
+        check(lib().dn_model_slot_frame(self._h, slot, ctypes.byref(h), ctypes.byref(w)))
+        return h.value, w.value
 
     def sync(self, stream=None) -> None:
         """Synchronise the stream and raise if a kernel flagged a device error."""

@@ -152,11 +152,16 @@ int dn_model_encode_frame(dn_model* m, const void* frame, int C, int H, int W, i
 
 int dn_model_frame_features(dn_model* m, int H, int W, int slot, int level, void** features, int64_t* rows,
                             int* channels) {
-    if (!m || !features || !rows || !channels)
+    if (!m || !rows || !channels)
         return dn_fail(DN_ERR_INVALID_ARG, "dn_model_frame_features: null argument");
     return guarded([&] {
         return m->eng->frame_features(H, W, slot, level, reinterpret_cast<__half**>(features), rows, channels);
     });
+}
+
+int dn_model_slot_frame(const dn_model* m, int slot, int* H, int* W) {
+    if (!m || !H || !W) return dn_fail(DN_ERR_INVALID_ARG, "dn_model_slot_frame: null argument");
+    return m->eng->slot_frame(slot, H, W);
 }
 
 int dn_model_decode_window(dn_model* m, const int* slots, int T, const void* beauty, int C, int H, int W, void* y,

@@ -504,6 +504,7 @@ void Engine::plan(const Shape& s) {
     shape_ = s;
     const int L = info_.num_levels;
     const bool temporal = info_.kind != 0;
+    slot_held_.assign(temporal ? s.T : 0, 0);
     const size_t n_enc = temporal ? s.T : s.N;  // images through the encoder
     const size_t n_dec = temporal ? 1 : s.N;
     std::vector<std::pair<size_t, void**>> req;
@@ -925,7 +926,7 @@ int Engine::run_stage(const std::vector<BlockW>& blocks, __half* x, int nimg, in
 
 // Shape of an input of N images (clips of T frames) of C x H x W, padded to
 // the model's multiple; DN_OK or an error for shapes the engine rejects.
-int Engine::make_shape(int N, int T, int C, int H, int W, Shape& sh) {
+int Engine::check_shape(int N, int T, int C, int H, int W, Shape& sh) const {
     if (N <= 0 || H <= 0 || W <= 0) return dn_fail(DN_ERR_INVALID_ARG, "forward: empty input");
     if (C < info_.in_channels)
         return dn_fail(DN_ERR_INVALID_ARG, "forward: input has fewer channels than model expects");
@@ -943,6 +944,12 @@ int Engine::make_shape(int N, int T, int C, int H, int W, Shape& sh) {
         return dn_fail(DN_ERR_INVALID_ARG, "forward: frame smaller than the reflect padding it needs");
     if (static_cast<long long>(N) * T * sh.Hp * sh.Wp > (1LL << 30))
         return dn_fail(DN_ERR_UNSUPPORTED, "forward: input too large");
+    return DN_OK;
+}
+
+// The same, and the buffers planned for it.
+int Engine::make_shape(int N, int T, int C, int H, int W, Shape& sh) {
+    DN_TRY(check_shape(N, T, C, H, W, sh));
     try {
         plan(sh);
     } catch (const std::exception& e) {
@@ -1195,6 +1202,7 @@ int Engine::forward(const __half* x, int N, int T, int C, int H, int W, __half* 
         DN_TRY(encode_into(clip, T, C * H * W, 0, s));
         DN_TRY(temporal_tail(slots.data(), clip + static_cast<size_t>(ref) * C * H * W, C * H * W,
                              y + static_cast<size_t>(n) * 3 * H * W, s));
+        slot_held_.assign(T, 1);
     }
     return DN_OK;
 }
@@ -1207,7 +1215,10 @@ int Engine::encode_frame(const __half* frame, int C, int H, int W, int slot, cud
     Shape sh;
     DN_TRY(make_shape(1, info_.num_frames, C, H, W, sh));
     launches_ = 0;
-    return encode_into(frame, 1, C * H * W, slot, s);
+    slot_held_[slot] = 0;
+    DN_TRY(encode_into(frame, 1, C * H * W, slot, s));
+    slot_held_[slot] = 1;
+    return DN_OK;
 }
 
 int Engine::decode_window(const int* slots, const __half* beauty, int C, int H, int W, __half* y, cudaStream_t s) {
@@ -1229,12 +1240,25 @@ int Engine::frame_features(int H, int W, int slot, int level, __half** features,
     if (level < 0 || level > L) return dn_fail(DN_ERR_INVALID_ARG, "frame_features: level outside [0, num_levels]");
     DeviceGuard dg(device_);
     Shape sh;
-    DN_TRY(make_shape(1, info_.num_frames, info_.in_channels, H, W, sh));
-    const int64_t n = static_cast<int64_t>(shape_.Hp >> level) * (shape_.Wp >> level);
+    const int C = std::max(3, info_.in_channels);
+    DN_TRY(features ? make_shape(1, info_.num_frames, C, H, W, sh) : check_shape(1, info_.num_frames, C, H, W, sh));
+    const int64_t n = static_cast<int64_t>(sh.Hp >> level) * (sh.Wp >> level);
     const int c = level < L ? levels_[level].C : levels_[L - 1].C * 2;
-    if (features) *features = (level < L ? enc_x_[level] : mid_x_) + slot * n * c;
+    if (features) {
+        *features = (level < L ? enc_x_[level] : mid_x_) + slot * n * c;
+        slot_held_[slot] = 1;
+    }
     if (rows) *rows = n;
     if (channels) *channels = c;
+    return DN_OK;
+}
+
+int Engine::slot_frame(int slot, int* H, int* W) const {
+    if (info_.kind == 0) return dn_fail(DN_ERR_INVALID_ARG, "slot_frame: spatial models have no frame cache");
+    if (slot < 0 || slot >= info_.num_frames) return dn_fail(DN_ERR_INVALID_ARG, "slot_frame: slot outside [0, T)");
+    const bool held = aarena_ && slot_held_[slot];
+    *H = held ? shape_.H : 0;
+    *W = held ? shape_.W : 0;
     return DN_OK;
 }
 

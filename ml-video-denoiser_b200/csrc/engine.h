@@ -83,8 +83,12 @@ public:
     int decode_window(const int* slots, const __half* beauty, int C, int H, int W, __half* y, cudaStream_t s);
 
     // The features of cache slot `slot` at `level` (num_levels = deep features)
-    // of H x W frames: FP16 [rows][channels].
+    // of H x W frames: FP16 [rows][channels]. Whoever has the address may fill
+    // the slot, which counts as held from then on; features null: the sizes
+    // alone, nothing is planned.
     int frame_features(int H, int W, int slot, int level, __half** features, int64_t* rows, int* channels);
+    // Size of the frame that `slot` holds, 0 x 0: none since the buffers were planned.
+    int slot_frame(int slot, int* H, int* W) const;
 
     // Waits for `s` and returns DN_ERR_DEVICE if a kernel flagged an error
     // since the last check (the word is cleared).
@@ -133,6 +137,7 @@ private:
 
     void build(const HostWeights& hw);
     void plan(const Shape& s);
+    int check_shape(int N, int T, int C, int H, int W, Shape& sh) const;
     int make_shape(int N, int T, int C, int H, int W, Shape& sh);
     int encode_into(const __half* src, int nimg, int in_stride, int slot0, cudaStream_t s);
     int decode_from(__half* xm, int nimg, const std::vector<__half*>& skips, const __half* beauty, int beauty_stride,
@@ -180,6 +185,7 @@ private:
     size_t aarena_bytes_ = 0;
     std::vector<__half*> enc_x_, dec_x_;  // per level (encoder state/skip, decoder state)
     __half* mid_x_ = nullptr;
+    std::vector<char> slot_held_;         // temporal: whether a frame is in the cache slot
     __half *buf_u_ = nullptr, *buf_g_ = nullptr, *buf_y_ = nullptr, *buf_t_ = nullptr;
     std::vector<__half*> fused_skip_;     // temporal: fused skip per level
     __half* warp_buf_ = nullptr;          // temporal: warped neighbours [T-1][...]

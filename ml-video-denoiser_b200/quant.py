@@ -229,7 +229,7 @@ class FrameStore:
         self.model, self.h, self.w, self.frames = model, h, w, frames
         self.caches = []
         for level in range(model.num_levels + 1):
-            rows, cols = model.frame_features(h, w, 0, level).shape
+            rows, cols = model.feature_shape(h, w, level)
             self.caches.append(RowCache(frames, rows, cols, bits=bits, group=group, device=model.device))
 
     def _entry(self, entry: int) -> int:
@@ -238,13 +238,19 @@ class FrameStore:
         return entry
 
     def park(self, slot: int, entry: int, stream=None) -> None:
-        """The frame in the model's cache slot `slot` into `entry`."""
+        """The h x w frame in the model's cache slot `slot` into `entry`."""
         self._entry(entry)
+        held = self.model.slot_frame(slot)
+        if held != (self.h, self.w):
+            _bad(f"FrameStore.park: slot {slot} holds " + (f"a {held[0]}x{held[1]} frame" if held[0] else "no frame") +
+                 f", the store {self.h}x{self.w} ones")
         for level, c in enumerate(self.caches):
             c.write(self.model.frame_features(self.h, self.w, slot, level), row0=entry * c.page_rows, stream=stream)
 
     def restore(self, entry: int, slot: int, stream=None) -> None:
-        """The frame of `entry` into the model's cache slot `slot`."""
+        """The frame of `entry` into the model's cache slot `slot` (where the
+        model was used with another frame size last, its other slots are
+        dropped, as by ``encode_frame``)."""
         self._entry(entry)
         for level, c in enumerate(self.caches):
             c.read_rows(row0=entry * c.page_rows, rows=c.page_rows,

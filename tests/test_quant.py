@@ -785,6 +785,54 @@ def test_streams_through_the_frame_store(pkg, Q, tmp_path, kind, T, bits):
 
 
 @gpu
+def test_a_slot_without_a_frame_of_the_size_is_not_parked(pkg, Q, tmp_path):
+    """Nothing is held that was not encoded: another frame size drops the slots,
+    a store that is made or that refuses drops none."""
+    m = small_temporal(pkg, tmp_path, "py", 3)
+    rng = np.random.default_rng(3)
+    small = dev(rng.uniform(0, 1, (1, 3, 30, 42)).astype(np.float16))
+    large = dev(rng.uniform(0, 1, (1, 3, 46, 42)).astype(np.float16))
+    store = Q.FrameStore(m, 30, 42, 2)
+    assert m.slot_frame(1) == (0, 0)
+    with pytest.raises(pkg.InvalidArgumentError):
+        store.park(1, 0)  # nothing was ever encoded
+    m.encode_frame(small, 1)
+    assert [m.slot_frame(s) for s in range(3)] == [(0, 0), (30, 42), (0, 0)]
+    want = [host(m.frame_features(30, 42, 1, l)).copy() for l in range(m.num_levels + 1)]
+    store.park(1, 0)
+    held = [host(c.codes).copy() for c in store.caches]
+    other = Q.FrameStore(m, 46, 42, 1)  # made for another size: the slots stay
+    assert m.slot_frame(1) == (30, 42)
+    for bad in (lambda: other.park(1, 0), lambda: store.park(0, 1), lambda: store.park(3, 1), lambda: m.slot_frame(-1),
+                lambda: m.feature_shape(30, 42, -1), lambda: m.feature_shape(0, 42, 0)):
+        with pytest.raises(pkg.InvalidArgumentError):
+            bad()
+    for l, f in enumerate(want):
+        assert m.feature_shape(30, 42, l) == f.shape
+        np.testing.assert_array_equal(host(m.frame_features(30, 42, 1, l)), f)
+    assert not any(host(c.codes).any() for c in other.caches)
+    m.encode_frame(large, 1)
+    assert m.slot_frame(1) == (46, 42)
+    with pytest.raises(pkg.InvalidArgumentError):
+        store.park(1, 0)  # the slot holds a frame of the other size
+    other.park(1, 0)
+    m.encode_frame(small, 0)  # drops slot 1 once more
+    with pytest.raises(pkg.InvalidArgumentError):
+        store.park(1, 0)
+    for c, codes in zip(store.caches, held):
+        np.testing.assert_array_equal(host(c.codes), codes)
+    store.restore(0, 2)
+    assert [m.slot_frame(s) for s in range(3)] == [(30, 42), (0, 0), (30, 42)]
+    for l, f in enumerate(want):
+        assert_read(host(m.frame_features(30, 42, 2, l)), *qo.quantise(f))
+    store.park(2, 1)
+    m(torch.cat([large] * 3).unsqueeze(0))  # a whole clip fills all slots
+    assert [m.slot_frame(s) for s in range(3)] == [(46, 42)] * 3
+    other.restore(0, 0)
+    m.sync()
+
+
+@gpu
 def test_streams_on_a_stream_of_their_own(pkg, Q, tmp_path):
     """The store is made on the stream it is used on: what the current stream
     does later does not reach it."""
