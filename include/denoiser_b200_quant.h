@@ -35,8 +35,9 @@ extern "C" {
  * the low half), and scales [capacity][cols / group]. `group` divides cols;
  * 0 = cols (one scale a row). Rows are counted in 64 bits, so a cache may
  * exceed 2^32 bytes; capacity < 2^31. All `capacity` rows have their ld_codes
- * bytes; those behind a row's codes are not written. Any alignment is right;
- * `codes` and ld_codes multiples of 16 are fastest.
+ * bytes; those behind a row's codes are not written. Any alignment of `codes`
+ * and ld_codes is right; multiples of 16 are fastest. Everything else is
+ * aligned to its type (DN_ERR_INVALID_ARG otherwise).
  *
  * The launchers run on the current device, which `stream` and the tensors
  * belong to. Calls that may overlap must not write what another one reads or

@@ -683,6 +683,15 @@ int run_read(const ReadArgs& a, int batch, int dtype, cudaStream_t s, const char
     return e == cudaSuccess ? DN_OK : dn_cuda_fail(e, name);
 }
 
+// The kernels read row numbers, page tables and lengths as the words that they are.
+int check_words(const void* slots, const void* table, const void* lengths, const void* err, const std::string& name) {
+    if (!aligned(slots, 8)) return dn_fail_str(DN_ERR_INVALID_ARG, name + ": slots must be 8-byte aligned");
+    if (!aligned(table, 4) || !aligned(lengths, 4))
+        return dn_fail_str(DN_ERR_INVALID_ARG, name + ": page table and lengths must be 4-byte aligned");
+    if (!aligned(err, 4)) return dn_fail_str(DN_ERR_INVALID_ARG, name + ": the error word must be 4-byte aligned");
+    return DN_OK;
+}
+
 // The shape of a cache: DN_OK, or the status of what is wrong with it.
 int check_cache(const void* codes, int64_t ldc, const float* scales, int64_t capacity, int cols, int bits, int& group,
                 int dtype, const std::string& name) {
@@ -752,6 +761,7 @@ int dn_launch_cache_write(const void* x, int dtype, int64_t ldx, int64_t rows, i
     const char* name = "dn_launch_cache_write";
     DN_TRY(check_cache(codes, ld_codes, scales, capacity, cols, bits, group, dtype, name));
     DN_TRY(check_rows(x, dtype, rows, ldx, cols, name));
+    DN_TRY(check_words(slots, nullptr, nullptr, err_dev, name));
     if (!slots && (row0 < 0 || row0 > capacity - rows))
         return dn_fail(DN_ERR_INVALID_ARG, "dn_launch_cache_write: rows outside the cache");
     if (rows == 0) return DN_OK;
@@ -766,6 +776,7 @@ int dn_launch_cache_read_rows(const void* codes, int64_t ld_codes, const float* 
     const char* name = "dn_launch_cache_read_rows";
     DN_TRY(check_cache(codes, ld_codes, scales, capacity, cols, bits, group, dtype, name));
     DN_TRY(check_rows(out, dtype, rows, ldo, cols, name));
+    DN_TRY(check_words(slots, nullptr, nullptr, err_dev, name));
     if (!slots && (row0 < 0 || row0 > capacity - rows))
         return dn_fail(DN_ERR_INVALID_ARG, "dn_launch_cache_read_rows: rows outside the cache");
     if (rows == 0) return DN_OK;
@@ -799,6 +810,7 @@ int dn_launch_cache_read_pages(const void* codes, int64_t ld_codes, const float*
     if (table_cols < 0 || table_cols >= (1LL << 31) || (batch > 1 && table_ld < table_cols))
         return dn_fail(DN_ERR_INVALID_ARG, "dn_launch_cache_read_pages: bad page table");
     DN_TRY(check_rows(out, dtype, max_rows, ldo, cols, name));
+    DN_TRY(check_words(nullptr, table, lengths, err_dev, name));
     const int64_t rows = std::min(max_rows, table_cols * page_rows);
     if (rows == 0 || batch == 0) return DN_OK;
     if (!table) return dn_fail(DN_ERR_INVALID_ARG, "dn_launch_cache_read_pages: null page table");

@@ -119,6 +119,21 @@ def test_cache_read_refuses(pkg, bad):
     assert rc == (pkg.DN_ERR_DTYPE if "dtype" in bad else pkg.DN_ERR_INVALID_ARG)
 
 
+def test_row_numbers_and_tables_that_are_not_aligned_to_their_type_are_refused(pkg):
+    """A kernel's load of such a word would be a fault. (No rows: what passes the check launches nothing.)"""
+    lib, bad = pkg.lib(), pkg.DN_ERR_INVALID_ARG
+    for off in (1, 2, 4):
+        assert lib.dn_launch_cache_write(*write_args(slots=FAKE + off, rows=0)) == bad
+        assert lib.dn_launch_cache_read_rows(FAKE, 32, FAKE, 8, 32, 8, 0, FAKE + off, 0, 0, FAKE, 1, 32, None, None) == bad
+    for off in (1, 2):
+        for k in (dict(table=FAKE + off), dict(lengths=FAKE + off), dict(err=FAKE + off)):
+            assert lib.dn_launch_cache_read_pages(*read_args(max_rows=0, **k)) == bad
+        assert lib.dn_launch_cache_write(*write_args(err=FAKE + off, rows=0)) == bad
+        assert lib.dn_launch_cache_read_rows(FAKE, 32, FAKE, 8, 32, 8, 0, None, 0, 0, FAKE, 1, 32, FAKE + off, None) == bad
+    assert lib.dn_launch_cache_write(*write_args(slots=FAKE + 8, err=FAKE + 4, rows=0)) == pkg.DN_OK
+    assert lib.dn_launch_cache_read_pages(*read_args(table=FAKE + 4, lengths=FAKE + 4, err=FAKE + 4, max_rows=0)) == pkg.DN_OK
+
+
 def test_nothing_to_do_needs_no_gpu(pkg):
     assert pkg.lib().dn_launch_cache_write(*write_args(rows=0, x=None)) == pkg.DN_OK
     for k in (dict(max_rows=0, out=None), dict(table_cols=0), dict(batch=0)):
