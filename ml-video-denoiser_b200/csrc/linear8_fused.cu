@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(Shape<PLANES, SG, NT>::kThreads) product_fused
     __shared__ uint32_t tslot;
     __shared__ volatile int s_abort;
     __shared__ float s_x[2][kRows];       // the tokens' scales, of this and the previous tile
-    __shared__ float2 s_par[NT];          // scale and bias of each weight row
+    __shared__ __align__(16) float2 s_par[NT];  // scale and bias of each weight row, read two at a time
     const ProductArgs& p = g.p;
     const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
     uint8_t* sa = smem;
