@@ -79,7 +79,8 @@ int dn_launch_cache_read_pages(const void* codes, int64_t ld_codes, const float*
  * Linear8: y[m, n] = s_x[m] s_w[n] sum_k q_x[m, k] q_w[n, k] + bias[n], the
  * tokens quantised to 8 bits with a scale each, the weights with a scale for
  * each output channel; the sum is exact in int32, the rest FP32, rounded once
- * to the output type. With `gate` (SimpleGate) the output has half the
+ * to the output type; what lies between overflows only where the product (with
+ * segments: a segment's part of it) does, whatever the scales. With `gate` (SimpleGate) the output has half the
  * channels: out[m, c] = y[m, c] * y[m, c + Cout / 2].
  *
  * segments > 1: the input channels are `segments` equal runs, each with a

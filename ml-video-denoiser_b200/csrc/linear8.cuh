@@ -75,6 +75,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, int (&r)[32]) {
         : "r"(taddr));
 }
 
+// An output is (sum s) w + b, s its token's scale, w and b its channel's: a sum
+// is below 2^31 (all segments of a token together), so that sum * s stays below
+// 2^128 as long as s is below this. Tokens with a larger scale (FP32 values of
+// 2^103 or more; FP16 ones never have one) take (sum w) s + b: there sum * w
+// overflows only where the output does.
+constexpr float kLargeScale = 7.9228163e28f;  // 2^96
+
 __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])

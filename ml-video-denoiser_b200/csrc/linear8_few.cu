@@ -172,7 +172,9 @@ __global__ void __launch_bounds__(kThreads) product_few_kernel(const __grid_cons
     float y = 0.f;
     if (in) {
         const float2 wb = __ldg(p.par + o + (p.gate && (j & 1) ? p.npad : 0));
-        y = fmaf(static_cast<float>(mine) * s_scale[r], wb.x, wb.y);
+        const float s = s_scale[r];
+        const bool large = s >= kLargeScale;
+        y = fmaf(static_cast<float>(mine) * (large ? wb.x : s), large ? s : wb.x, wb.y);
     }
     if (p.gate) y *= __shfl_down_sync(0xffffffffu, y, 1);
     if (in && r < rows && !(p.gate && (j & 1))) {

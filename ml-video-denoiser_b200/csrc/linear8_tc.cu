@@ -29,6 +29,7 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "denoiser_b200.h"
 #include "launch.cuh"
@@ -85,6 +86,16 @@ __device__ __forceinline__ void finish32(const float2* par, float (&y)[32]) {
         const float4 w = __ldg(reinterpret_cast<const float4*>(par + i));
         const float2 z = ffma2(make_float2(y[i], y[i + 1]), make_float2(w.x, w.z), make_float2(w.y, w.w));
         y[i] = z.x, y[i + 1] = z.y;
+    }
+}
+
+// 32 columns of tokens some of which have a large scale (see kLargeScale).
+__device__ __forceinline__ void finish32_large(const float2* par, const int (&a)[32], float s, float (&y)[32]) {
+    const bool large = s >= kLargeScale;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        const float2 w = __ldg(par + i);
+        y[i] = fmaf(static_cast<float>(a[i]) * (large ? w.x : s), large ? s : w.x, w.y);
     }
 }
 
@@ -316,9 +327,12 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
         load_scales(blockIdx.x);
         for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
             const float s = next[0];
+            [[maybe_unused]] bool large = false;
             if constexpr (SEG) {
 #pragma unroll
                 for (int t = 0; t < kScales; ++t) s_scale[warp][t][lane] = next[t];  // read by this lane alone
+#pragma unroll
+                for (int t = 0; t < kScales; ++t) large = large || next[t] >= kLargeScale;
             }
             load_scales(tile + gridDim.x);
             const int64_t m0 = static_cast<int64_t>(tile / g.n_tiles) * kRows + quad * 32;
@@ -333,36 +347,59 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
                 int col[kBlocks];
 #pragma unroll
                 for (int k = 0; k < kBlocks; ++k) col[k] = p.gate ? k * half + group * 32 : group * half + k * 32;
+                auto par_of = [&](int k) { return p.par + (p.gate ? k * p.npad + n0 + group * 32 : n0 + col[k]); };
                 bool ok = g.seg_full || full_wait(&bar_tile[n & 7], n >> 3);
                 if (!ok) break;
 #pragma unroll
                 for (int k = 0; k < kBlocks; ++k)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) y[k][i] = 0.f;
+                // The sums of the segments, scaled; any_large: a token of the warp
+                // has a large scale in one of them.
+                auto add_segments = [&](auto any_large) {
 #pragma unroll 1
-                for (int t = 0; t < p.segs; ++t) {
-                    const float st = s_scale[warp][t][lane];
-                    if (g.seg_full && !(ok = full_wait(&bar_acc_full[q % kAcc], q / kAcc))) break;
+                    for (int t = 0; t < p.segs; ++t) {
+                        const float st = s_scale[warp][t][lane];
+                        if (g.seg_full && !(ok = full_wait(&bar_acc_full[q % kAcc], q / kAcc))) break;
 #pragma unroll
-                    for (int k = 0; k < kBlocks; ++k) {
-                        int a[32];
-                        tmem_ld32(lane_base + (q % kAcc) * NT + col[k], a);
-                        tmem_ld_wait();
-                        const float2 st2 = make_float2(st, st);
+                        for (int k = 0; k < kBlocks; ++k) {
+                            int a[32];
+                            tmem_ld32(lane_base + (q % kAcc) * NT + col[k], a);
+                            tmem_ld_wait();
+                            const float2 st2 = make_float2(st, st);
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const float2 z = ffma2(make_float2(static_cast<float>(a[i]), static_cast<float>(a[i + 1])), st2,
-                                                   make_float2(y[k][i], y[k][i + 1]));
-                            y[k][i] = z.x, y[k][i + 1] = z.y;
+                            for (int i = 0; i < 32; i += 2) {
+                                float2 v = make_float2(static_cast<float>(a[i]), static_cast<float>(a[i + 1]));
+                                if constexpr (any_large) {
+                                    const float2* par = par_of(k) + i;
+                                    if (large) v.x *= __ldg(par).x, v.y *= __ldg(par + 1).x;
+                                }
+                                const float2 z = ffma2(v, st2, make_float2(y[k][i], y[k][i + 1]));
+                                y[k][i] = z.x, y[k][i + 1] = z.y;
+                            }
                         }
+                        acc_done(q);
+                        ++q;
                     }
-                    acc_done(q);
-                    ++q;
-                }
+                };
+                const bool any_large = __any_sync(0xffffffffu, large);
+                if (any_large)
+                    add_segments(std::true_type{});
+                else
+                    add_segments(std::false_type{});
                 if (!ok) break;
 #pragma unroll
-                for (int k = 0; k < kBlocks; ++k)
-                    finish32(p.par + (p.gate ? k * p.npad + n0 + group * 32 : n0 + col[k]), y[k]);
+                for (int k = 0; k < kBlocks; ++k) {
+                    if (any_large) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const float2 w = __ldg(par_of(k) + i);
+                            y[k][i] = fmaf(y[k][i], large ? 1.f : w.x, w.y);
+                        }
+                    } else {
+                        finish32(par_of(k), y[k]);
+                    }
+                }
                 if (p.gate) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) y[0][i] *= y[kBlocks - 1][i];
@@ -382,10 +419,15 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
             } else {
                 if (!full_wait(&bar_acc_full[q % kAcc], q / kAcc)) break;
                 const uint32_t acc = lane_base + (q % kAcc) * NT;
+                const bool large = __any_sync(0xffffffffu, s >= kLargeScale);
                 auto scaled = [&](int c, const float2* par, float (&y)[32]) {
                     int a[32];
                     tmem_ld32(acc + c, a);
                     tmem_ld_wait();
+                    if (large) {
+                        finish32_large(par, a, s, y);
+                        return;
+                    }
 #pragma unroll
                     for (int i = 0; i < 32; ++i) y[i] = static_cast<float>(a[i]) * s;
                     finish32(par, y);

@@ -583,6 +583,57 @@ def test_rows_that_are_not_finite_stay_by_themselves(Q, rows, k):
     np.testing.assert_array_equal(pix[0, :, 0].T, got)
 
 
+def far_rows(rng, rows, k):
+    """FP32 tokens from 2^-100 to the largest numbers, far ones beside ordinary ones."""
+    x = rng.standard_normal((rows, k)) * 2.0 ** np.resize([0, 125, -100, 96, 103, 124, 20], rows)[:, None]
+    return np.clip(x, -np.finfo(np.float32).max, np.finfo(np.float32).max).astype(np.float32)
+
+
+@gpu
+@pytest.mark.parametrize("rows,k,n", [(1, 512, 40), (2, 64, 8), (3, 300, 66), (7, 512, 1024), (13, 1000, 34),
+                                      (150, 512, 96), (260, 100, 200), (700, 1030, 520), (129, 64, 30)])
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("y_type", [torch.float16, torch.float32])
+def test_tokens_far_from_one(Q, rows, k, n, gate, y_type):
+    """The output is finite although the sum of codes times the token's scale is
+    not (and the sum times the channel's scale alone is far below one)."""
+    rng = np.random.default_rng(rows + n)
+    x = far_rows(rng, rows + 1, k)[1:]  # the single token is a far one
+    w = (rng.standard_normal((n, k)) * 2.0 ** -120 / np.sqrt(k)).astype(np.float32)
+    b = rng.standard_normal(n).astype(np.float32)
+    layer = Q.Linear8.from_tensors(dev(w), dev(b), gate=gate)
+    q, s = qo.quantise(x)
+    y, e = qo.product(q, s, *qo.quantise(w), b, gate)
+    sums = q.astype(np.float64) @ qo.quantise(w)[0].astype(np.float64).T
+    assert np.abs(sums * s).max() > 2.0 ** 128 and np.abs(y).max() < 60000
+    got = host(layer(dev(x), out_dtype=y_type))
+    layer.sync()
+    assert np.isfinite(got).all()
+    assert_product(got, y, e)
+
+
+@gpu
+@pytest.mark.parametrize("frames,rows,cols,n", [(1, 300, 64, 64), (2, 130, 20, 6), (3, 203, 96, 100), (5, 170, 64, 64),
+                                                (8, 390, 128, 256)])
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("y_type", [torch.float16, torch.float32])
+def test_cached_rows_far_from_one(Q, frames, rows, cols, n, gate, y_type):
+    rng = np.random.default_rng(frames + rows)
+    x = far_rows(rng, frames * rows, cols)
+    w = (rng.standard_normal((n, frames * cols)) * 2.0 ** -120 / np.sqrt(cols)).astype(np.float32)
+    b = rng.standard_normal(n).astype(np.float32)
+    layer = Q.Linear8.from_tensors(dev(w), dev(b), gate=gate, segments=frames)
+    cache = Q.RowCache(frames, rows, cols)
+    cache.write(dev(x))
+    q, s = (np.concatenate(list(a.reshape(frames, rows, -1)), 1) for a in qo.quantise(x))
+    y, e = qo.product(q, s, *qo.quantise(w), b, gate, frames)
+    assert np.abs(y).max() < 60000
+    got = host(layer.forward_cached(cache, list(range(frames)), out_dtype=y_type))
+    layer.sync()
+    assert np.isfinite(got).all()
+    assert_product(got, y, e)
+
+
 @gpu
 def test_the_longest_sum(Q):
     """131072 channels, every product of codes 127 * 127: the int32 sum's limit."""
