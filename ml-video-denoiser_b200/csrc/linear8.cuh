@@ -118,6 +118,17 @@ __device__ __forceinline__ bool elect_one() {
     return e != 0;
 }
 
+// After a wait that ran out: the MMAs that the elected lane of this warp has
+// issued end before the CTA gives back its TMEM and shared memory. `bar`: a
+// barrier of one arrival, not used otherwise. Warp-wide.
+__device__ __forceinline__ void drain_mmas(uint64_t* bar) {
+    if (elect_one()) {
+        mma_commit(bar);
+        mbar_wait(bar, 0, 100000000ull);
+    }
+    __syncwarp();
+}
+
 // The warp's index as a value that the compiler knows to be warp-uniform.
 __device__ __forceinline__ int warp_index() { return __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0); }
 

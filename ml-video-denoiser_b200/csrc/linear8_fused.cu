@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(Shape<PLANES, SG, NT>::kThreads) product_fused
     using Q = QuantOf<__half>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    __shared__ uint64_t bar;
+    __shared__ uint64_t bar, bar_end;
     __shared__ uint32_t tslot;
     __shared__ volatile int s_abort;
     __shared__ float s_x[2][kRows];       // the tokens' scales, of this and the previous tile
@@ -97,6 +97,7 @@ __global__ void __launch_bounds__(Shape<PLANES, SG, NT>::kThreads) product_fused
     }
     if (tid == 0) {
         mbar_init(&bar, 1);
+        mbar_init(&bar_end, 1);
         s_abort = 0;
         fence_mbar_init();
         if (g.tma_out) prefetch_tmap(&out_map);
@@ -323,7 +324,10 @@ __global__ void __launch_bounds__(Shape<PLANES, SG, NT>::kThreads) product_fused
     if (!PLANES && g.tma_out && lane == 0) bulk_wait_read0();
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) tmem_dealloc(tmem, kCols);
+    if (warp == 0) {
+        if (s_abort) drain_mmas(&bar_end);
+        tmem_dealloc(tmem, kCols);
+    }
 }
 
 template <typename T, bool PLANES, int SG, int NT, bool RUN>

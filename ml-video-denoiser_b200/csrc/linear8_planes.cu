@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(kThreads) product_planes_kernel(const __grid_c
     using Q = QuantOf<__half>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    __shared__ uint64_t bar, bar_in[2];
+    __shared__ uint64_t bar, bar_in[2], bar_end;
     __shared__ uint32_t tslot;
     __shared__ volatile int s_abort;
     __shared__ float s_x[2][kRows];
@@ -81,6 +81,7 @@ __global__ void __launch_bounds__(kThreads) product_planes_kernel(const __grid_c
     }
     if (tid == 0) {
         mbar_init(&bar, 1);
+        mbar_init(&bar_end, 1);
         mbar_init(&bar_in[0], 1);
         mbar_init(&bar_in[1], 1);
         s_abort = 0;
@@ -257,10 +258,13 @@ __global__ void __launch_bounds__(kThreads) product_planes_kernel(const __grid_c
     tc_fence_before();
     __syncthreads();
     if (warp == 0) {
-        // After a wait that ran out: the loads in flight land before the CTA leaves.
-        if (elect_one() && s_abort)
-            for (int k = max(0, issued - 2); k < issued; ++k) mbar_wait(&bar_in[k & 1], (k >> 1) & 1, 100000000ull);
-        __syncwarp();
+        // After a wait that ran out: the loads and MMAs in flight end before the CTA leaves.
+        if (s_abort) {
+            if (elect_one())
+                for (int k = max(0, issued - 2); k < issued; ++k) mbar_wait(&bar_in[k & 1], (k >> 1) & 1, 100000000ull);
+            __syncwarp();
+            drain_mmas(&bar_end);
+        }
         tmem_dealloc(tmem, kCols);
     }
 }

@@ -109,7 +109,8 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
     constexpr uint32_t kCols = kAcc * NT;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    __shared__ uint64_t bar_full[P::kStages], bar_empty[P::kStages], bar_b, bar_acc_full[kAcc], bar_acc_empty[kAcc], bar_tile[8];
+    __shared__ uint64_t bar_full[P::kStages], bar_empty[P::kStages], bar_b, bar_acc_full[kAcc], bar_acc_empty[kAcc], bar_tile[8],
+        bar_end;
     // A tile's scales, [segment][token] per epilogue warp.
     __shared__ float s_scale[SEG ? kEpiWarps : 1][SEG ? kMaxSegments : 1][32];
     __shared__ uint32_t tslot;
@@ -128,6 +129,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
             mbar_init(&bar_empty[s], 1);
         }
         mbar_init(&bar_b, 1);
+        mbar_init(&bar_end, 1);
         // The ring holds at most four tiles of two segments, so that a tile's
         // barrier is waited for before it comes round again.
         for (int b = 0; b < 8; ++b) mbar_init(&bar_tile[b], 1);
@@ -162,8 +164,9 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
                 tma_load_2d(sb, &maps.b, k, 0, &bar_b);
                 if (p.gate) tma_load_2d(sb + half * kc, &maps.b, k, p.n_out, &bar_b);
             }
-            // It has landed before this CTA leaves, whatever became of the others.
-            wait_or_abort(&bar_b, 0, &s_abort, p.err, 0x77);
+            // It has landed before this CTA leaves, whatever became of the others
+            // (another role's timeout ends the first wait at once).
+            if (!wait_or_abort(&bar_b, 0, &s_abort, p.err, 0x77)) mbar_wait(&bar_b, 0, 100000000ull);
         }
     } else if (warp == 8) {
         const uint32_t bytes = static_cast<uint32_t>(g.box_rows * kc * units);
@@ -269,6 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
                 if (++b == kAcc) b = 0, acc_ph ^= 1;
             }
         }
+        if (!ok) drain_mmas(&bar_end);
     } else {
         const int quad = warp & 3, group = warp >> 2;
         uint8_t* stg = smem + P::kRing + warp * kStgWarp;
