@@ -153,6 +153,12 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
     constexpr int half = NT / 2;
     const int out_cols = p.gate ? half : NT;  // output columns of a tile
 
+    // Whole warps run the loops of warps 8 to 10 and elect a lane in them, which
+    // every lane has to reach. Where a wait ends at another role's timeout the
+    // lanes' answers (ok) may differ, so a lane that has given up goes through
+    // the rest of the tile, waiting and issuing no more, and the warp leaves
+    // together. (A vote at every wait: 5 x 2088960 x 32 -> 32 218.4 us, 216.5 this way.)
+    auto leaves = [](bool ok) { return !__all_sync(0xffffffffu, ok); };
     uint8_t* b_res = smem + kSt * g.stage;  // resident weight: its chunks one behind the other
     const int seg_c = p.seg_c, segs = p.segs, chunks = g.chunks, kc = g.kc, units = g.units, stage = g.stage;
     if (warp == 9 && g.resident) {
@@ -173,23 +179,23 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
         int filled = 0, left = 0, s = 0;  // stages begun, chunks that the current one still takes
         uint32_t ph = 1;
         bool ok = true;
-        for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
             const int m0 = (tile / g.n_tiles) * kRows;
-            for (int t = 0; ok && t < segs; ++t) {
+            for (int t = 0; t < segs; ++t) {
                 const int row = static_cast<int>(p.arow[t]) + m0;
                 for (int j = 0; j < chunks; ++j) {
                     if (left == 0) {
-                        ok = wait_or_abort(&bar_empty[s], ph, &s_abort, p.err, 0x70);
-                        if (!ok) break;
-                        if (elect_one()) mbar_arrive_expect_tx(&bar_full[s], bytes);
+                        ok = ok && wait_or_abort(&bar_empty[s], ph, &s_abort, p.err, 0x70);
+                        if (elect_one() && ok) mbar_arrive_expect_tx(&bar_full[s], bytes);
                         left = units;
-                        ++filled;
+                        if (ok) ++filled;
                     }
                     uint8_t* sa = smem + s * stage + (units - left) * (kRows * kc);
-                    if (elect_one()) tma_load_2d(sa, &maps.a, j * kc, row, &bar_full[s]);
+                    if (elect_one() && ok) tma_load_2d(sa, &maps.a, j * kc, row, &bar_full[s]);
                     if (--left == 0 && ++s == kSt) s = 0, ph ^= 1;
                 }
             }
+            if (leaves(ok)) break;
         }
         // After a wait that ran out: the copies in flight land before the CTA leaves.
         if (!ok)
@@ -199,25 +205,25 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
         int filled = 0, s = 0;
         uint32_t ph = 1;
         bool ok = true;
-        for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
             const int n0 = (tile % g.n_tiles) * out_cols;
-            for (int t = 0; ok && t < segs; ++t)
+            for (int t = 0; t < segs; ++t)
                 for (int j = 0; j < chunks; ++j) {
                     // The ring filled up once ahead of the earlier kernels; what
                     // empties it waits for them, however long they take.
                     if (filled == kSt) pdl_wait();
-                    ok = wait_or_abort(&bar_empty[s], ph, &s_abort, p.err, 0x70);
-                    if (!ok) break;
+                    ok = ok && wait_or_abort(&bar_empty[s], ph, &s_abort, p.err, 0x70);
                     uint8_t* sb = smem + s * stage + kStageA;
                     const int k = t * p.seg_p + j * kc;
-                    if (elect_one()) {
+                    if (elect_one() && ok) {
                         mbar_arrive_expect_tx(&bar_full[s], bytes);
                         tma_load_2d(sb, &maps.b, k, n0, &bar_full[s]);
                         if (p.gate) tma_load_2d(sb + half * kc, &maps.b, k, p.n_out + n0, &bar_full[s]);
                     }
-                    ++filled;
+                    if (ok) ++filled;
                     if (++s == kSt) s = 0, ph ^= 1;
                 }
+            if (leaves(ok)) break;
         }
         if (!ok)
             for (int k = max(0, filled - kSt); k < filled; ++k) mbar_wait(&bar_full[k % kSt], (k / kSt) & 1, 100000000ull);
@@ -233,24 +239,22 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
         uint32_t ph = 0, acc_ph = 1;
         uint64_t ad = ad0;
         bool ok = !g.resident || wait_or_abort(&bar_b, 0, &s_abort, p.err, 0x78);
-        for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++n) {
+        for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++n) {
             uint64_t bd = bd0;  // of the chunk, but for the stage
-            for (int t = 0; ok && t < segs; ++t) {
-                ok = wait_or_abort(&bar_acc_empty[b], acc_ph, &s_abort, p.err, 0x71);
-                if (!ok) break;
+            for (int t = 0; t < segs; ++t) {
+                ok = ok && wait_or_abort(&bar_acc_empty[b], acc_ph, &s_abort, p.err, 0x71);
                 tc_fence_after();
                 const uint32_t acc = tmem + b * NT;
                 int steps_left = (seg_c + 31) / 32;
                 for (int j = 0; j < chunks; ++j) {
                     if (left == 0) {
-                        ok = wait_or_abort(&bar_full[s], ph, &s_abort, p.err, 0x72);
-                        if (!ok) break;
+                        ok = ok && wait_or_abort(&bar_full[s], ph, &s_abort, p.err, 0x72);
                         tc_fence_after();
                         left = units;
                         ad = ad0 + static_cast<uint32_t>(s * (stage >> 4));
                     }
                     const uint64_t bs = bd + s * b_stage;
-                    if (elect_one()) {
+                    if (elect_one() && ok) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             if (k < steps_left && k * 32 < kc)
@@ -271,8 +275,9 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
                 }
                 if (++b == kAcc) b = 0, acc_ph ^= 1;
             }
+            if (leaves(ok)) break;
         }
-        if (!ok) drain_mmas(&bar_end);
+        if (leaves(ok)) drain_mmas(&bar_end);
     } else {
         const int quad = warp & 3, group = warp >> 2;
         uint8_t* stg = smem + P::kRing + warp * kStgWarp;
