@@ -953,6 +953,7 @@ int Engine::make_shape(int N, int T, int C, int H, int W, Shape& sh) {
     try {
         plan(sh);
     } catch (const std::exception& e) {
+        cudaGetLastError();  // reported here, so it is not the next launch's error
         return dn_fail(DN_ERR_CUDA, e.what());
     }
     return DN_OK;

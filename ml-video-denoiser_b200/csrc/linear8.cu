@@ -264,7 +264,6 @@ int create(const void* weight, int dtype, int64_t ldw, const void* bias, int cou
     const cudaError_t e = lay_out(L.get(), weight, dtype, ldw, bias, s, rc);
     if (e != cudaSuccess || rc != DN_OK) {
         cudaFree(L->arena);
-        cudaGetLastError();  // a failed allocation is not the next launch's error
         return rc != DN_OK ? rc : dn_cuda_fail(e, "dn_linear8_create: upload");
     }
     *out = L.release();

@@ -21,6 +21,7 @@ int dn_fail_str(int code, const std::string& msg) {
 }
 
 int dn_cuda_fail(cudaError_t e, const char* where) {
+    cudaGetLastError();  // reported here, so it is not the next launch's error
     g_last_error = std::string(where) + ": " + cudaGetErrorString(e);
     return DN_ERR_CUDA;
 }

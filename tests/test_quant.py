@@ -688,6 +688,28 @@ def test_layers_from_a_store_and_from_tensors_are_the_same(pkg, Q, tmp_path):
 
 
 @gpu
+def test_a_layer_that_finds_no_memory_does_not_fail_the_next_one(pkg, Q, tmp_path):
+    """The failed allocation is reported once, by the call that made it."""
+    big, small = np.zeros((4096, 4096), np.float16), np.ones((8, 16), np.float16)
+    store = store_of(pkg, tmp_path, {"big.weight": big, "small.weight": small})
+    Q.Linear8(store, "small.weight")(torch.ones(2, 16, dtype=torch.float16, device="cuda"))
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    taken = []
+    while torch.cuda.mem_get_info()[0] > 60 << 20:  # the layer's weight passes through 64 MB
+        taken.append(torch.empty(torch.cuda.mem_get_info()[0] - (40 << 20), dtype=torch.uint8, device="cuda"))
+    with pytest.raises(pkg.DenoiserError) as e:
+        Q.Linear8(store, "big.weight")
+    assert e.value.code == pkg.DN_ERR_CUDA
+    del taken
+    torch.cuda.empty_cache()
+    layer = Q.Linear8(store, "small.weight")
+    x = torch.ones(2, 16, dtype=torch.float16, device="cuda")
+    assert bool((layer(x) == 16).all())
+    Q.Linear8(store, "big.weight")
+
+
+@gpu
 def test_layers_of_a_device_that_is_not_there_are_refused(pkg, tmp_path):
     store = store_of(pkg, tmp_path, {"b.weight": np.ones((4, 16), np.float16)})
     w, lib, h = torch.ones(4, 16, dtype=torch.float16, device="cuda"), pkg.lib(), ctypes.c_void_p()
