@@ -109,12 +109,14 @@ int dn_linear8_info(const dn_linear8* layer, int* out_channels, int* in_channels
  * itself may be shared by any number of calls. */
 int dn_linear8_workspace(const dn_linear8* layer, int64_t rows, int dtype, int nchw, int64_t* bytes);
 /* Token rows: x [rows][Cin] (row stride ldx) -> out [rows][out_channels] (row
- * stride ldo), unit column strides, the two apart from each other. Segments
- * must be 1. */
+ * stride ldo), unit column strides, the two apart from each other (columns
+ * side by side of one buffer are; DN_ERR_INVALID_ARG otherwise). Segments must
+ * be 1. */
 int dn_linear8_forward(dn_linear8* layer, const void* x, int dtype, int64_t ldx, int64_t rows, void* out, int out_dtype,
                        int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream);
 /* A 1x1 convolution over NCHW planes: input (N, Cin, H, W) -> output
- * (N, out_channels, H, W), both FP16 and contiguous; a pixel is a token. */
+ * (N, out_channels, H, W), both FP16 and contiguous, apart from each other; a
+ * pixel is a token. */
 int dn_linear8_forward_nchw(dn_linear8* layer, const void* input, int N, int H, int W, void* output, void* workspace,
                             int64_t workspace_bytes, void* stream);
 /* Straight from an 8-bit row cache with one scale a row and

@@ -298,6 +298,18 @@ int check_matrix(const void* p, int dtype, int64_t rows, int64_t ld, int64_t col
     return DN_OK;
 }
 
+// Whether rows of x (xb bytes, stride xs) and of out (ob bytes, stride os) share
+// bytes: tokens are read while others' outputs are written. Columns side by
+// side of one buffer (one stride) do not; of rows that lie among each other with
+// two strides it is taken that they do.
+bool share_bytes(const void* x, int64_t xs, int64_t xb, const void* out, int64_t os, int64_t ob, int64_t rows) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(out);
+    if (a + (rows - 1) * xs + xb <= b || b + (rows - 1) * os + ob <= a) return false;
+    if (rows == 1 || xs != os) return true;
+    const int64_t d = (static_cast<int64_t>(b - a) % xs + xs) % xs;
+    return d < xb || d + ob > xs;
+}
+
 // How the product of `rows` tokens runs. One pass where the tokens are few or
 // the layer is narrow; otherwise the tokens are quantised into the workspace
 // and the product reads their codes. (Narrow layers in one pass and in two:
@@ -413,6 +425,9 @@ int dn_linear8_forward(dn_linear8* L, const void* x, int dtype, int64_t ldx, int
     DN_TRY(check_matrix(x, dtype, rows, ldx, L->cin, name));
     DN_TRY(check_matrix(out, out_dtype, rows, ldo, L->n_out(), name));
     if (rows == 0) return DN_OK;
+    const int xe = dtype == 1 ? 2 : 4, oe = out_dtype == 1 ? 2 : 4;
+    if (share_bytes(x, ldx * xe, static_cast<int64_t>(L->cin) * xe, out, ldo * oe, static_cast<int64_t>(L->n_out()) * oe, rows))
+        return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_forward: input and output overlap");
     ProductArgs a = product_args(L);
     a.rows = rows;
     a.out = out;
@@ -447,6 +462,8 @@ int dn_linear8_forward_nchw(dn_linear8* L, const void* input, int N, int H, int 
     DN_TRY(check_matrix(input, 1, rows, L->cin, L->cin, name));
     DN_TRY(check_matrix(output, 1, rows, L->n_out(), L->n_out(), name));
     if (rows == 0) return DN_OK;
+    if (share_bytes(input, 0, rows * L->cin * 2, output, 0, rows * L->n_out() * 2, 1))
+        return dn_fail(DN_ERR_INVALID_ARG, "dn_linear8_forward_nchw: input and output overlap");
     ProductArgs a = product_args(L);
     a.rows = rows;
     a.out = output;

@@ -340,7 +340,8 @@ class Linear8:
 
     def forward(self, x, out=None, out_dtype=None, stream=None):
         """Token rows x (rows, in_channels), FP16 or FP32, any row stride that
-        holds a row -> (rows, out_channels) in ``out_dtype`` (default: x's) or into ``out``."""
+        holds a row -> (rows, out_channels) in ``out_dtype`` (default: x's) or into
+        ``out``, which may not share memory with x."""
         if _elsewhere(self.device, stream):
             with _on(self.device, stream):
                 return self.forward(x, out, out_dtype)
@@ -360,7 +361,8 @@ class Linear8:
 
     def forward_nchw(self, x, out=None, stream=None):
         """A 1x1 convolution: x (N, in_channels, H, W) FP16 contiguous ->
-        (N, out_channels, H, W) FP16, a scale for every pixel."""
+        (N, out_channels, H, W) FP16, a scale for every pixel; ``out`` may not
+        share memory with x."""
         if _elsewhere(self.device, stream):
             with _on(self.device, stream):
                 return self.forward_nchw(x, out)

@@ -635,6 +635,35 @@ def test_cached_rows_far_from_one(Q, frames, rows, cols, n, gate, y_type):
 
 
 @gpu
+def test_in_place_calls_are_refused_and_columns_side_by_side_are_not(pkg, Q):
+    rng = np.random.default_rng(5)
+    layer, (qw, sw, b) = make(Q, rng, 32, 32, False, True)
+    one = Q.Linear8.from_tensors(torch.ones(8, 32, dtype=torch.float16, device="cuda"))
+    for rows in (1, 3, 40, 300):
+        flat = torch.zeros(rows * 64 + 200, dtype=torch.float16, device="cuda")
+        x = flat[:rows * 32].view(rows, 32)
+        shifted = flat[16:16 + rows * 32].view(rows, 32)
+        wide = flat[:rows * 64].view(rows, 64)
+        floats = flat[:rows * 64].view(torch.float32).view(rows, 32)
+        for bad in (lambda: layer(x, out=x), lambda: layer(x, out=shifted), lambda: layer(shifted, out=x),
+                    lambda: layer(wide[:, :32], out=wide[:, 16:48]), lambda: layer(wide[:, 24:56], out=wide[:, :32]),
+                    lambda: layer(floats, out=wide[:, :32]), lambda: one(x, out=x[:, 24:]),
+                    lambda: layer.forward_nchw(x.view(1, 32, rows, 1), out=shifted.view(1, 32, rows, 1))):
+            with pytest.raises(pkg.InvalidArgumentError):
+                bad()
+        assert not bool(flat.any())
+        x0 = rows_of(rng, rows, 32)
+        y, e = qo.product(*qo.quantise(x0), qw, sw, b)
+        for i, o in ((slice(0, 32), slice(32, 64)), (slice(32, 64), slice(0, 32))):  # one buffer, side by side
+            wide[:, i] = dev(x0)
+            layer(wide[:, i], out=wide[:, o])
+            assert_product(host(wide[:, o]), y, e)
+            np.testing.assert_array_equal(host(wide[:, i]), x0)
+        x.copy_(dev(x0))  # one behind the other
+        assert_product(host(layer(x, out=flat[rows * 32:rows * 64].view(rows, 32))), y, e)
+
+
+@gpu
 def test_the_longest_sum(Q):
     """131072 channels, every product of codes 127 * 127: the int32 sum's limit."""
     k = 131072
