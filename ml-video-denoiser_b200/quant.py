@@ -112,16 +112,29 @@ class RowCache:
         self.device = _device_of(device)
         d = torch.device("cuda", self.device)
         row = ((cols * bits + 7) // 8 + 15) // 16 * 16
-        self.codes = torch.zeros(self.capacity, row, dtype=torch.uint8, device=d)
-        self.scales = torch.zeros(self.capacity, cols // group, dtype=torch.float32, device=d)
+        self._codes = torch.zeros(self.capacity, row, dtype=torch.uint8, device=d)
+        self._scales = torch.zeros(self.capacity, cols // group, dtype=torch.float32, device=d)
         self._err = torch.zeros(1, dtype=torch.int32, device=d)
         # The zeros are there before any call, whatever stream it is on. (In a
         # capture they are part of the graph, in front of what uses them.)
         with torch.cuda.device(d):
             if not torch.cuda.is_current_stream_capturing():
                 torch.cuda.current_stream(d).synchronize()
-        self._held = (self.codes.data_ptr(), row, self.scales.data_ptr(), self.capacity)
+        self._bind()
+
+    def _bind(self) -> None:
+        """The addresses that the calls take, of the tensors that this cache holds."""
+        self.device = self._codes.get_device()
+        self._held = (self._codes.data_ptr(), self._codes.shape[1], self._scales.data_ptr(), self.capacity)
         self._err_ptr = self._err.data_ptr()
+
+    def __setstate__(self, state) -> None:  # a copy or a loaded cache has tensors of its own
+        self.__dict__.update(state)
+        self._bind()
+
+    # Tensors to look at or write into; another one cannot take their place.
+    codes = property(lambda self: self._codes)
+    scales = property(lambda self: self._scales)
 
     def _slots(self, slots, rows: int | None):
         _on_device(slots, self.device, "RowCache: slots")
@@ -163,7 +176,7 @@ class RowCache:
         else:
             p, n = self._slots(slots, rows), slots.shape[0]
         if out is None:
-            out = torch.zeros(n, self.cols, dtype=dtype or torch.float16, device=self.codes.device)
+            out = torch.zeros(n, self.cols, dtype=dtype or torch.float16, device=self._codes.device)
         code = _code(out.dtype, "RowCache.read_rows")
         ldo = _matrix(out, n, self.cols, self.device, "RowCache.read_rows: out")
         codes, ld, scales, cap = self._held
@@ -191,7 +204,7 @@ class RowCache:
             if lengths.dtype is not torch.int32 or lengths.shape != (b,) or not lengths.is_contiguous():
                 _bad(f"RowCache.read: lengths must be a contiguous int32 tensor ({b},)")
         if out is None:
-            out = torch.zeros(b, n * self.page_rows, self.cols, dtype=dtype or torch.float16, device=self.codes.device)
+            out = torch.zeros(b, n * self.page_rows, self.cols, dtype=dtype or torch.float16, device=self._codes.device)
         code = _code(out.dtype, "RowCache.read")
         _on_device(out, self.device, "RowCache.read: out")
         if out.dim() != 3 or out.shape[0] != b or out.shape[2] != self.cols:
@@ -402,7 +415,7 @@ class Linear8:
         if not 0 <= rows <= cache.page_rows:
             _bad(f"Linear8.forward_cached: {rows} rows of pages of {cache.page_rows}")
         if out is None:
-            out = torch.empty(rows, self.out_channels, dtype=out_dtype or torch.float16, device=cache.codes.device)
+            out = torch.empty(rows, self.out_channels, dtype=out_dtype or torch.float16, device=cache._codes.device)
         code = _code(out.dtype, "Linear8.forward_cached: out")
         ldo = _matrix(out, rows, self.out_channels, self.device, "Linear8.forward_cached: out")
         codes, ld, scales, cap = cache._held

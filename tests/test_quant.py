@@ -149,6 +149,28 @@ def test_classes_refuse(pkg, Q):
         Q.Linear8.from_tensors(torch.zeros(4, 4))
 
 
+def test_a_copied_or_loaded_cache_uses_its_own_tensors(Q, monkeypatch):
+    """Not the addresses of the cache that it was made from. (Tensors of the CPU stand in.)"""
+    import contextlib
+    import copy
+    import pickle
+
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    zeros = torch.zeros
+    monkeypatch.setattr(torch, "zeros", lambda *a, device=None, **k: zeros(*a, **k))
+    cache = Q.RowCache(2, 3, 20, bits=4)
+    cache.codes.fill_(3)
+    for other in (copy.deepcopy(cache), pickle.loads(pickle.dumps(cache))):
+        assert other._held == (other.codes.data_ptr(), 16, other.scales.data_ptr(), 6)
+        assert other._err_ptr == other._err.data_ptr() != cache._err_ptr and other._held[0] != cache._held[0]
+        assert (other.pages, other.page_rows, other.cols, other.bits, other.group) == (2, 3, 20, 4, 20)
+        assert torch.equal(other.codes, cache.codes)
+    for name in ("codes", "scales"):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, torch.ones(1))
+
+
 def test_layer_create_refuses(pkg):
     lib, h = pkg.lib(), ctypes.c_void_p()
     for args in [(FAKE, 1, 8, None, 0, 8, 0, 1), (FAKE, 1, 8, None, 3, 8, 1, 1), (FAKE, 1, 8, None, 4, 8, 0, 3),
@@ -426,6 +448,27 @@ def test_pages(Q, bits, cols, group, page_rows, dtype):
     full = host(cache.read(dev(table[:1]), dtype=dtype))
     r = (table[0][:, None] * page_rows + np.arange(page_rows)).ravel()
     assert_read(full[0], q[r], s[r])
+
+
+@gpu
+def test_a_copied_cache(pkg, Q):
+    import copy
+
+    rng = np.random.default_rng(12)
+    x, x2 = rows_of(rng, 9, 48), rows_of(rng, 9, 48)
+    cache = Q.RowCache(3, 3, 48)
+    cache.write(dev(x))
+    other = copy.deepcopy(cache)
+    other.write(dev(x2))
+    assert_held(cache, slice(None), *qo.quantise(x), 8)
+    assert_held(other, slice(None), *qo.quantise(x2), 8)
+    del cache
+    torch.cuda.empty_cache()
+    q, s = qo.quantise(x2)
+    assert_read(host(other.read_rows(rows=9)), q, s)
+    other.write(dev(x), slots=torch.full((9,), 9, device="cuda"))
+    with pytest.raises(pkg.DenoiserError):
+        other.sync()
 
 
 @gpu
