@@ -323,6 +323,9 @@ class Linear8:
         self.gate, self.segments = bool(vals[2].value), vals[3].value
         self._need = {}  # workspace bytes of the sizes met
 
+    def __reduce_ex__(self, protocol):  # two objects would destroy the one layer
+        raise TypeError("a Linear8 cannot be copied or pickled: make another one of its weights")
+
     def close(self) -> None:
         h = getattr(self, "_h", None)
         if h:

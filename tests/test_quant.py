@@ -171,6 +171,17 @@ def test_a_copied_or_loaded_cache_uses_its_own_tensors(Q, monkeypatch):
             setattr(cache, name, torch.ones(1))
 
 
+def test_a_layer_is_not_copied(Q):
+    import copy
+    import pickle
+
+    layer = Q.Linear8.__new__(Q.Linear8)
+    layer._h = None
+    for f in (copy.copy, copy.deepcopy, pickle.dumps):
+        with pytest.raises(TypeError):
+            f(layer)
+
+
 def test_layer_create_refuses(pkg):
     lib, h = pkg.lib(), ctypes.c_void_p()
     for args in [(FAKE, 1, 8, None, 0, 8, 0, 1), (FAKE, 1, 8, None, 3, 8, 1, 1), (FAKE, 1, 8, None, 4, 8, 0, 3),
