@@ -157,6 +157,8 @@ class RowCache:
         ldx = _matrix(x, None, self.cols, self.device, "RowCache.write: x")
         rows = x.shape[0]
         codes, ld, scales, cap = self._held
+        if slots is None and not 0 <= row0 <= cap:  # ctypes would cut a number that 64 bits do not hold
+            _bad(f"RowCache.write: row0 {row0} outside a cache of {cap} rows")
         check(lib().dn_launch_cache_write(
             x.data_ptr(), dtype, ldx, rows, self.cols, None if slots is None else self._slots(slots, rows), row0, codes,
             ld, scales, cap, self.bits, self.group, self._err_ptr, _stream(self.device)))
@@ -180,6 +182,8 @@ class RowCache:
         code = _code(out.dtype, "RowCache.read_rows")
         ldo = _matrix(out, n, self.cols, self.device, "RowCache.read_rows: out")
         codes, ld, scales, cap = self._held
+        if slots is None and not 0 <= row0 <= cap:
+            _bad(f"RowCache.read_rows: row0 {row0} outside a cache of {cap} rows")
         check(lib().dn_launch_cache_read_rows(codes, ld, scales, cap, self.cols, self.bits, self.group, p, row0, n,
                                               out.data_ptr(), code, ldo, self._err_ptr, _stream(self.device)))
         return out
@@ -422,6 +426,9 @@ class Linear8:
         code = _code(out.dtype, "Linear8.forward_cached: out")
         ldo = _matrix(out, rows, self.out_channels, self.device, "Linear8.forward_cached: out")
         codes, ld, scales, cap = cache._held
+        for p in pages:
+            if not 0 <= p < cache.pages:  # ctypes would cut a number that 64 bits do not hold
+                _bad(f"Linear8.forward_cached: page {p} of a cache of {cache.pages}")
         check(lib().dn_linear8_forward_cached(self._h, codes, ld, scales, cap, cache.page_rows,
                                               (ctypes.c_int64 * len(pages))(*pages), len(pages), rows, out.data_ptr(),
                                               code, ldo, _stream(self.device)))

@@ -182,6 +182,38 @@ def test_a_layer_is_not_copied(Q):
             f(layer)
 
 
+def test_row_numbers_that_no_64_bit_word_holds_are_refused(pkg, Q, monkeypatch):
+    """ctypes would cut them to a row or page that is there."""
+    import contextlib
+
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
+    monkeypatch.setattr(Q, "_stream", lambda d: 0)
+    zeros, empty = torch.zeros, torch.empty
+    monkeypatch.setattr(torch, "zeros", lambda *a, device=None, **k: zeros(*a, **k))
+    monkeypatch.setattr(torch, "empty", lambda *a, device=None, **k: empty(*a, **k))
+    calls = []
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *args: calls.append(args) or 0
+
+    monkeypatch.setattr(Q, "lib", Lib)
+    cache = Q.RowCache(4, 2, 16)
+    layer = Q.Linear8.__new__(Q.Linear8)
+    layer._h, layer.device, layer.segments, layer.in_channels, layer.out_channels = None, -1, 1, 16, 4
+    x = zeros(2, 16, dtype=torch.float16)
+    for far in (1 << 64, (1 << 64) + 1, -(1 << 64)):
+        for bad in (lambda: cache.write(x, row0=far), lambda: cache.read_rows(row0=far, rows=2),
+                    lambda: layer.forward_cached(cache, [far])):
+            with pytest.raises(pkg.InvalidArgumentError):
+                bad()
+    assert not calls
+    cache.write(x, row0=6), cache.read_rows(row0=6, rows=2), layer.forward_cached(cache, [3])
+    assert len(calls) == 3
+
+
 def test_layer_create_refuses(pkg):
     lib, h = pkg.lib(), ctypes.c_void_p()
     for args in [(FAKE, 1, 8, None, 0, 8, 0, 1), (FAKE, 1, 8, None, 3, 8, 1, 1), (FAKE, 1, 8, None, 4, 8, 0, 3),
