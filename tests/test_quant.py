@@ -403,6 +403,74 @@ def test_strides_and_alignment(Q):
 
 
 @gpu
+@pytest.mark.parametrize("cols,group", [(1, 0), (24, 0), (33, 0), (40, 8), (48, 16), (64, 0), (64, 32), (200, 0), (250, 0),
+                                        (256, 0), (300, 0), (512, 64), (1000, 0), (2049, 0), (2304, 0), (4608, 2304)])
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+def test_caches_of_any_alignment(pkg, cols, group, bits, dtype):
+    """The C entry points over codes that begin anywhere, with any stride that
+    holds a row: written (consecutive and scattered rows) and read back by row and
+    by page, and no byte beside a row's own is touched."""
+    rng = np.random.default_rng(cols + bits)
+    lib, stream = pkg.lib(), torch.cuda.current_stream().cuda_stream
+    code, t = (1, torch.float16) if dtype == np.float16 else (0, torch.float32)
+    rows, cap, page_rows, n = 13, 24, 5, bytes_of(cols, bits)
+    groups = cols // (group or cols)
+    x, x2 = rows_of(rng, rows, cols, dtype), rows_of(rng, rows, cols, dtype)
+    slots = rng.integers(-1, cap, rows)
+    slots[4], slots[9] = slots[1], slots[0]  # the later row counts
+    want = np.zeros((cap, cols), dtype)
+    want[3:3 + rows] = x
+    for r, at in enumerate(slots):
+        if at >= 0:
+            want[at] = x2[r]
+    q, s = qo.quantise(want, bits, group)
+    written = np.zeros(cap, bool)
+    written[3:3 + rows] = True
+    written[slots[slots >= 0]] = True
+    table = np.array([[4, 0, 2], [1, 1, 3]], np.int32)
+    for first, gap in ((0, 0), (1, 0), (2, 3), (4, 4), (8, 8), (3, 1), (16, (-n) % 16), (8, (-n) % 8), (4, (-n) % 4)):
+        ld = n + gap
+        flat = torch.full((16 + first + cap * ld + 16,), 0xa5, dtype=torch.uint8, device="cuda")
+        scales = torch.full((cap + 2, groups), -3.0, device="cuda")
+        err = torch.zeros(1, dtype=torch.int32, device="cuda")
+        p, ps = flat.data_ptr() + 16 + first, scales[1:].data_ptr()
+        dx, dx2, dslots = dev(x), dev(x2), dev(slots)
+        pkg.check(lib.dn_launch_cache_write(dx.data_ptr(), code, cols, rows, cols, None, 3, p, ld, ps, cap, bits, group,
+                                            err.data_ptr(), stream))
+        pkg.check(lib.dn_launch_cache_write(dx2.data_ptr(), code, cols, rows, cols, dslots.data_ptr(), 0, p, ld, ps, cap,
+                                            bits, group, err.data_ptr(), stream))
+        held = host(flat)
+        body = held[16 + first:16 + first + cap * ld].reshape(cap, ld)
+        np.testing.assert_array_equal(body[written][:, :n], qo.pack(q, bits)[written])
+        np.testing.assert_array_equal(host(scales)[1:-1][written], s[written])
+        assert (body[:, n:] == 0xa5).all() and (body[~written] == 0xa5).all() and (host(scales)[[0, -1]] == -3).all()
+        assert (held[:16 + first] == 0xa5).all() and (held[16 + first + cap * ld:] == 0xa5).all()
+        out = torch.full((rows, cols), 7.0, dtype=t, device="cuda")
+        pkg.check(lib.dn_launch_cache_read_rows(p, ld, ps, cap, cols, bits, group, dslots.data_ptr(), 0, rows, out.data_ptr(),
+                                                code, cols, err.data_ptr(), stream))
+        got = host(out)
+        assert (got[slots < 0] == 7).all()
+        assert_read(got[slots >= 0], q[slots[slots >= 0]], s[slots[slots >= 0]])
+        pkg.check(lib.dn_launch_cache_read_rows(p, ld, ps, cap, cols, bits, group, None, 3, rows, out.data_ptr(), code, cols,
+                                                err.data_ptr(), stream))
+        assert_read(host(out), q[3:3 + rows], s[3:3 + rows])
+        seqs = torch.full((2, 13, cols), 7.0, dtype=t, device="cuda")
+        dt, lengths = dev(table), dev(np.array([12, 7], np.int32))
+        pkg.check(lib.dn_launch_cache_read_pages(p, ld, ps, cap, cols, bits, group, page_rows, dt.data_ptr(), 3, 3,
+                                                 lengths.data_ptr(), 2, 13, seqs.data_ptr(), code, 13 * cols, cols,
+                                                 err.data_ptr(), stream))
+        got = host(seqs)
+        for b, length in enumerate((12, 7)):
+            at = (table[b][:, None] * page_rows + np.arange(page_rows)).ravel()[:length]
+            fine = (at < cap) & written[np.minimum(at, cap - 1)]  # the last page ends behind the cache
+            assert_read(got[b, :length][fine], q[at[fine]], s[at[fine]])
+            assert (got[b, :length][at >= cap] == 7).all() and (got[b, length:] == 7).all()
+        assert (host(flat) == held).all()
+        assert bool(err.item()) == bool((table * page_rows + page_rows > cap).any())
+
+
+@gpu
 @pytest.mark.parametrize("rows,cols,group", [(1, 32, 0), (40, 32, 0), (256, 24, 0), (300, 32, 0), (2000, 64, 16),
                                              (300, 33, 0), (90, 512, 32), (260, 2304, 0), (30, 2304, 0),
                                              (90, 333, 0), (400, 1001, 0), (2, 5, 0)])
