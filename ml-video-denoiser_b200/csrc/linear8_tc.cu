@@ -156,8 +156,9 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
     // Whole warps run the loops of warps 8 to 10 and elect a lane in them, which
     // every lane has to reach. Where a wait ends at another role's timeout the
     // lanes' answers (ok) may differ, so a lane that has given up goes through
-    // the rest of the tile, waiting and issuing no more, and the warp leaves
-    // together. (A vote at every wait: 5 x 2088960 x 32 -> 32 218.4 us, 216.5 this way.)
+    // the rest of the tile, waiting and loading no more (what it multiplies then
+    // is wasted), and the warp leaves together. (A vote at every wait: 5 x 2088960 x
+    // 32 -> 32 218.4 us, 215 this way.)
     auto leaves = [](bool ok) { return !__all_sync(0xffffffffu, ok); };
     uint8_t* b_res = smem + kSt * g.stage;  // resident weight: its chunks one behind the other
     const int seg_c = p.seg_c, segs = p.segs, chunks = g.chunks, kc = g.kc, units = g.units, stage = g.stage;
@@ -254,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_tc_kernel(const __grid_co
                         ad = ad0 + static_cast<uint32_t>(s * (stage >> 4));
                     }
                     const uint64_t bs = bd + s * b_stage;
-                    if (elect_one() && ok) {
+                    if (elect_one()) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             if (k < steps_left && k * 32 < kc)
