@@ -30,8 +30,8 @@ constexpr int kMaxK = 131072;  // 127 * 127 * 131072 < 2^31
 // registers; with pixel pairs the next `kept` ones stay in shared memory (each
 // lane its own vectors), what a very wide layer has beyond them is read again.
 // Single pixels read all of them again: there the occupancy is worth more (2
-// images of 36867 pixels, 1296 -> 26 gated: 152 us, 274 with 96 KB kept; pairs of
-// 36868: 112 us, 120 without).
+// images of 36867 pixels, 1296 -> 26 gated: 151 us, 274 with 96 KB kept; pairs of
+// 36868: 111 us, 120 without).
 template <int PX>
 __global__ void __launch_bounds__(256) quantise_planes_kernel(const __half* __restrict__ x, int64_t rows, int K, int64_t hw,
                                                               uint8_t* __restrict__ codes, int64_t ldc,

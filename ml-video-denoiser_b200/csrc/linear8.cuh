@@ -1,5 +1,6 @@
-// Device pieces shared by the tensor-core kernels of the 8-bit product
-// (linear8_tc.cu, linear8_fused.cu), and the tensor maps they use.
+// Device pieces shared by the kernels of the 8-bit product (linear8_tc.cu,
+// linear8_fused.cu, linear8_planes.cu, linear8_few.cu), and the tensor maps they
+// use.
 #pragma once
 
 #include <cuda.h>

@@ -1,5 +1,6 @@
 // Internal interface of the 8-bit product: what a launch needs, shared by the
-// layer (linear8.cu) and its kernels (linear8_tc.cu).
+// layer (linear8.cu) and its kernels (linear8_tc.cu, linear8_fused.cu,
+// linear8_planes.cu, linear8_few.cu).
 #pragma once
 
 #include <cuda_runtime.h>

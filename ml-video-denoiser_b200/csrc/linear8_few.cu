@@ -6,9 +6,10 @@
 // L2), behind the loads of its first weight bytes; a warp then takes CPW
 // weight rows at a time, a lane 16 bytes of each, and R tokens with dp4a:
 // each weight byte is used R times from registers, and the int32 sums meet in
-// one warp-wide reduction per (token, channel). One token, on the device: 512 ->
-// 1024 2.1 us (5.8 by the tensor cores), 4096 -> 4096 5.1 us (12.4), 4096 ->
-// 16384 8.9 us (22; 67 MB of weight out of L2).
+// one warp-wide reduction per (token, channel). One token, on the device (calls
+// behind each other in a graph): 512 -> 1024 2.0 us (5.2 by the tensor cores),
+// 4096 -> 4096 5.3 us (12.3), 4096 -> 16384 8.9 us (14.2; 67 MB of weight out of
+// L2).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -28,13 +29,13 @@ constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTokens = 16;
 // Codes of all tokens in shared memory. Every CTA makes them all, which costs
-// more than the tensor-core path from there on (8 x 4096 -> 4096: 19 us against
-// 12, -> 512: 15 against 11; 4 x 4096 -> 4096: 8.7 against 12).
+// more than the tensor-core path from there on (8 x 4096 -> 4096: 16.1 us against
+// 12.3, -> 512: 12.4 against 12.2; 4 x 4096 -> 4096: 10.2 against 12.2).
 constexpr int kMaxBytes = 16 * 1024;
 // Nine to sixteen tokens: one launch and no workspace are worth five
 // microseconds of the host, where no SM has more than two CTAs (13 x 1000 ->
-// 520, FP32: 10.3 us a call, 14 by the tensor cores, replayed 8.0 and 6.9; 13 x
-// 1024 -> 16384: 22 and 13.8).
+// 520, FP32: 10.3 us a call, 14 by the tensor cores, but replayed 9.1 and 7.3; 13
+// x 1024 -> 16384 replayed: 21.7 and 8.0).
 constexpr int kManyTokens = 8, kManyChannels = 2 * 148 * 8;
 
 struct FewArgs {
@@ -195,7 +196,7 @@ cudaError_t run(const FewArgs& g, cudaStream_t s) {
 template <typename T, int R>
 cudaError_t run_cpw(const FewArgs& g, int sms, cudaStream_t s) {
     // Four weight rows a warp where that still gives every SM a CTA (one token,
-    // 4096 -> 16384: 8.9 us, 10.5 with two rows; 8 x 512 -> 1024: 3.5 and 3.3).
+    // 4096 -> 16384: 8.9 us, 10.6 with two rows; 8 x 512 -> 1024: 3.0 and 2.9).
     return g.p.cout >= sms * kWarps * 4 ? run<T, R, 4>(g, s) : run<T, R, 2>(g, s);
 }
 

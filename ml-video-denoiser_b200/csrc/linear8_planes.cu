@@ -16,9 +16,10 @@
 //         of all channels x 64 pixels, each filled by two warps.
 // A CTA of four warps takes tiles of 128 pixels of one image, keeps the weight
 // in shared memory and two tiles' loads in flight; several CTAs per SM overlap
-// each other's phases. 32 -> 64 over 1088x1920 takes 92 us (4.3 TB/s); 96 planes
-// of 4 MB cost address translations, 16 images of 272x480 (the same bytes) take
-// 79.
+// each other's phases. 32 -> 64 over 1088x1920 takes 92 us (4.3 TB/s); the same
+// bytes in 16 images of 272x480 take 77: planes that lie megabytes apart cost
+// something (address translations, it seems; no counter was read), and there are
+// two CTA-wide barriers a tile.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 

@@ -20,10 +20,12 @@
 // segments keep their columns' running sums in registers (NT <= 128: 64 a
 // lane). Every wait is bounded.
 //
-// Measured on the device: 8192 x 4096 -> 4096 113 us with its quantisation (2.43
-// POP/s; copies into shared memory, 48 KB a chunk, and the power limit bind),
-// the fusion of 5 cached frames of 522240 x 64 -> 64 62 us (3.9 TB/s; the
-// epilogue's instructions bind).
+// Measured on the device: 8192 x 4096 -> 4096 116 us with its quantisation (2.37
+// POP/s; the product alone 98 us, tensor pipe 75% busy; copies into shared memory,
+// 48 KB a chunk, and the power limit bind), the fusion of 5 cached frames of
+// 522240 x 64 -> 64 61 us (4.0 TB/s; no pipe is full: issue slots 47%, DRAM 40%,
+// so latency binds, of the epilogue's chain of accumulator load, wait and sums
+// in two warps a scheduler).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 

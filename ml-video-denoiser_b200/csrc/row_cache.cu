@@ -2,17 +2,20 @@
 // or consecutive cache rows, and read back through row numbers or page tables
 // (include/denoiser_b200_quant.h has the definition, quant.cuh the arithmetic).
 //
-// Both directions move each byte once and are bound by HBM. A sub-warp of SG
-// lanes takes one group of a row, a lane 8 columns (a 16-byte load of FP16),
-// so the group's maximum is log2(SG) shuffles and nothing passes through
-// shared memory; every lane has the loads of several groups in flight before
-// it uses the first. Rows that begin anywhere (odd column counts, strides and
-// addresses) move between their own boundaries and the vectors' in registers.
-// What is left (cache rows without the vectors' alignment, groups that are wide
-// and odd) takes a warp per group with scalar accesses.
+// Both directions are bound by HBM. A sub-warp of SG lanes takes one group of a
+// row, a lane 8 columns (a 16-byte load of FP16), so each byte moves once, the
+// group's maximum is log2(SG) shuffles and nothing passes through shared memory;
+// every lane has the loads of several groups in flight before it uses the first.
+// Rows that begin anywhere (odd column counts, strides and addresses) move
+// between their own boundaries and the vectors' in registers. Groups of more than
+// 2048 columns take a CTA each (their warps' maxima meet in shared memory), and
+// what is left (cache rows without the vectors' alignment, groups that are wide
+// and odd) a warp per group with scalar accesses; both read what their registers
+// do not hold twice.
 //
-// Measured: 2088960 x 32 FP16 written in 41 us and read back in 35 (both 206 MB;
-// out of L2 in part); five frames of 522240 x 64 read in 93 (512 MB).
+// Measured: 2088960 x 32 FP16 written in 41.5 us and read back in 36 (209 MB each;
+// in turn 79 to 82, out of L2 in part); five frames of 522240 x 64 read in 91 to 93
+// (512 MB).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
