@@ -16,9 +16,17 @@ namespace dnb {
 
 // A tensor map over a [rows][cols] matrix of `esz`-byte elements, row stride
 // ld elements, boxes of box_rows x box_cols swizzled by their width (32, 64 or
-// 128 bytes). Base and row stride are multiples of 16 bytes.
+// 128 bytes). Base and row stride are multiples of 16 bytes; a load reads what
+// lies behind a row up to the next multiple of 16 bytes, and zeros from there on.
 int linear8_map(CUtensorMap* m, CUtensorMapDataType type, int esz, const void* base, int64_t cols, int64_t rows,
                 int64_t ld, int box_cols, int box_rows);
+
+// Whether TMA may store rows of n elements: it cuts what lies behind a row only
+// to 16 bytes, so that a row that is no multiple of them would run over what is
+// beside it.
+inline bool tma_rows(const void* out, int esz, int64_t n, int64_t ld) {
+    return reinterpret_cast<uintptr_t>(out) % 16 == 0 && ld * esz % 16 == 0 && n * esz % 16 == 0 && ld >= n;
+}
 
 // The same over FP16 planes [images][channels][pixels], boxes of box_ch x
 // box_px pixels of one image (64 or 32, swizzled by their 128 or 64 bytes).
@@ -144,7 +152,7 @@ __device__ __forceinline__ uint4 pack16(const float* y, float*) {
     return make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
 }
 
-// Rows that TMA cannot store (address or stride no multiple of 16 bytes): a
+// Rows that TMA cannot store (address, stride or length no multiple of 16 bytes): a
 // warp's block of 32 rows x 32 columns (a lane holds a row's columns c .. c +
 // 31) goes through its 4 KB staging tile and leaves row by row, lanes along the
 // columns. (Stored by each lane along its own row, 2 bytes at a time, 522240 x

@@ -335,9 +335,7 @@ int run(FusedArgs& g, int sms, cudaStream_t s) {
     using S = Shape<PLANES, SG, NT>;
     const ProductArgs& p = g.p;
     const int out_cols = p.gate ? NT / 2 : NT;
-    const bool al16 = !PLANES && reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo * sizeof(T) % 16 == 0 &&
-                      p.ldo >= p.n_out;
-    g.tma_out = al16;
+    g.tma_out = !PLANES && tma_rows(p.out, sizeof(T), p.n_out, p.ldo);
     g.pairs = reinterpret_cast<uintptr_t>(p.out) % 4 == 0 && p.ldo % 2 == 0;
     // Staging rows of 128 bytes, or shorter ones so that every group of four
     // warps has columns to finish.

@@ -545,8 +545,7 @@ int run(TcArgs& g, int sms, cudaStream_t s) {
     g.chunks = (p.seg_c + g.kc - 1) / g.kc;
     g.m_tiles = static_cast<int>((p.rows + kRows - 1) / kRows);
     g.n_tiles = (p.n_out + out_cols - 1) / out_cols;
-    const bool al16 = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.ldo * sizeof(T) % 16 == 0 && p.ldo >= p.n_out;
-    g.tma_out = !p.planes && al16;
+    g.tma_out = !p.planes && tma_rows(p.out, sizeof(T), p.n_out, p.ldo);
     g.pairs = reinterpret_cast<uintptr_t>(p.out) % 4 == 0 && p.ldo % 2 == 0;
     // A weight of one column tile that leaves room for four stages of codes
     // stays in shared memory (5 x 522240 x 64 -> 64: 63 us, 66.5 without; 5 x

@@ -789,6 +789,46 @@ def test_cached_rows_far_from_one(Q, frames, rows, cols, n, gate, y_type):
 
 
 @gpu
+@pytest.mark.parametrize("n", [1, 2, 5, 9, 12, 20, 33, 100, 259, 854])
+@pytest.mark.parametrize("k", [40, 300])
+@pytest.mark.parametrize("y_type", [torch.float16, torch.float32])
+def test_rows_with_something_beside_them(Q, n, k, y_type):
+    """Output rows of any length with an aligned stride: what lies between them,
+    in front of the first and behind the last one stays as it was."""
+    rng = np.random.default_rng(n + k)
+    ld = (n + 7) // 8 * 8 + 8
+    cached = Q.RowCache(2, 150, k)
+    for rows in (5, 74, 150):
+        for gate in (False, True):
+            layer, (qw, sw, b) = make(Q, rng, k, 2 * n if gate else n, gate, True)
+            x = rows_of(rng, rows, k)
+            y, e = qo.product(*qo.quantise(x), qw, sw, b, gate)
+            cached.write(dev(x))
+            for off in (0, 8, 4):
+                def calls():
+                    yield lambda o: layer(dev(x), out=o)
+                    yield lambda o: layer(dev(x.astype(np.float32)), out=o)
+                    yield lambda o: layer.forward_cached(cached, [0], rows=rows, out=o)
+                for call in calls():
+                    flat = torch.full((16 + (rows + 1) * ld,), 9.0, dtype=y_type, device="cuda")
+                    out = flat[16 + off:].as_strided((rows, n), (ld, 1))
+                    call(out)
+                    assert_product(host(out.contiguous()), y, e)
+                    out.fill_(9.0)
+                    assert (host(flat) == 9).all()
+            layer.sync()
+        pair, (qp, sp, bp) = make(Q, rng, 2 * k, n, False, True, segments=2)
+        flat = torch.full(((rows + 1) * ld,), 9.0, dtype=y_type, device="cuda")
+        out = flat.as_strided((rows, n), (ld, 1))
+        pair.forward_cached(cached, [0, 0], rows=rows, out=out)
+        q, s = qo.quantise(x)
+        assert_product(host(out.contiguous()), *qo.product(np.concatenate([q, q], 1), np.concatenate([s, s], 1), qp, sp, bp,
+                                                           False, 2))
+        out.fill_(9.0)
+        assert (host(flat) == 9).all()
+
+
+@gpu
 def test_in_place_calls_are_refused_and_columns_side_by_side_are_not(pkg, Q):
     rng = np.random.default_rng(5)
     layer, (qw, sw, b) = make(Q, rng, 32, 32, False, True)
